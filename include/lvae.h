@@ -416,6 +416,76 @@ int lvae_profile_end(double* total_ms, int* launches);
  * running process calls this to have them read again.  Not for use while other threads are inside the library. */
 int lvae_dev_reload_env(void);
 
+/* ---------------------------------------------------------------------------------------------
+ * Log-likelihood of tokens under a softmax over the vocabulary, straight from the decoder's hidden states: the logits
+ * are never kept.  No single counterpart in the reference, whose decoder materialises [tokens, vocab] logits and calls
+ * cross_entropy on them; its sums over a sentence are the log p(x|z) of iw_log_p_x
+ * (loss_and_optimisation.py:783-794, utils_evaluation.py:176-180).
+ *     l[t,v] = hidden[t] . weight[v] + bias[v];   ll[t] = l[t,y_t] - LSE_v l[t,v]
+ * Element types: LVAE_F32, LVAE_BF16, LVAE_F16 (hidden and weight of one type; bias of any).  Tokens are counted over
+ * three axes with strides of their own (in elements), so a batch cut out of a longer one, or targets shared by all
+ * latent samples of a sentence (stride 0), are passed as they lie; the last axis of hidden and of weight is contiguous.
+ * A token whose target is ignore_index has ll = 0 and no gradient, whatever its hidden state holds (NaN too).  Any other
+ * target outside [0, V) makes ll, and every gradient that the token takes part in, NaN.  A bias of -inf bans a word.
+ * All arithmetic accumulates in float32.
+ * ------------------------------------------------------------------------------------------- */
+#define LVAE_F32 0
+#define LVAE_BF16 1
+#define LVAE_F16 2
+
+typedef struct {
+    const void* hidden;           /* [size0, size1, size2, H] of dtype                       */
+    const void* weight;           /* [V, H] of dtype, rows weight_stride apart               */
+    const void* bias;             /* [V] of bias_dtype, or NULL                              */
+    const int64_t* targets;       /* [size0, size1, size2] class indices                     */
+    int64_t size[3], hidden_stride[3], target_stride[3];
+    int64_t V, weight_stride, ignore_index;
+    int32_t H, dtype, bias_dtype, reserved;
+} lvae_vocab_problem;
+
+/* ll, lse [size0*size1*size2] float32, contiguous; lse (0 for ignored tokens) is what the backward needs and may be
+ * NULL.  Up to LVAE_VOCAB_FEW tokens the weights are streamed once past all tokens in registers; beyond, matrix-core tiles. */
+#define LVAE_VOCAB_FEW 64
+int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* problem, int64_t* out_bytes);
+int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, void* ws, int64_t ws_bytes, void* stream);
+
+/* Backward: g is the upstream gradient on ll, over the token axes with strides g_stride (0: shared), times the device
+ * scalar g_scale if that is given.  d_hidden [tokens, H], d_weight [V, H] (contiguous, dtype) and d_bias [V]
+ * (bias_dtype) may each be NULL.  The gradient of the logits exists a piece of the vocabulary at a time, in the
+ * workspace.  Deterministic. */
+int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* problem, int want_hidden, int want_weight, int want_bias,
+                                      int64_t* out_bytes);
+int lvae_vocab_ll_bwd(const lvae_vocab_problem* problem, const float* lse, const float* g, const int64_t* g_stride,
+                      const float* g_scale, void* d_hidden, void* d_weight, void* d_bias, void* ws, int64_t ws_bytes,
+                      void* stream);
+
+/* loss[0] = factor * sum(ll); with mean != 0, over max(1, tokens whose target is not ignore_index).  loss[1] is the
+ * factor of each ll in it (the g_scale of the backward).  One workgroup, float64. */
+int lvae_vocab_loss_f32(const lvae_vocab_problem* problem, const float* ll, int mean, float factor, float* loss,
+                        void* stream);
+
+/* out[i] = sum_k x[i * len + k], float64 inside; len may be 0. */
+int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Norm of many gradients together, and clipping (what a training step does between backward and update; the reference
+ * leaves it to torch).  list: `count` entries in host memory; each names `n` contiguous elements of device memory.
+ *     norm = (sum |g|^2)^(1/2)  (float64 inside), or max |g| with inf_norm;  c = min(1, max_norm / (norm + 1e-6))
+ * norm is a float32 on the device.  With scale != 0 the gradients are scaled too: in place (dst NULL or src) where c < 1
+ * (nothing is touched where c = 1), else dst = c * src in out_dtype, rounded once.  A norm of NaN makes every result NaN.
+ * An element that is written may belong to one entry only (LVAE_ERR_INVALID otherwise).
+ * ------------------------------------------------------------------------------------------- */
+typedef struct {
+    const void* src;
+    void* dst;
+    int64_t n;
+    int32_t dtype, out_dtype;
+} lvae_grad_entry;
+int lvae_clip_workspace_bytes(int64_t count, int64_t* out_bytes);
+int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int inf_norm, int scale, double max_norm, float* norm,
+                    void* ws, int64_t ws_bytes, void* stream);
+
+
 #ifdef __cplusplus
 }
 #endif

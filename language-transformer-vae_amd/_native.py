@@ -22,6 +22,19 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
 
+# element types of the vocabulary and gradient entry points
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class VocabProblem(ctypes.Structure):
+    """lvae_vocab_problem (include/lvae.h)."""
+    _fields_ = [("hidden", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+                ("targets", ctypes.c_void_p), ("size", _i64 * 3), ("hidden_stride", _i64 * 3),
+                ("target_stride", _i64 * 3), ("V", _i64), ("weight_stride", _i64), ("ignore_index", _i64),
+                ("H", ctypes.c_int32), ("dtype", ctypes.c_int32), ("bias_dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 _SIGNATURES = {
     "lvae_last_error": (ctypes.c_char_p, []),
     "lvae_version": (_int, []),
@@ -107,6 +120,17 @@ _SIGNATURES = {
                                  ctypes.c_void_p]),
     "lvae_kernel_matrix_f32": (_int, [_c_f32p, _c_f32p, _i64, _i64, _int, ctypes.POINTER(_f32), _int, _f32,
                                       _c_f32p, ctypes.c_void_p, _i64, ctypes.c_void_p]),
+    "lvae_vocab_ll_workspace_bytes": (_int, [ctypes.POINTER(VocabProblem), ctypes.POINTER(_i64)]),
+    "lvae_vocab_ll": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.c_void_p, _i64, ctypes.c_void_p]),
+    "lvae_vocab_ll_bwd_workspace_bytes": (_int, [ctypes.POINTER(VocabProblem), _int, _int, _int, ctypes.POINTER(_i64)]),
+    "lvae_vocab_ll_bwd": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.POINTER(_i64), _c_f32p,
+                                 ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _i64,
+                                 ctypes.c_void_p]),
+    "lvae_vocab_loss_f32": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _int, _f32, _c_f32p, ctypes.c_void_p]),
+    "lvae_segment_sum_f32": (_int, [_c_f32p, _i64, _i64, _c_f32p, ctypes.c_void_p]),
+    "lvae_clip_workspace_bytes": (_int, [_i64, ctypes.POINTER(_i64)]),
+    "lvae_clip_grads": (_int, [ctypes.c_void_p, _i64, _int, _int, ctypes.c_double, _c_f32p, ctypes.c_void_p, _i64,
+                               ctypes.c_void_p]),
     "lvae_profile_begin": (_int, [_int]),
     "lvae_profile_end": (_int, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_int)]),
     "lvae_dev_reload_env": (_int, []),

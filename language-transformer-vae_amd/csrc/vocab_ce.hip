@@ -1,0 +1,858 @@
+// Log-likelihood of tokens under the softmax over the vocabulary, from hidden states, with its gradient: the host side
+// of the tile products (vocab_gemm.h) and the kernels around them.
+//
+//   forward   rows -> pack -> tiles (running maximum and sum of each token over 256 words) -> finish
+//   backward  rows -> pack -> per piece of the vocabulary: logits again -> G (16 bits, workspace) -> dHidden += G W,
+//             dWeight = G^T H -> finish
+//   few       up to 64 tokens: every wave streams 16 rows of W past all tokens in registers -> finish
+//
+// `rows` lists the tokens that count, in order, with the place of their hidden state: padding costs nothing in the
+// products, and what a hidden state of padding holds (NaN) meets nothing.
+#include "vocab_gemm.h"
+
+int lvae_vg_launch_bf16(int mode, int narrow, const VgArgs& p, hipStream_t st);
+int lvae_vg_launch_f16(int mode, int narrow, const VgArgs& p, hipStream_t st);
+int lvae_vg_launch_f32(int mode, int narrow, const VgArgs& p, hipStream_t st);
+
+namespace {
+
+// G in 16 bits is kept relative to the largest upstream gradient: the -1 of a target is then exact (with the 1 / n of a
+// mean inside, all targets would share one rounding error), and fp16, with the largest at 2^14, holds what is 2^-28 of it
+constexpr float F16_G_SCALE = 16384.f;
+
+struct Axes {
+    int64_t size[3], stride[3];
+};
+__device__ __forceinline__ int64_t at_axes(const Axes& a, int64_t t) {
+    const int64_t k = t % a.size[2], r = t / a.size[2];
+    return (r / a.size[1]) * a.stride[0] + (r % a.size[1]) * a.stride[1] + k * a.stride[2];
+}
+
+template <int DT> __device__ __forceinline__ float load_as_float(const void* p, int64_t i) {
+    if constexpr (DT == LVAE_F32) return ((const float*)p)[i];
+    else if constexpr (DT == LVAE_BF16) return vg_bf16(((const uint16_t*)p)[i]);
+    else return (float)((const _Float16*)p)[i];
+}
+__device__ __forceinline__ float load_any(const void* p, int64_t i, int dt) {
+    return dt == LVAE_F32 ? load_as_float<LVAE_F32>(p, i)
+         : dt == LVAE_BF16 ? load_as_float<LVAE_BF16>(p, i) : load_as_float<LVAE_F16>(p, i);
+}
+__device__ __forceinline__ void store_any(void* p, int64_t i, float x, int dt) {
+    if (dt == LVAE_F32) ((float*)p)[i] = x;
+    else ((uint16_t*)p)[i] = dt == LVAE_BF16 ? vg_round<LVAE_BF16>(x) : vg_round<LVAE_F16>(x);
+}
+
+__device__ __forceinline__ int block_sum_int(int v, int* red) {          // 1024 threads
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    int s = 0;
+    for (int w = 0; w < 16; ++w) s += red[w];
+    return s;
+}
+
+struct RowsArgs {
+    Axes hid, tgt, g;
+    const int64_t* targets;
+    const float* lse;           // backward: LSE of every token
+    const float* gy;            // backward: upstream gradient
+    const float* g_scale;
+    int64_t T, V, ignore;
+    float g_scale_to;           // what the largest |g| becomes; 0: gradients stay as they are
+    int64_t* off;               // place of the kept token's hidden state
+    int *tok, *tgt_of, *inv;    // its number, its target; and back (-1: not kept)
+    float *lse_of, *gy_of, *unscale;
+    float *ll, *lse_out;        // forward: zeros for tokens that do not count
+    int* n_rows;
+};
+
+// One workgroup per 1,024 tokens.  Each counts the kept tokens before its own by itself (targets are 8 bytes a token
+// and stay in L2; at 65,536 tokens the last workgroup reads 512 KB) instead of a second launch for the prefix.
+__global__ __launch_bounds__(1024) void rows_kernel(RowsArgs p) {
+    __shared__ int red[16];
+    __shared__ float redf[16];
+    const int64_t first = (int64_t)blockIdx.x * 1024;
+    int before = 0;
+    for (int64_t u = threadIdx.x; u < first; u += 1024) before += p.targets[at_axes(p.tgt, u)] != p.ignore;
+    before = block_sum_int(before, red);
+    float factor = 1.f;
+    if (p.gy_of && p.g_scale) factor = p.g_scale[0];
+    float norm = 1.f;
+    if (p.gy_of && p.g_scale_to > 0.f) {                              // the same in every workgroup
+        float top = 0.f;
+        for (int64_t u = threadIdx.x; u < p.T; u += 1024)
+            if (p.targets[at_axes(p.tgt, u)] != p.ignore) {
+                const float a = fabsf(p.gy[at_axes(p.g, u)] * factor);
+                top = a > top ? a : top;
+            }
+        top = wave_max(top);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) redf[threadIdx.x >> 6] = top;
+        __syncthreads();
+        for (int w = 0; w < 16; ++w) norm = w == 0 ? redf[0] : fmaxf(norm, redf[w]);
+        if (!(norm > 0.f) || !(norm < INFINITY)) norm = p.g_scale_to;      // nothing to keep in range: a factor of 1
+        if (blockIdx.x == 0 && threadIdx.x == 0) p.unscale[0] = norm / p.g_scale_to;
+    }
+    const int64_t t = first + threadIdx.x;
+    const int64_t y = t < p.T ? p.targets[at_axes(p.tgt, t)] : p.ignore;
+    const bool keep = t < p.T && y != p.ignore;
+    const unsigned long long mask = __ballot(keep);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __syncthreads();
+    if (lane == 0) red[wave] = __popcll(mask);
+    __syncthreads();
+    int64_t j = before + __popcll(mask & ((1ull << lane) - 1));
+    int all = 0;
+    for (int w = 0; w < 16; ++w) {
+        if (w < wave) j += red[w];
+        all += red[w];
+    }
+    if (t < p.T) {
+        if (p.inv) p.inv[t] = keep ? (int)j : -1;
+        if (keep) {
+            p.off[j] = at_axes(p.hid, t);
+            p.tok[j] = (int)t;
+            p.tgt_of[j] = y >= 0 && y < p.V ? (int)y : -2;
+            if (p.lse_of) {
+                p.lse_of[j] = p.lse[t];
+                const float g = -(p.gy[at_axes(p.g, t)] * factor);     // on the negative log-likelihood: G = (softmax - onehot) g
+                p.gy_of[j] = p.g_scale_to > 0.f ? (g / norm) * p.g_scale_to : g;
+            }
+        } else {
+            if (p.ll) p.ll[t] = 0.f;
+            if (p.lse_out) p.lse_out[t] = 0.f;
+        }
+    }
+    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) p.n_rows[0] = before + all;
+}
+
+// Rows of hidden (listed, zeros behind the last up to a whole tile) or of W (strided) as the tile products read them:
+// Kp columns, zero behind H; float32 as three limb planes.  One wave per row.
+template <int DT> __global__ __launch_bounds__(256) void pack_kernel(const void* src, const int64_t* off, int64_t stride,
+                                                                     const int* n_rows, int64_t rows, int H, int Kp,
+                                                                     uint16_t* out, int64_t plane) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= rows) return;
+    const int lane = threadIdx.x & 63;
+    bool there = true;
+    if (off) {
+        const int64_t n = n_rows[0];
+        if (r >= (n + 255) / 256 * 256) return;
+        there = r < n;
+    }
+    const int64_t base = there ? (off ? off[r] : r * stride) : 0;
+    uint16_t* o = out + r * Kp;
+    constexpr int SZ = DT == LVAE_F32 ? 4 : 2;
+    const bool vec = ((((uintptr_t)src + base * SZ) & 15) == 0) && H % 8 == 0;       // of this row
+    for (int k = lane * 8; k < Kp; k += 512) {
+        float x[8];
+        s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if constexpr (DT == LVAE_F32) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+            if (there && vec && k < H) {
+                const f32x4 a = *(const f32x4*)((const float*)src + base + k), b = *(const f32x4*)((const float*)src + base + k + 4);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
+            } else if (there) {
+                for (int e = 0; e < 8; ++e) if (k + e < H) x[e] = ((const float*)src)[base + k + e];
+            }
+            s16x8 w[3];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                uint16_t l[3];
+                vg_limbs(x[e], l);
+                w[0][e] = l[0]; w[1][e] = l[1]; w[2][e] = l[2];
+            }
+#pragma unroll
+            for (int l = 0; l < 3; ++l) *(s16x8*)(o + l * plane + k) = w[l];
+        } else {
+            if (there && vec && k < H) v = *(const s16x8*)((const uint16_t*)src + base + k);
+            else if (there) {
+                for (int e = 0; e < 8; ++e) if (k + e < H) v[e] = ((const uint16_t*)src)[base + k + e];
+            }
+            *(s16x8*)(o + k) = v;
+        }
+    }
+}
+
+// bias in float32, -inf behind the vocabulary: what the tiles add, so that no word beyond the last can count
+__global__ __launch_bounds__(256) void bias_kernel(const void* bias, int dt, int64_t V, int64_t Vpad, float* out) {
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (v < Vpad) out[v] = v >= V ? -INFINITY : bias ? load_any(bias, v, dt) : 0.f;
+}
+
+__device__ __forceinline__ float2 merge_lse(float2 a, float2 b) {
+    const float top = fmaxf(a.x, b.x), ref = top == -INFINITY ? 0.f : top;
+    return make_float2(top, a.y * lvae_exp2((a.x - ref) * LVAE_LOG2E) + b.y * lvae_exp2((b.x - ref) * LVAE_LOG2E));
+}
+
+// LSE of each kept token from its partials [tiles][ldp]; 32 tokens a workgroup, 8 threads a token
+__global__ __launch_bounds__(256) void finish_kernel(const float2* part, int tiles, int64_t ldp, const float* picked,
+                                                     const int* tok, const int* tgt, const int* n_rows, float* ll,
+                                                     float* lse) {
+    __shared__ float2 red[8][32];
+    const int64_t j = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int g = threadIdx.x >> 5;
+    const int64_t n = n_rows[0];
+    float2 x = make_float2(-INFINITY, 0.f);
+    if (j < n)
+        for (int i = g; i < tiles; i += 8) x = merge_lse(x, part[(int64_t)i * ldp + j]);
+    red[g][threadIdx.x & 31] = x;
+    __syncthreads();
+    if (g == 0 && j < n) {
+        for (int i = 1; i < 8; ++i) x = merge_lse(x, red[i][threadIdx.x]);
+        float l = x.x + logf(x.y);
+        const bool bad = tgt[j] < 0;
+        if (bad) l = NAN;
+        ll[tok[j]] = bad ? NAN : picked[j] - l;
+        if (lse) lse[tok[j]] = l;
+    }
+}
+
+// ---- few tokens: W streamed once -------------------------------------------------------------------------------
+// A wave owns 16 words; its A operand comes from memory in registers (a lane reads 32 consecutive bytes of its word's
+// row: 128 bytes a row and step), the tokens' rows are its B operand.  The order of the summed index inside a step is
+// the lanes' own (the same on both sides).  Bound by the read of W.
+template <int DT> struct FewStep {
+    static constexpr int K = DT == LVAE_F32 ? 32 : 64, LANE = K / 4;       // elements a step, and a lane's share
+};
+// a lane's share of a row at k, zeros behind H
+template <int DT, bool ALIGNED> __device__ __forceinline__ void few_load(const void* row, int k, int H, f32x4 out[2]) {
+    constexpr int SZ = DT == LVAE_F32 ? 4 : 2, E = 16 / SZ;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int at = k + h * E;
+        out[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (ALIGNED) {
+            // behind H the row's first piece is read and dropped: no branch, so that the loads of a step go out together
+            const f32x4 v = *(const f32x4*)((const char*)row + (at < H ? at : 0) * SZ);
+            out[h] = at < H ? v : out[h];
+        } else if constexpr (DT == LVAE_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (at + e < H) out[h][e] = ((const float*)row)[at + e];
+        } else {
+            s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) if (at + e < H) v[e] = ((const uint16_t*)row)[at + e];
+            out[h] = __builtin_bit_cast(f32x4, v);
+        }
+    }
+}
+template <int DT> __device__ __forceinline__ f32x4 few_mma(const f32x4 a[2], const f32x4 b[2], f32x4 c) {
+    if constexpr (DT == LVAE_F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[h][e], b[h][e], c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) c = vg_mma<DT>(__builtin_bit_cast(s16x8, a[h]), __builtin_bit_cast(s16x8, b[h]), c);
+    }
+    return c;
+}
+
+struct FewArgs {
+    const void *hidden, *weight, *bias;
+    const int64_t* targets;
+    Axes hid, tgt;
+    int64_t V, wstride;
+    int T, H, bias_dtype, blocks;
+    float2* part;               // [T][blocks]
+    float* picked;              // [T]
+};
+
+template <int DT, int NT, bool ALIGNED> __global__ __launch_bounds__(256) void few_kernel(FewArgs p) {
+    constexpr int SZ = DT == LVAE_F32 ? 4 : 2, KS = FewStep<DT>::K, KL = FewStep<DT>::LANE;
+    __shared__ float2 red[4][NT * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mp = lane & 15, g4 = lane >> 4;
+    const int64_t vw = ((int64_t)blockIdx.x * 4 + wave) * 16;
+    const char* wrow = (const char*)p.weight + min(vw + mp, p.V - 1) * p.wstride * SZ;
+    const char* hrow[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) hrow[n] = (const char*)p.hidden + at_axes(p.hid, min(n * 16 + mp, p.T - 1)) * SZ;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    constexpr int U = ALIGNED ? 4 : 1;      // steps whose loads of W are in flight together
+    for (int k0 = 0; k0 < p.H; k0 += U * KS) {
+        f32x4 a[U][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) few_load<DT, ALIGNED>(wrow, k0 + u * KS + g4 * KL, p.H, a[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                f32x4 b[2];
+                few_load<DT, ALIGNED>(hrow[n], k0 + u * KS + g4 * KL, p.H, b);
+                acc[n] = few_mma<DT>(a[u], b, acc[n]);
+            }
+    }
+    const int64_t v0 = vw + g4 * 4;
+    float bias[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bias[r] = v0 + r >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v0 + r, p.bias_dtype) : 0.f;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int t = n * 16 + mp;
+        const int64_t rel = t < p.T ? p.targets[at_axes(p.tgt, t)] - v0 : -1;
+        float x[4], top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            x[r] = acc[n][r] + bias[r];
+            if (v0 + r >= p.V) x[r] = -INFINITY;
+            if (rel == r && v0 + r < p.V) p.picked[t] = x[r];
+            top = fmaxf(top, x[r]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += lvae_exp2((x[r] - ref) * LVAE_LOG2E);
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (g4 == 0) red[wave][t] = make_float2(top, sum);
+    }
+    __syncthreads();
+    for (int t = threadIdx.x; t < p.T; t += 256) {
+        float2 x = red[0][t];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) x = merge_lse(x, red[w][t]);
+        p.part[(int64_t)t * p.blocks + blockIdx.x] = x;
+    }
+}
+
+__global__ __launch_bounds__(256) void few_finish_kernel(const float2* part, int blocks, const float* picked,
+                                                         const int64_t* targets, Axes tgt, int64_t V, int64_t ignore,
+                                                         float* ll, float* lse) {
+    __shared__ float2 red[4];
+    const int t = blockIdx.x;
+    const int64_t y = targets[at_axes(tgt, t)];
+    if (y == ignore) {
+        if (threadIdx.x == 0) {
+            ll[t] = 0.f;
+            if (lse) lse[t] = 0.f;
+        }
+        return;
+    }
+    float2 x = make_float2(-INFINITY, 0.f);
+    for (int i = threadIdx.x; i < blocks; i += 256) x = merge_lse(x, part[(int64_t)t * blocks + i]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = merge_lse(x, make_float2(__shfl_xor(x.x, o, 64), __shfl_xor(x.y, o, 64)));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 4; ++w) x = merge_lse(x, red[w]);
+        float l = x.x + logf(x.y);
+        const bool bad = y < 0 || y >= V;
+        if (bad) l = NAN;
+        ll[t] = bad ? NAN : picked[t] - l;
+        if (lse) lse[t] = l;
+    }
+}
+
+// ---- backward: sums of the partial products ----------------------------------------------------------------------
+// d_hidden of every token: the slabs of its row, in order; zeros where the token does not count
+__global__ __launch_bounds__(256) void dhidden_kernel(const float* slab, int splits, int64_t slab_stride, int64_t ld,
+                                                      const int* inv, int64_t T, int H, const float* unscale, void* out,
+                                                      int dt) {
+    const int per = (H + 3) / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= T * per) return;
+    const int64_t t = i / per;
+    const int h = (int)(i - t * per) * 4;
+    const int j = inv[t];
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (j >= 0) {
+        for (int s = 0; s < splits; ++s) x += *(const f32x4*)(slab + s * slab_stride + j * ld + h);
+        if (unscale) x *= unscale[0];
+    }
+    const int64_t o = t * H + h;
+    if (H % 4 == 0 && dt == LVAE_F32) { *(f32x4*)((float*)out + o) = x; return; }
+    if (H % 4 == 0) {
+        s16x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = dt == LVAE_BF16 ? vg_round<LVAE_BF16>(x[e]) : vg_round<LVAE_F16>(x[e]);
+        *(s16x4*)((uint16_t*)out + o) = v;
+        return;
+    }
+    for (int e = 0; e < 4; ++e) if (h + e < H) store_any(out, o + e, x[e], dt);
+}
+
+// rows [0, rows) of the split weight gradient
+__global__ __launch_bounds__(256) void dweight_kernel(const float* slab, int splits, int64_t slab_stride, int64_t ld,
+                                                      int64_t rows, int H, const float* unscale, void* out, int dt) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= rows * H) return;
+    const int64_t v = i / H;
+    const int h = (int)(i - v * H);
+    float x = 0.f;
+    for (int s = 0; s < splits; ++s) x += slab[s * slab_stride + v * ld + h];
+    store_any(out, i, unscale ? x * unscale[0] : x, dt);
+}
+
+// d_bias of a piece: the partial column sums of the tiles that hold kept tokens
+__global__ __launch_bounds__(256) void dbias_kernel(const float* part, int64_t ld, int per_tile, int tile_rows, const int* n_rows,
+                                                    int64_t rows, const float* unscale, void* out, int dt, int64_t v0) {
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (v >= rows) return;
+    const int n = (n_rows[0] + tile_rows - 1) / tile_rows * per_tile;
+    double x = 0.0;
+    for (int i = 0; i < n; ++i) x += part[(int64_t)i * ld + v];
+    const float f = (float)x;
+    store_any(out, v0 + v, unscale ? f * unscale[0] : f, dt);
+}
+
+__global__ __launch_bounds__(256) void segment_sum_kernel(const float* x, int64_t n, int64_t len, float* out) {
+    const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (s >= n) return;
+    double a = 0.0;
+    for (int64_t i = threadIdx.x & 63; i < len; i += 64) a += x[s * len + i];
+    a = wave_sum_d(a);
+    if ((threadIdx.x & 63) == 0) out[s] = (float)a;
+}
+
+__global__ __launch_bounds__(1024) void loss_kernel(const int64_t* targets, Axes tgt, int64_t T, int64_t ignore,
+                                                    const float* ll, int mean, float factor, float* out) {
+    __shared__ double red[16];
+    __shared__ int redi[16];
+    double a = 0.0;
+    int c = 0;
+    for (int64_t t = threadIdx.x; t < T; t += 1024) {
+        a += ll[t];
+        if (mean) c += targets[at_axes(tgt, t)] != ignore;
+    }
+    a = wave_sum_d(a);
+    c = block_sum_int(c, redi);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double s = 0.0;
+        for (int w = 0; w < 16; ++w) s += red[w];
+        const double f = (double)factor / (mean ? (double)max(1, c) : 1.0);
+        out[0] = (float)(s * f);
+        out[1] = (float)f;
+    }
+}
+
+// ---- the plan ------------------------------------------------------------------------------------------------------
+struct Plan {
+    int64_t T, Tpad, V, Vpad, H, Kp;
+    int planes;
+    bool few, direct_w;
+    int narrow, tile_n;
+    int64_t piece;              // words of the vocabulary a time (backward)
+    int splits_h, splits_w;
+    // offsets into the workspace, bytes
+    int64_t off, tok, tgt, inv, lse, gy, head, bias, hpack, wpack, part, picked, g, slab, slab_w, dbias, bytes;
+    int64_t few_blocks;
+};
+
+int check_problem(const lvae_vocab_problem* q, Plan* pl) {
+    LVAE_CHECK_ARG(q, "problem must be non-NULL");
+    LVAE_CHECK_ARG(q->dtype >= LVAE_F32 && q->dtype <= LVAE_F16, "unknown dtype %d", q->dtype);
+    LVAE_CHECK_ARG(q->bias_dtype >= LVAE_F32 && q->bias_dtype <= LVAE_F16, "unknown bias_dtype %d", q->bias_dtype);
+    LVAE_CHECK_ARG(q->V >= 1 && q->V < (1ll << 31) - 512 && q->H >= 1 && q->H <= 65536, "bad shape: V=%lld H=%d (1 <= H <= 65536)",
+                   (long long)q->V, q->H);
+    int64_t T = 1;
+    for (int i = 0; i < 3; ++i) {
+        LVAE_CHECK_ARG(q->size[i] >= 1 && q->size[i] < (1ll << 31), "bad shape: size[%d]=%lld", i, (long long)q->size[i]);
+        T *= q->size[i];
+        LVAE_CHECK_ARG(T < (1ll << 31) - 512, "too many tokens");
+    }
+    LVAE_CHECK_ARG(q->weight_stride >= q->H, "weight_stride %lld < H %d", (long long)q->weight_stride, q->H);
+    pl->T = T;
+    pl->Tpad = lvae_round_up(T, 256);
+    pl->V = q->V;
+    pl->Vpad = lvae_round_up(q->V, 256);
+    pl->H = q->H;
+    pl->Kp = lvae_round_up(q->H, VG_BK);
+    pl->planes = q->dtype == LVAE_F32 ? 3 : 1;
+    // the tiles read W where it lies if its rows are whole 128-byte slices on 16-byte boundaries; else a padded copy
+    pl->direct_w = q->dtype != LVAE_F32 && q->H % VG_BK == 0 && q->weight_stride % 8 == 0 &&
+                   q->weight_stride < (1 << 22) && ((uintptr_t)q->weight & 15) == 0;
+    // 64-token tiles where 256-token ones would be mostly empty
+    pl->narrow = T <= 128;
+    pl->tile_n = pl->narrow ? 64 : 256;
+    return LVAE_OK;
+}
+
+int64_t take(int64_t& at, int64_t bytes) {
+    const int64_t o = at;
+    at += lvae_round_up(bytes, 256);
+    return o;
+}
+
+void plan_common(Plan* pl) {
+    int64_t at = 0;
+    pl->head = take(at, 256);                            // n_rows, unscale
+    pl->off = take(at, pl->Tpad * 8);
+    pl->tok = take(at, pl->Tpad * 4);
+    pl->tgt = take(at, pl->Tpad * 4);
+    pl->bias = take(at, pl->Vpad * 4);
+    pl->hpack = take(at, pl->planes * pl->Tpad * pl->Kp * 2);
+    pl->wpack = pl->direct_w ? 0 : take(at, pl->planes * pl->V * pl->Kp * 2);
+    pl->bytes = at;
+}
+
+void plan_forward(Plan* pl) {
+    pl->few = pl->T <= LVAE_VOCAB_FEW;
+    if (pl->few) {
+        int64_t at = 0;
+        pl->few_blocks = lvae_ceil_div(pl->V, 64);
+        pl->part = take(at, pl->T * pl->few_blocks * 8);
+        pl->picked = take(at, pl->T * 4);
+        pl->bytes = at;
+        return;
+    }
+    plan_common(pl);
+    int64_t at = pl->bytes;
+    pl->part = take(at, pl->Vpad / 256 * pl->Tpad * 8);
+    pl->picked = take(at, pl->Tpad * 4);
+    pl->bytes = at;
+}
+
+void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
+    plan_common(pl);
+    int64_t at = pl->bytes;
+    pl->inv = take(at, pl->T * 4);
+    pl->lse = take(at, pl->Tpad * 4);
+    pl->gy = take(at, pl->Tpad * 4);
+    // pieces of the vocabulary: G of one piece takes at most 512 MiB, and every piece is as large as the others
+    const int64_t per_word = pl->Tpad * pl->planes * 2;
+    int64_t piece = (512ll << 20) / per_word / 256 * 256;
+    if (piece < 1024) piece = 1024;
+    if (piece > 32768) piece = 32768;
+    const int64_t pieces = lvae_ceil_div(pl->Vpad, piece);
+    pl->piece = lvae_round_up(lvae_ceil_div(pl->V, pieces), 256);
+    pl->g = take(at, pl->planes * pl->Tpad * pl->piece * 2);
+    const int64_t th = lvae_ceil_div(pl->H, 256);
+    // few output tiles and a long sum: the sum is split so that the launch fills the 256 CUs
+    const int64_t tiles_h = th * lvae_ceil_div(pl->T, pl->tile_n), tiles_w = th * lvae_ceil_div(pl->piece, 256);
+    pl->splits_h = (int)lvae_ceil_div(256, tiles_h);
+    const int64_t most_h = lvae_ceil_div(pl->piece, 512);
+    if (pl->splits_h > most_h) pl->splits_h = (int)most_h;
+    if (pl->splits_h > 32) pl->splits_h = 32;
+    pl->splits_w = 1;
+    if (tiles_w <= 128 && pl->T >= 1024) {
+        pl->splits_w = (int)(256 / tiles_w);
+        const int64_t most_w = pl->T / 512;
+        if (pl->splits_w > most_w) pl->splits_w = (int)most_w;
+        if (pl->splits_w > 32) pl->splits_w = 32;
+    }
+    pl->slab = want_h ? take(at, pl->splits_h * pl->Tpad * pl->Kp * 4) : 0;
+    pl->slab_w = want_w && pl->splits_w > 1 ? take(at, pl->splits_w * pl->piece * pl->Kp * 4) : 0;
+    pl->dbias = want_b ? take(at, pl->Tpad / pl->tile_n * 4 * pl->piece * 4) : 0;
+    pl->bytes = at;
+}
+
+Axes axes_of(const lvae_vocab_problem* q, const int64_t* stride) {
+    Axes a;
+    for (int i = 0; i < 3; ++i) {
+        a.size[i] = q->size[i];
+        a.stride[i] = stride[i];
+    }
+    return a;
+}
+
+int check_ws(const Plan& pl, void* ws, int64_t ws_bytes) {
+    if (!ws) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace is NULL (%lld bytes needed)", (long long)pl.bytes);
+    if ((uintptr_t)ws & 255) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+    if (ws_bytes < pl.bytes)
+        return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace too small: %lld < %lld bytes", (long long)ws_bytes, (long long)pl.bytes);
+    return LVAE_OK;
+}
+
+int check_data(const lvae_vocab_problem* q) {
+    LVAE_CHECK_ARG(q->hidden && q->weight && q->targets, "hidden, weight and targets must be non-NULL");
+    return LVAE_OK;
+}
+
+int launch_tiles(int dtype, int mode, int narrow, const VgArgs& a, hipStream_t st) {
+    return dtype == LVAE_F32 ? lvae_vg_launch_f32(mode, narrow, a, st)
+         : dtype == LVAE_BF16 ? lvae_vg_launch_bf16(mode, narrow, a, st) : lvae_vg_launch_f16(mode, narrow, a, st);
+}
+
+int launch_pack(int dtype, const void* src, const int64_t* off, int64_t stride, const int* n_rows, int64_t rows, int H, int Kp,
+                uint16_t* out, hipStream_t st) {
+    const dim3 grid((unsigned)lvae_ceil_div(rows, 4));
+    const int64_t plane = rows * Kp;
+    if (dtype == LVAE_F32) pack_kernel<LVAE_F32><<<grid, 256, 0, st>>>(src, off, stride, n_rows, rows, H, Kp, out, plane);
+    else pack_kernel<LVAE_BF16><<<grid, 256, 0, st>>>(src, off, stride, n_rows, rows, H, Kp, out, plane);
+    LVAE_LAUNCH_CHECK();
+    return LVAE_OK;
+}
+
+#define RUN(call)                    \
+    do {                             \
+        const int rc__ = (call);     \
+        if (rc__ != LVAE_OK) return rc__; \
+    } while (0)
+
+// rows, packed hidden, packed weight and bias; fills the operands of the logits' product
+int launch_operands(const lvae_vocab_problem* q, const Plan& pl, const RowsArgs& rows, char* ws, VgArgs* a, hipStream_t st) {
+    rows_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 1024)), 1024, 0, st>>>(rows);
+    LVAE_LAUNCH_CHECK();
+    uint16_t* hp = (uint16_t*)(ws + pl.hpack);
+    RUN(launch_pack(q->dtype, q->hidden, rows.off, 0, rows.n_rows, pl.Tpad, (int)pl.H, (int)pl.Kp, hp, st));
+    float* bias = (float*)(ws + pl.bias);
+    bias_kernel<<<dim3((unsigned)(pl.Vpad / 256)), 256, 0, st>>>(q->bias, q->bias_dtype, pl.V, pl.Vpad, bias);
+    LVAE_LAUNCH_CHECK();
+    *a = VgArgs{};
+    a->a = (const uint16_t*)q->weight;
+    a->lda = q->weight_stride;
+    a->a_cols = pl.H;
+    if (!pl.direct_w) {
+        uint16_t* wp = (uint16_t*)(ws + pl.wpack);
+        RUN(launch_pack(q->dtype, q->weight, nullptr, q->weight_stride, nullptr, pl.V, (int)pl.H, (int)pl.Kp, wp, st));
+        a->a = wp;
+        a->lda = a->a_cols = pl.Kp;
+        a->plane_a = pl.V * pl.Kp;
+    }
+    a->b = hp;
+    a->ldb = pl.Kp;
+    a->plane_b = pl.Tpad * pl.Kp;
+    a->N = pl.T;
+    a->K = pl.Kp;
+    a->n_rows = rows.n_rows;
+    a->tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_n);
+    a->splits = 1;
+    a->bias = bias;
+    a->tgt = rows.tgt_of;
+    return LVAE_OK;
+}
+
+RowsArgs rows_args(const lvae_vocab_problem* q, const Plan& pl, char* ws) {
+    RowsArgs r = {};
+    r.hid = axes_of(q, q->hidden_stride);
+    r.tgt = axes_of(q, q->target_stride);
+    r.targets = q->targets;
+    r.T = pl.T;
+    r.V = pl.V;
+    r.ignore = q->ignore_index;
+    r.off = (int64_t*)(ws + pl.off);
+    r.tok = (int*)(ws + pl.tok);
+    r.tgt_of = (int*)(ws + pl.tgt);
+    r.n_rows = (int*)(ws + pl.head);
+    r.unscale = (float*)(ws + pl.head + 64);
+    return r;
+}
+
+template <int DT, int NT> void start_few(const FewArgs& f, bool aligned, hipStream_t st) {
+    if (aligned) few_kernel<DT, NT, true><<<dim3((unsigned)f.blocks), 256, 0, st>>>(f);
+    else few_kernel<DT, NT, false><<<dim3((unsigned)f.blocks), 256, 0, st>>>(f);
+}
+template <int DT> void start_few_n(const FewArgs& f, bool aligned, hipStream_t st) {
+    if (f.T <= 16) start_few<DT, 1>(f, aligned, st);
+    else if (f.T <= 32) start_few<DT, 2>(f, aligned, st);
+    else start_few<DT, 4>(f, aligned, st);
+}
+
+}  // namespace
+
+extern "C" int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* q, int64_t* out_bytes) {
+    Plan pl = {};
+    LVAE_CHECK_ARG(out_bytes, "out_bytes must be non-NULL");
+    RUN(check_problem(q, &pl));
+    plan_forward(&pl);
+    *out_bytes = pl.bytes;
+    return LVAE_OK;
+}
+
+extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, void* wsv, int64_t ws_bytes, void* stream) {
+    Plan pl = {};
+    RUN(check_problem(q, &pl));
+    RUN(check_data(q));
+    LVAE_CHECK_ARG(ll, "ll must be non-NULL");
+    plan_forward(&pl);
+    RUN(check_ws(pl, wsv, ws_bytes));
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)wsv;
+    float2* part = (float2*)(ws + pl.part);
+    float* picked = (float*)(ws + pl.picked);
+    if (pl.few) {
+        FewArgs f = {};
+        f.hidden = q->hidden;
+        f.weight = q->weight;
+        f.bias = q->bias;
+        f.targets = q->targets;
+        f.hid = axes_of(q, q->hidden_stride);
+        f.tgt = axes_of(q, q->target_stride);
+        f.V = pl.V;
+        f.wstride = q->weight_stride;
+        f.T = (int)pl.T;
+        f.H = q->H;
+        f.bias_dtype = q->bias_dtype;
+        f.blocks = (int)pl.few_blocks;
+        f.part = part;
+        f.picked = picked;
+        const int per16 = q->dtype == LVAE_F32 ? 4 : 8;          // elements of 16 bytes
+        bool aligned = (((uintptr_t)q->hidden | (uintptr_t)q->weight) & 15) == 0 && q->H % per16 == 0 && q->weight_stride % per16 == 0;
+        for (int i = 0; i < 3; ++i) aligned = aligned && q->hidden_stride[i] % per16 == 0;
+        if (q->dtype == LVAE_F32) start_few_n<LVAE_F32>(f, aligned, st);
+        else if (q->dtype == LVAE_BF16) start_few_n<LVAE_BF16>(f, aligned, st);
+        else start_few_n<LVAE_F16>(f, aligned, st);
+        LVAE_LAUNCH_CHECK();
+        few_finish_kernel<<<dim3((unsigned)pl.T), 256, 0, st>>>(part, f.blocks, picked, q->targets, f.tgt, pl.V, q->ignore_index, ll, lse);
+        LVAE_LAUNCH_CHECK();
+        return LVAE_OK;
+    }
+    RowsArgs rows = rows_args(q, pl, ws);
+    rows.ll = ll;
+    rows.lse_out = lse;
+    VgArgs a;
+    RUN(launch_operands(q, pl, rows, ws, &a, st));
+    a.M = pl.V;
+    a.tiles_m = (int)(pl.Vpad / 256);
+    a.part = part;
+    a.ldp = pl.Tpad;
+    a.picked = picked;
+    RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow, a, st));
+    finish_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 32)), 256, 0, st>>>(part, a.tiles_m, pl.Tpad, picked, rows.tok, rows.tgt_of,
+                                                                          rows.n_rows, ll, lse);
+    LVAE_LAUNCH_CHECK();
+    return LVAE_OK;
+}
+
+extern "C" int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* q, int want_hidden, int want_weight, int want_bias,
+                                                 int64_t* out_bytes) {
+    Plan pl = {};
+    LVAE_CHECK_ARG(out_bytes, "out_bytes must be non-NULL");
+    RUN(check_problem(q, &pl));
+    plan_backward(&pl, want_hidden != 0, want_weight != 0, want_bias != 0);
+    *out_bytes = pl.bytes;
+    return LVAE_OK;
+}
+
+extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, const float* g, const int64_t* g_stride,
+                                 const float* g_scale, void* d_hidden, void* d_weight, void* d_bias, void* wsv,
+                                 int64_t ws_bytes, void* stream) {
+    Plan pl = {};
+    RUN(check_problem(q, &pl));
+    RUN(check_data(q));
+    LVAE_CHECK_ARG(lse && g && g_stride, "lse, g and g_stride must be non-NULL");
+    LVAE_CHECK_ARG(d_hidden || d_weight || d_bias, "no gradient asked for");
+    plan_backward(&pl, d_hidden != nullptr, d_weight != nullptr, d_bias != nullptr);
+    RUN(check_ws(pl, wsv, ws_bytes));
+    hipStream_t st = (hipStream_t)stream;
+    char* ws = (char*)wsv;
+    RowsArgs rows = rows_args(q, pl, ws);
+    rows.g = axes_of(q, g_stride);
+    rows.lse = lse;
+    rows.gy = g;
+    rows.g_scale = g_scale;
+    rows.g_scale_to = q->dtype == LVAE_F16 ? F16_G_SCALE : q->dtype == LVAE_BF16 ? 1.f : 0.f;
+    rows.inv = (int*)(ws + pl.inv);
+    rows.lse_of = (float*)(ws + pl.lse);
+    rows.gy_of = (float*)(ws + pl.gy);
+    VgArgs a;
+    RUN(launch_operands(q, pl, rows, ws, &a, st));
+    const float* unscale = rows.g_scale_to > 0.f ? rows.unscale : nullptr;
+    const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2, th = lvae_ceil_div(pl.H, 256);
+    const uint16_t* w0 = a.a;
+    const uint16_t* hp = a.b;
+    uint16_t* gbuf = (uint16_t*)(ws + pl.g);
+    const int64_t plane_g = pl.Tpad * pl.piece;
+    const int waves_n = pl.narrow ? 2 : 4;
+    for (int64_t v0 = 0; v0 < pl.V; v0 += pl.piece) {
+        const int64_t words = pl.V - v0 < pl.piece ? pl.V - v0 : pl.piece;
+        VgArgs l = a;                                    // G of this piece
+        l.a = w0 + v0 * a.lda;
+        l.M = words;
+        l.tiles_m = (int)lvae_ceil_div(words, 256);
+        l.bias = a.bias + v0;
+        l.v0 = v0;
+        l.lse = rows.lse_of;
+        l.gy = rows.gy_of;
+        l.g = gbuf;
+        l.ldg = pl.piece;
+        l.plane_g = plane_g;
+        l.dbias = d_bias ? (float*)(ws + pl.dbias) : nullptr;
+        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, l, st));
+        if (d_bias) {
+            dbias_kernel<<<dim3((unsigned)lvae_ceil_div(words, 256)), 256, 0, st>>>(l.dbias, pl.piece, waves_n, pl.tile_n, rows.n_rows,
+                                                                                   words, unscale, d_bias, q->bias_dtype, v0);
+            LVAE_LAUNCH_CHECK();
+        }
+        if (d_hidden) {
+            VgArgs h = {};
+            h.a = w0 + v0 * a.lda;
+            h.lda = a.lda;
+            h.plane_a = a.plane_a;
+            h.a_cols = a.a_cols;
+            h.b = gbuf;
+            h.ldb = pl.piece;
+            h.plane_b = plane_g;
+            h.M = pl.H;
+            h.N = pl.T;
+            h.K = words;
+            h.n_rows = rows.n_rows;
+            h.tiles_m = (int)th;
+            h.tiles_n = a.tiles_n;
+            h.splits = pl.splits_h;
+            h.slab = (float*)(ws + pl.slab);
+            h.ld_slab = pl.Kp;
+            h.slab_stride = pl.Tpad * pl.Kp;
+            h.slab_add = v0 > 0;
+            RUN(launch_tiles(q->dtype, VG_DHIDDEN, pl.narrow, h, st));
+        }
+        if (d_weight) {
+            VgArgs w = {};
+            w.a = hp;
+            w.lda = pl.Kp;
+            w.plane_a = a.plane_b;
+            w.a_cols = pl.Kp;
+            w.b = gbuf;
+            w.ldb = pl.piece;
+            w.plane_b = plane_g;
+            w.M = pl.H;
+            w.N = words;
+            w.n_rows = rows.n_rows;
+            w.tiles_m = (int)th;
+            w.tiles_n = (int)lvae_ceil_div(words, 256);
+            w.splits = pl.splits_w;
+            char* out = (char*)d_weight + v0 * pl.H * esz;
+            if (pl.splits_w > 1) {
+                w.slab = (float*)(ws + pl.slab_w);
+                w.ld_slab = pl.Kp;
+                w.slab_stride = pl.piece * pl.Kp;
+                RUN(launch_tiles(q->dtype, VG_DWEIGHT_SLAB, 0, w, st));
+                dweight_kernel<<<dim3((unsigned)lvae_ceil_div(words * pl.H, 256)), 256, 0, st>>>(
+                    w.slab, pl.splits_w, w.slab_stride, w.ld_slab, words, (int)pl.H, unscale, out, q->dtype);
+                LVAE_LAUNCH_CHECK();
+            } else {
+                w.out = out;
+                w.ld_out = pl.H;
+                w.unscale = unscale;
+                RUN(launch_tiles(q->dtype, VG_DWEIGHT, 0, w, st));
+            }
+        }
+    }
+    if (d_hidden) {
+        const int64_t n = pl.T * ((pl.H + 3) / 4);
+        dhidden_kernel<<<dim3((unsigned)lvae_ceil_div(n, 256)), 256, 0, st>>>((float*)(ws + pl.slab), pl.splits_h, pl.Tpad * pl.Kp, pl.Kp,
+                                                                             rows.inv, pl.T, (int)pl.H, unscale, d_hidden, q->dtype);
+        LVAE_LAUNCH_CHECK();
+    }
+    return LVAE_OK;
+}
+
+extern "C" int lvae_vocab_loss_f32(const lvae_vocab_problem* q, const float* ll, int mean, float factor, float* loss, void* stream) {
+    Plan pl = {};
+    RUN(check_problem(q, &pl));
+    LVAE_CHECK_ARG(ll && loss && q->targets, "ll, loss and targets must be non-NULL");
+    loss_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(q->targets, axes_of(q, q->target_stride), pl.T, q->ignore_index, ll, mean, factor, loss);
+    LVAE_LAUNCH_CHECK();
+    return LVAE_OK;
+}
+
+extern "C" int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream) {
+    LVAE_CHECK_ARG(n >= 1 && n < (1ll << 33) && len >= 0, "bad shape: n=%lld len=%lld", (long long)n, (long long)len);
+    LVAE_CHECK_ARG(out && (x || len == 0), "x and out must be non-NULL");
+    segment_sum_kernel<<<dim3((unsigned)lvae_ceil_div(n, 4)), 256, 0, (hipStream_t)stream>>>(x, n, len, out);
+    LVAE_LAUNCH_CHECK();
+    return LVAE_OK;
+}

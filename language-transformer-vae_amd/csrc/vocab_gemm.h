@@ -1,0 +1,436 @@
+// Tile products of the vocabulary cross entropy on the bf16 / fp16 matrix cores (gfx950), shared by its three products:
+//
+//   logits  l[v,t]  = sum_h W[v,h] H[t,h]      both operands hold the summed index contiguously
+//   dHidden d[h,t]  = sum_v W[v,h] G[t,v]      W is read ACROSS its rows (transposing LDS read), G along them
+//   dWeight d[h,v]  = sum_t H[t,h] G[t,v]      both read across their rows
+//
+// One workgroup owns a tile of TM x TN outputs and walks the summed index 64 at a time: the two operand slices
+// (TM x 64 and TN x 64, 16-bit) go from memory straight into LDS (global_load_lds, 16 bytes a lane), double buffered,
+// so the loads of the next slice fly while the matrix cores work on this one.  Nothing is ever transposed in memory:
+// an operand stored [k][m] is staged as it lies and read with ds_read_b64_tr_b16, which hands each lane four k values of
+// its own column.
+//
+// float32 operands are three bf16 limbs (x = x1 + x2 + x3, 8 bits each, exact to 2^-24): six limb products, smallest
+// first, on the same code by walking the summed index once per product.  The products left out are below 2^-24 of
+// |a||b|, the rounding of a float32 product itself.
+//
+// Row order.  A lane of the 16x16x32 instruction ends up with rows 4g..4g+3 (g = lane / 16) of each of its eight row
+// tiles.  The rows of W that feed row tile i are chosen as m = 32 g + 4 i + r, so that a lane's 8 x 4 results are 32
+// CONSECUTIVE m of one column: the epilogues store 64 (16-bit) or 128 (float32) contiguous bytes a lane, and the
+// reduction over the vocabulary is 32 values in registers plus two cross-lane steps.
+//
+// LDS.  Both layouts XOR the 16-byte piece index with bits of the row, chosen so that the 16 lanes that one LDS cycle
+// serves fall on different banks for this row order; the direct-to-LDS load writes linearly, so the XOR is applied to
+// the global address instead.
+#pragma once
+#include "lvae_common.h"
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+#define VG_BK 64
+
+// what one launch computes; pointers in elements of 16 bits unless named otherwise
+struct VgArgs {
+    const uint16_t* a;          // first row of the tile range (W at its first vocabulary row of the piece, or H)
+    int64_t lda, plane_a;       // row pitch, distance between limb planes
+    const uint16_t* b;
+    int64_t ldb, plane_b;
+    int64_t M;                  // valid outputs along m (rows of W, or columns h)
+    int64_t a_cols;             // valid columns of an operand read across its rows
+    int64_t N;                  // outputs along n: upper bound; the kept tokens are min(N, *n_rows) where n is tokens
+    int64_t K;                  // summed index: vocabulary rows of the piece, padded H, or tokens (bound by *n_rows)
+    const int* n_rows;          // kept tokens (device)
+    int tiles_m, tiles_n, splits;
+    // epilogues
+    const float* bias;          // [>= M rounded up to 256] float32 of the piece, -inf behind the vocabulary
+    const int* tgt;             // target of each kept token
+    const float* lse;           // LSE of each kept token
+    const float* gy;            // (scaled) upstream gradient of each kept token
+    int64_t v0;                 // first vocabulary row of the piece
+    float2* part;               // [tiles_m][ldp] running maximum and sum of each token over the tile
+    int64_t ldp;
+    float* picked;              // logit of the target
+    uint16_t* g;                // [planes][rows][ldg] gradient of the logits
+    int64_t ldg, plane_g;
+    float* dbias;               // [tiles_n * waves along n][ldg] partial column sums, or NULL
+    float* slab;                // [splits][slab_rows][ld_slab] float32 partial products
+    int64_t ld_slab, slab_stride;
+    int slab_add;               // add to what the slab holds
+    void* out;                  // direct output [N][ld_out] of the operand type (float32 for three limbs)
+    int64_t ld_out;
+    const float* unscale;       // device factor of the outputs, or NULL
+};
+
+enum { VG_LSE = 0, VG_GRAD = 1, VG_SLAB = 2, VG_OUT = 3 };
+// the products as launched
+enum { VG_LOGITS_LSE = 0, VG_LOGITS_GRAD = 1, VG_DHIDDEN = 2, VG_DWEIGHT_SLAB = 3, VG_DWEIGHT = 4 };
+// element types: LVAE_F32 (three bf16 limbs), LVAE_BF16, LVAE_F16
+
+template <int DT> __device__ __forceinline__ f32x4 vg_mma(s16x8 a, s16x8 b, f32x4 c) {
+    if constexpr (DT == LVAE_F16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// round to nearest even (the compiler's conversions: v_cvt_pk_bf16_f32 / v_cvt_f16_f32)
+template <int DT> __device__ __forceinline__ uint16_t vg_round(float x) {
+    if constexpr (DT == LVAE_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+    else return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+__device__ __forceinline__ float vg_bf16(uint16_t x) { return __uint_as_float((unsigned)x << 16); }
+
+// x as three bf16 limbs; an infinity or NaN stays in the first one
+__device__ __forceinline__ void vg_limbs(float x, uint16_t l[3]) {
+    l[0] = vg_round<LVAE_BF16>(x);
+    float r = x - vg_bf16(l[0]);
+    if (!(fabsf(x) < INFINITY) || !(fabsf(r) < INFINITY)) r = 0.f;
+    l[1] = vg_round<LVAE_BF16>(r);
+    l[2] = vg_round<LVAE_BF16>(r - vg_bf16(l[1]));
+}
+
+// 16 bytes a lane from base + off (bytes) to LDS at the wave-uniform byte address lds (+ 16 lane).  As inline assembly:
+// with the builtin the compiler waits for every load in flight before each transposing LDS read.  It has no output
+// register; the waits are vg_wait_loads().
+__device__ __forceinline__ void vg_load_lds(unsigned lds, unsigned off, const void* base) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :: "s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void vg_wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// sum over the 16 lanes of a row, by DPP (every lane gets it)
+__device__ __forceinline__ float vg_row_sum(float v) {
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));    // quad_perm 1,0,3,2
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));    // quad_perm 2,3,0,1
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xF, 0xF, true));   // half-row mirror
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x140, 0xF, 0xF, true));   // row mirror
+    return v;
+}
+
+// TRA / TRB: the operand is stored [k][m] / [k][n].  WM x WN waves, each 128 x (16 NJ).
+template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ>
+__global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
+    constexpr int W = WM * WN, MI = 8, TM = 128 * WM, TN = 16 * NJ * WN;
+    constexpr int A_BYTES = TM * VG_BK * 2, B_BYTES = TN * VG_BK * 2, STAGE = A_BYTES + B_BYTES;
+    constexpr int QA = A_BYTES / 1024 / W, QB = B_BYTES / 1024 / W;
+    static_assert(QA * W * 1024 == A_BYTES && QB * W * 1024 == B_BYTES, "whole loads");
+    __shared__ __align__(1024) char lds[2 * STAGE];
+
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave % WM, wn = wave / WM;
+
+    // ---- which tile.  Workgroups go round the 8 XCDs; each XCD walks a contiguous range of tiles, four row tiles
+    // wide, so that the operand slices it shares stay in its own L2.
+    const int n_kept = __builtin_amdgcn_readfirstlane(p.n_rows[0]);
+    int tm, tn, split;
+    {
+        const int per = p.tiles_m * p.tiles_n, total = per * p.splits;
+        const int each = total / 8, rest = total % 8, x = blockIdx.x & 7, l = blockIdx.x >> 3;
+        int id = x * each + min(x, rest) + l;
+        if (l >= each + (x < rest ? 1 : 0)) return;
+        split = id / per;
+        id -= split * per;
+        const int group = 4 * p.tiles_n, g = id / group, first = g * 4, wide = min(4, p.tiles_m - first);
+        tm = first + (id - g * group) % wide;
+        tn = (id - g * group) / wide;
+    }
+    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+    constexpr bool N_TOKENS = !TRB;                     // n counts tokens unless G is read across its rows
+    const int64_t n_lim = N_TOKENS ? (int64_t)n_kept : p.N;
+    if (N_TOKENS && n0 >= n_lim) return;                // uniform: every wave leaves
+    const int64_t k_lim = TRB ? (int64_t)n_kept : p.K;
+
+    constexpr int NP = DT == LVAE_F32 ? 6 : 1;
+    const int ks_all = (int)((k_lim + VG_BK - 1) / VG_BK);
+    const int ks_per = (ks_all + p.splits - 1) / p.splits;
+    const int ks0 = min(split * ks_per, ks_all), ks = min(ks_per, ks_all - ks0);
+    const int steps = ks * NP;
+
+    // ---- per-lane byte offsets of the loads, relative to the tile's (scalar) base
+    unsigned offa[QA], offa_last[QA], offb[QB];
+    const uint16_t* abase;
+    const uint16_t* bbase;
+    constexpr int SA = TM / 8, SB = TN / 8;             // 16-byte pieces of a row stored across
+    if constexpr (!TRA) {
+        abase = p.a + m0 * p.lda;
+#pragma unroll
+        for (int q = 0; q < QA; ++q) {
+            const int r = (q * W + wave) * 8 + (lane >> 3);
+            const int sw = ((r >> 1) & 1) | (((r >> 5) & 3) << 1);
+            const int64_t rc = min((int64_t)r, p.M - 1 - m0);
+            offa[q] = (unsigned)(rc * p.lda * 2 + (((lane & 7) ^ sw) << 4));
+            offa_last[q] = offa[q];
+        }
+    } else {
+        abase = p.a + m0;
+        const int64_t last = (int64_t)(ks_all - 1) * VG_BK;
+        const int64_t rows = TRB ? (int64_t)VG_BK : max((int64_t)1, k_lim - last);   // H is padded to whole slices
+#pragma unroll
+        for (int q = 0; q < QA; ++q) {
+            const int r = (q * W + wave) * (64 / SA) + lane / SA;
+            const int64_t piece = min((int64_t)((lane % SA) ^ (r & 3)), (p.a_cols - m0) / 8 - 1);
+            offa[q] = (unsigned)(r * p.lda * 2 + piece * 16);
+            offa_last[q] = (unsigned)(min((int64_t)r, rows - 1) * p.lda * 2 + piece * 16);
+        }
+    }
+    if constexpr (!TRB) {
+        bbase = p.b + n0 * p.ldb;
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+            const int r = (q * W + wave) * 8 + (lane >> 3);
+            offb[q] = (unsigned)(r * p.ldb * 2 + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
+        }
+    } else {
+        bbase = p.b + n0;
+#pragma unroll
+        for (int q = 0; q < QB; ++q) {
+            const int r = (q * W + wave) * (64 / SB) + lane / SB;
+            offb[q] = (unsigned)(r * p.ldb * 2 + (((lane % SB) ^ ((r & 3) << 1)) << 4));
+        }
+    }
+
+    const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
+    auto issue = [&](int buf, int pair, int k) {
+        // limb planes of the six products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+        const int la = pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
+        const int lb = DT != LVAE_F32 ? 0 : pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0;
+        const int64_t kk = (int64_t)(ks0 + k) * VG_BK;
+        const uint16_t* ab = abase + la * p.plane_a + (TRA ? kk * p.lda : kk);
+        const uint16_t* bb = bbase + lb * p.plane_b + (TRB ? kk * p.ldb : kk);
+        const bool last = TRA && !TRB && (ks0 + k == ks_all - 1);
+        const unsigned dst = lds0 + buf * STAGE + wave * 1024;
+#pragma unroll
+        for (int q = 0; q < QA; ++q)
+            vg_load_lds(dst + q * W * 1024, (TRA && !TRB) ? (last ? offa_last[q] : offa[q]) : offa[q], ab);
+#pragma unroll
+        for (int q = 0; q < QB; ++q) vg_load_lds(dst + A_BYTES + q * W * 1024, offb[q], bb);
+    };
+
+    f32x4 acc[MI][NJ];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int mp = lane & 15, g4 = lane >> 4;
+    // lane constants of the LDS reads
+    int a_n[2], b_n[2];                    // along rows: byte offsets for the two halves of a slice
+    {
+        const int row = wm * 128 + (mp >> 2) * 32 + (mp & 3);
+        const int sw = ((row >> 1) & 1) | (((row >> 5) & 3) << 1);
+        const int rb = wn * 16 * NJ + mp;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            a_n[kk] = row * 128 + (((kk * 4 + g4) ^ sw) << 4);
+            b_n[kk] = rb * 128 + (((kk * 4 + g4) ^ ((rb >> 1) & 7)) << 4);
+        }
+    }
+    const int kr = g4 * 8 + (mp >> 2);     // across rows: the k row this lane addresses (+ 32 kk + 4 half)
+
+    auto compute = [&](int buf) {
+        const char* la = lds + buf * STAGE;
+        const char* lb = la + A_BYTES;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            s16x8 af[MI], bf[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                if constexpr (!TRB) {
+                    bf[j] = *(const s16x8*)(lb + b_n[kk] + j * 16 * 128);
+                } else {
+                    const int piece = (wn * 2 * NJ + j * 2 + ((mp & 3) >> 1)) ^ ((mp >> 2) << 1);
+                    const int at = (kk * 32 + kr) * (TN * 2) + piece * 16 + (mp & 1) * 8;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lb + at));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lb + at + 4 * TN * 2));
+                    bf[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                if constexpr (!TRA) {
+                    af[i] = *(const s16x8*)(la + a_n[kk] + i * 4 * 128);
+                } else {
+                    const int piece = (wm * 16 + (mp & 3) * 4 + (i >> 1)) ^ (mp >> 2);
+                    const int at = (kk * 32 + kr) * (TM * 2) + piece * 16 + (i & 1) * 8;
+                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(la + at));
+                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(la + at + 4 * TM * 2));
+                    af[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = vg_mma<DT>(af[i], bf[j], acc[i][j]);
+        }
+    };
+
+    if (steps > 0) {
+        int pair = 0, k = 0;
+        issue(0, 0, 0);
+        vg_wait_loads();
+        __syncthreads();
+        for (int s = 0; s < steps; ++s) {
+            if (++k == ks) { k = 0; ++pair; }
+            if (s + 1 < steps) issue((s + 1) & 1, pair, k);
+            compute(s & 1);
+            vg_wait_loads();
+            __syncthreads();
+        }
+    }
+
+    // ---- epilogues.  This lane holds, for column n = n0 + 16 (NJ wn + j) + mp, the rows m = mb + 4 i + r.
+    const int64_t mb = m0 + wm * 128 + g4 * 32;
+    const int nb = wn * 16 * NJ + mp;
+    if constexpr (EPI == VG_LSE || EPI == VG_GRAD) {
+        float bias[MI][4];
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const f32x4 v = *(const f32x4*)(p.bias + mb + 4 * i);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) bias[i][r] = v[r];
+        }
+        if constexpr (EPI == VG_LSE) {
+            float2* red = (float2*)lds;                 // [WM][TN]; the last barrier has passed
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int64_t n = n0 + nb + j * 16;
+                const bool there = n < n_lim;
+                const int64_t rel = there ? (int64_t)p.tgt[n] - p.v0 - mb : -1;
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        acc[i][j][r] += bias[i][r];
+                        top = fmaxf(top, acc[i][j][r]);
+                    }
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float ref = top == -INFINITY ? 0.f : top;
+                float sum = 0.f, hit = 0.f;
+                bool any = false;
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        sum += lvae_exp2((acc[i][j][r] - ref) * LVAE_LOG2E);
+                        const bool is = rel == 4 * i + r;
+                        hit = is ? acc[i][j][r] : hit;
+                        any |= is;
+                    }
+                sum += __shfl_xor(sum, 16, 64);
+                sum += __shfl_xor(sum, 32, 64);
+                if (any) p.picked[n] = hit;
+                if (g4 == 0) red[wm * TN + nb + j * 16] = make_float2(top, sum);
+            }
+            __syncthreads();
+            for (int c = threadIdx.x; c < TN; c += 64 * W) {
+                if (n0 + c >= n_lim) continue;
+                float2 x = red[c];
+#pragma unroll
+                for (int w = 1; w < WM; ++w) {
+                    const float2 y = red[w * TN + c];
+                    const float top = fmaxf(x.x, y.x), ref = top == -INFINITY ? 0.f : top;
+                    x.y = x.y * lvae_exp2((x.x - ref) * LVAE_LOG2E) + y.y * lvae_exp2((y.x - ref) * LVAE_LOG2E);
+                    x.x = top;
+                }
+                p.part[(int64_t)tm * p.ldp + n0 + c] = x;
+            }
+        } else {
+            float colsum[MI][4];
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) colsum[i][r] = 0.f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                const int64_t n = n0 + nb + j * 16;
+                const bool there = n < n_lim;           // rows behind the last kept token are written as zeros
+                const int64_t rel = there ? (int64_t)p.tgt[n] - p.v0 - mb : -1;
+                const float lse = there ? p.lse[n] : 0.f, gy = there ? p.gy[n] : 0.f;
+                uint16_t* row = p.g + n * p.ldg + mb;
+#pragma unroll
+                for (int i = 0; i < MI; i += 2) {
+                    s16x8 o[3];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int ii = i + (e >> 2), r = e & 3;
+                        float x = lvae_exp2((acc[ii][j][r] + bias[ii][r] - lse) * LVAE_LOG2E);
+                        x = (rel == 4 * ii + r ? x - 1.f : x) * gy;
+                        x = there ? x : 0.f;
+                        colsum[ii][r] += x;
+                        if constexpr (DT == LVAE_F32) {
+                            uint16_t l[3];
+                            vg_limbs(x, l);
+                            o[0][e] = l[0]; o[1][e] = l[1]; o[2][e] = l[2];
+                        } else {
+                            // G is rounded once to the operand type, half a step of each element: the products need a
+                            // 16-bit operand, and the gradients are rounded to the same type themselves
+                            o[0][e] = vg_round<DT>(x);
+                        }
+                    }
+#pragma unroll
+                    for (int l = 0; l < (DT == LVAE_F32 ? 3 : 1); ++l) *(s16x8*)(row + l * p.plane_g + 4 * i) = o[l];
+                }
+            }
+            if (p.dbias) {
+                float* d = p.dbias + ((int64_t)tn * WN + wn) * p.ldg + mb;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    f32x4 v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) v[r] = vg_row_sum(colsum[i][r]);
+                    if (mp == 0) *(f32x4*)(d + 4 * i) = v;
+                }
+            }
+        }
+    } else if constexpr (EPI == VG_SLAB) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int64_t n = n0 + nb + j * 16;
+            if (n >= n_lim) continue;
+            float* row = p.slab + split * p.slab_stride + n * p.ld_slab + mb;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                if (mb + 4 * i >= p.ld_slab) continue;  // the pitch is a multiple of 64
+                f32x4 v = acc[i][j];
+                if (p.slab_add) v += *(const f32x4*)(row + 4 * i);
+                *(f32x4*)(row + 4 * i) = v;
+            }
+        }
+    } else {
+        const float f = p.unscale ? p.unscale[0] : 1.f;
+        const bool whole = mb + 32 <= p.M && (p.ld_out & 7) == 0;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int64_t n = n0 + nb + j * 16;
+            if (n >= n_lim) continue;
+            if constexpr (DT == LVAE_F32) {
+                float* row = (float*)p.out + n * p.ld_out + mb;
+#pragma unroll
+                for (int i = 0; i < MI; ++i) {
+                    if (whole) *(f32x4*)(row + 4 * i) = acc[i][j];
+                    else
+                        for (int r = 0; r < 4; ++r)
+                            if (mb + 4 * i + r < p.M) row[4 * i + r] = acc[i][j][r];
+                }
+            } else {
+                uint16_t* row = (uint16_t*)p.out + n * p.ld_out + mb;
+#pragma unroll
+                for (int i = 0; i < MI; i += 2) {
+                    s16x8 o;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) o[e] = vg_round<DT>(acc[i + (e >> 2)][j][e & 3] * f);
+                    if (whole) *(s16x8*)(row + 4 * i) = o;
+                    else
+                        for (int e = 0; e < 8; ++e)
+                            if (mb + 4 * i + e < p.M) row[4 * i + e] = o[e];
+                }
+            }
+        }
+    }
+}

@@ -1,0 +1,4 @@
+// Tile products of the vocabulary cross entropy, element type bf16.
+#define VG_DT LVAE_BF16
+#define VG_NAME lvae_vg_launch_bf16
+#include "vocab_tiles.h"
