@@ -397,11 +397,17 @@ __global__ __launch_bounds__(256) void dweight_kernel(const float* slab, int spl
 // d_bias of a piece: the partial column sums of the tiles that hold kept tokens
 __global__ __launch_bounds__(256) void dbias_kernel(const float* part, int64_t ld, int per_tile, int tile_rows, const int* n_rows,
                                                     int64_t rows, const float* unscale, void* out, int dt, int64_t v0) {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v >= rows) return;
+    __shared__ double red[8][32];
+    const int64_t v = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
+    const int g = threadIdx.x >> 5;
     const int n = (n_rows[0] + tile_rows - 1) / tile_rows * per_tile;
     double x = 0.0;
-    for (int i = 0; i < n; ++i) x += part[(int64_t)i * ld + v];
+    if (v < rows)
+        for (int i = g; i < n; i += 8) x += part[(int64_t)i * ld + v];
+    red[g][threadIdx.x & 31] = x;
+    __syncthreads();
+    if (g || v >= rows) return;
+    for (int i = 1; i < 8; ++i) x += red[i][threadIdx.x];
     const float f = (float)x;
     store_any(out, v0 + v, unscale ? f * unscale[0] : f, dt);
 }
@@ -773,7 +779,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         l.dbias = d_bias ? (float*)(ws + pl.dbias) : nullptr;
         RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, l, st));
         if (d_bias) {
-            dbias_kernel<<<dim3((unsigned)lvae_ceil_div(words, 256)), 256, 0, st>>>(l.dbias, pl.piece, waves_n, pl.tile_n, rows.n_rows,
+            dbias_kernel<<<dim3((unsigned)lvae_ceil_div(words, 32)), 256, 0, st>>>(l.dbias, pl.piece, waves_n, pl.tile_n, rows.n_rows,
                                                                                    words, unscale, d_bias, q->bias_dtype, v0);
             LVAE_LAUNCH_CHECK();
         }

@@ -30,7 +30,7 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-#define VG_BK 64
+#define VG_BK 64               // a slice of the summed index: rows of 128 bytes, whole cache lines (64-byte rows load at half the rate)
 
 // what one launch computes; pointers in elements of 16 bits unless named otherwise
 struct VgArgs {
@@ -95,11 +95,46 @@ __device__ __forceinline__ void vg_limbs(float x, uint16_t l[3]) {
 // 16 bytes a lane from base + off (bytes) to LDS at the wave-uniform byte address lds (+ 16 lane).  As inline assembly:
 // with the builtin the compiler waits for every load in flight before each transposing LDS read.  It has no output
 // register; the waits are vg_wait_loads().
+__device__ __forceinline__ const void* vg_uniform(const void* p) {
+    const uint64_t a = (uint64_t)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    return (const void*)((uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ void vg_load_lds(unsigned lds, unsigned off, const void* base) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :: "s"(lds), "v"(off), "s"(base) : "memory");
 }
-__device__ __forceinline__ void vg_wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// until at most N of this wave's loads are in flight (they complete in order)
+template <int N> __device__ __forceinline__ void vg_wait_loads() {
+    static_assert(N < 64, "six bits");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x70 | 0xF00);      // vmcnt alone
+    asm volatile("" ::: "memory");
+}
+
+// until at most N of this wave's LDS reads are under way (they complete in order)
+template <int N> __device__ __forceinline__ void vg_wait_lds() {
+    static_assert(N < 16, "four bits");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F | N << 8);                               // lgkmcnt alone
+    asm volatile("" ::: "memory");
+}
+// a barrier that nothing is scheduled across, the matrix instructions included
+__device__ __forceinline__ void vg_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// Which 16-byte piece of an LDS row holds piece 0 of its slice (XOR), for an operand stored along the summed index.  One
+// LDS cycle serves 16 lanes of a 16-byte read, and not neighbours: rows 0-3 and 12-15 of one piece go together with rows
+// 4-11 of the next.  With either reading (neighbours, or this) every set of 16 falls on different banks; measured without
+// conflicts.  a: rows 32 q + 4 i + r in the row order above, 4 q + r counting for 16; b: 16 consecutive rows.
+__device__ __forceinline__ int vg_swizzle(int row16) { return row16 >> 1; }
+__device__ __forceinline__ int vg_swizzle_a(int row) { return vg_swizzle(((row >> 5) & 3) * 4 + (row & 3)); }
+__device__ __forceinline__ int vg_swizzle_b(int row) { return vg_swizzle(row & 15); }
 
 // sum over the 16 lanes of a row, by DPP (every lane gets it)
 __device__ __forceinline__ float vg_row_sum(float v) {
@@ -110,14 +145,15 @@ __device__ __forceinline__ float vg_row_sum(float v) {
     return v;
 }
 
-// TRA / TRB: the operand is stored [k][m] / [k][n].  WM x WN waves, each 128 x (16 NJ).
-template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ>
+// TRA / TRB: the operand is stored [k][m] / [k][n].  WM x WN waves, each 128 x (16 NJ); NA slices of a and
+// two of b in LDS at a time.
+template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
 __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
-    constexpr int W = WM * WN, MI = 8, TM = 128 * WM, TN = 16 * NJ * WN;
-    constexpr int A_BYTES = TM * VG_BK * 2, B_BYTES = TN * VG_BK * 2, STAGE = A_BYTES + B_BYTES;
+    constexpr int W = WM * WN, MI = 8, TM = 128 * WM, TN = 16 * NJ * WN, BK = VG_BK;
+    constexpr int A_BYTES = TM * BK * 2, B_BYTES = TN * BK * 2;
     constexpr int QA = A_BYTES / 1024 / W, QB = B_BYTES / 1024 / W;
     static_assert(QA * W * 1024 == A_BYTES && QB * W * 1024 == B_BYTES, "whole loads");
-    __shared__ __align__(1024) char lds[2 * STAGE];
+    __shared__ __align__(1024) char lds[NA * A_BYTES + 2 * B_BYTES];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -145,7 +181,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
     const int64_t k_lim = TRB ? (int64_t)n_kept : p.K;
 
     constexpr int NP = DT == LVAE_F32 ? 6 : 1;
-    const int ks_all = (int)((k_lim + VG_BK - 1) / VG_BK);
+    const int ks_all = (int)((k_lim + BK - 1) / BK);
     const int ks_per = (ks_all + p.splits - 1) / p.splits;
     const int ks0 = min(split * ks_per, ks_all), ks = min(ks_per, ks_all - ks0);
     const int steps = ks * NP;
@@ -154,21 +190,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
     unsigned offa[QA], offa_last[QA], offb[QB];
     const uint16_t* abase;
     const uint16_t* bbase;
-    constexpr int SA = TM / 8, SB = TN / 8;             // 16-byte pieces of a row stored across
+    constexpr int SK = BK / 8, SA = TM / 8, SB = TN / 8;    // 16-byte pieces of a row stored along / across
     if constexpr (!TRA) {
         abase = p.a + m0 * p.lda;
 #pragma unroll
         for (int q = 0; q < QA; ++q) {
-            const int r = (q * W + wave) * 8 + (lane >> 3);
-            const int sw = ((r >> 1) & 1) | (((r >> 5) & 3) << 1);
+            const int r = (q * W + wave) * (64 / SK) + lane / SK;
             const int64_t rc = min((int64_t)r, p.M - 1 - m0);
-            offa[q] = (unsigned)(rc * p.lda * 2 + (((lane & 7) ^ sw) << 4));
+            offa[q] = (unsigned)(rc * p.lda * 2 + (((lane % SK) ^ vg_swizzle_a(r)) << 4));
             offa_last[q] = offa[q];
         }
     } else {
         abase = p.a + m0;
-        const int64_t last = (int64_t)(ks_all - 1) * VG_BK;
-        const int64_t rows = TRB ? (int64_t)VG_BK : max((int64_t)1, k_lim - last);   // H is padded to whole slices
+        const int64_t last = (int64_t)(ks_all - 1) * BK;
+        const int64_t rows = TRB ? (int64_t)BK : max((int64_t)1, k_lim - last);     // H is padded to whole slices
 #pragma unroll
         for (int q = 0; q < QA; ++q) {
             const int r = (q * W + wave) * (64 / SA) + lane / SA;
@@ -181,8 +216,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
         bbase = p.b + n0 * p.ldb;
 #pragma unroll
         for (int q = 0; q < QB; ++q) {
-            const int r = (q * W + wave) * 8 + (lane >> 3);
-            offb[q] = (unsigned)(r * p.ldb * 2 + (((lane & 7) ^ ((r >> 1) & 7)) << 4));
+            const int r = (q * W + wave) * (64 / SK) + lane / SK;
+            offb[q] = (unsigned)(r * p.ldb * 2 + (((lane % SK) ^ vg_swizzle_b(r)) << 4));
         }
     } else {
         bbase = p.b + n0;
@@ -194,198 +229,268 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
     }
 
     const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) char*)lds;
-    auto issue = [&](int buf, int pair, int k) {
-        // limb planes of the six products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-        const int la = pair == 1 ? 2 : pair == 2 || pair == 4 ? 1 : 0;
-        const int lb = DT != LVAE_F32 ? 0 : pair == 0 ? 2 : pair == 2 || pair == 3 ? 1 : 0;
-        const int64_t kk = (int64_t)(ks0 + k) * VG_BK;
-        const uint16_t* ab = abase + la * p.plane_a + (TRA ? kk * p.lda : kk);
-        const uint16_t* bb = bbase + lb * p.plane_b + (TRB ? kk * p.ldb : kk);
-        const bool last = TRA && !TRB && (ks0 + k == ks_all - 1);
-        const unsigned dst = lds0 + buf * STAGE + wave * 1024;
-#pragma unroll
-        for (int q = 0; q < QA; ++q)
-            vg_load_lds(dst + q * W * 1024, (TRA && !TRB) ? (last ? offa_last[q] : offa[q]) : offa[q], ab);
-#pragma unroll
-        for (int q = 0; q < QB; ++q) vg_load_lds(dst + A_BYTES + q * W * 1024, offb[q], bb);
+    // the next slice to load, of each operand: limb pair, slice, ring slot
+    struct Next { int pair, k, slot; };
+    Next na = {0, 0, 0}, nb_ = {0, 0, 0};
+    const void *l_a = nullptr, *l_b = nullptr;
+    unsigned l_dst_a = 0, l_dst_b = 0;
+    bool l_last = false;
+    // limb planes of the six products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+    auto next_a = [&]() {
+        const int limb = na.pair == 1 ? 2 : na.pair == 2 || na.pair == 4 ? 1 : 0;
+        const int64_t kk = (int64_t)(ks0 + na.k) * BK;
+        l_a = vg_uniform(abase + limb * p.plane_a + (TRA ? kk * p.lda : kk));
+        l_last = TRA && !TRB && (ks0 + na.k == ks_all - 1);
+        l_dst_a = __builtin_amdgcn_readfirstlane(lds0 + na.slot * A_BYTES + wave * 1024);
+        if (++na.k == ks) { na.k = 0; ++na.pair; }
+        na.slot = na.slot + 1 == NA ? 0 : na.slot + 1;
     };
+    auto next_b = [&]() {
+        const int limb = DT != LVAE_F32 ? 0 : nb_.pair == 0 ? 2 : nb_.pair == 2 || nb_.pair == 3 ? 1 : 0;
+        const int64_t kk = (int64_t)(ks0 + nb_.k) * BK;
+        l_b = vg_uniform(bbase + limb * p.plane_b + (TRB ? kk * p.ldb : kk));
+        l_dst_b = __builtin_amdgcn_readfirstlane(lds0 + NA * A_BYTES + nb_.slot * B_BYTES + wave * 1024);
+        if (++nb_.k == ks) { nb_.k = 0; ++nb_.pair; }
+        nb_.slot ^= 1;
+    };
+    auto load_a = [&](int q) { vg_load_lds(l_dst_a + q * W * 1024, (TRA && !TRB) ? (l_last ? offa_last[q] : offa[q]) : offa[q], l_a); };
+    auto load_b = [&](int q) { vg_load_lds(l_dst_b + q * W * 1024, offb[q], l_b); };
+    auto load_slice_a = [&]() {
+        next_a();
+#pragma unroll
+        for (int q = 0; q < QA; ++q) load_a(q);
+    };
+    auto load_slice_b = [&]() {
+        next_b();
+#pragma unroll
+        for (int q = 0; q < QB; ++q) load_b(q);
+    };
+    if (steps > 0) { load_slice_a(); load_slice_b(); }
+    if (steps > 1) { load_slice_a(); load_slice_b(); }
+    if (NA == 3 && steps > 2) load_slice_a();
+
+    const int mp = lane & 15, g4 = lane >> 4;
+    // this lane holds, for column n = n0 + 16 (NJ wn + j) + mp, the rows m = mb + 4 i + r
+    const int64_t mb = m0 + wm * 128 + g4 * 32;
+    const int nb = wn * 16 * NJ + mp;
 
     f32x4 acc[MI][NJ];
 #pragma unroll
-    for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if constexpr (EPI == VG_LSE || EPI == VG_GRAD) x = *(const f32x4*)(p.bias + mb + 4 * i);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    const int mp = lane & 15, g4 = lane >> 4;
-    // lane constants of the LDS reads
-    int a_n[2], b_n[2];                    // along rows: byte offsets for the two halves of a slice
-    {
-        const int row = wm * 128 + (mp >> 2) * 32 + (mp & 3);
-        const int sw = ((row >> 1) & 1) | (((row >> 5) & 3) << 1);
-        const int rb = wn * 16 * NJ + mp;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            a_n[kk] = row * 128 + (((kk * 4 + g4) ^ sw) << 4);
-            b_n[kk] = rb * 128 + (((kk * 4 + g4) ^ ((rb >> 1) & 7)) << 4);
-        }
+        for (int j = 0; j < NJ; ++j) acc[i][j] = x;
     }
-    const int kr = g4 * 8 + (mp >> 2);     // across rows: the k row this lane addresses (+ 32 kk + 4 half)
 
-    auto compute = [&](int buf) {
-        const char* la = lds + buf * STAGE;
-        const char* lb = la + A_BYTES;
+    // lane constants of the LDS reads
+    const int row_a = wm * 128 + (mp >> 2) * 32 + (mp & 3), row_b = wn * 16 * NJ + mp;
+    int a_n[2], b_n[2];                    // along rows, for the two halves of a slice
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            s16x8 af[MI], bf[NJ];
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                if constexpr (!TRB) {
-                    bf[j] = *(const s16x8*)(lb + b_n[kk] + j * 16 * 128);
-                } else {
-                    const int piece = (wn * 2 * NJ + j * 2 + ((mp & 3) >> 1)) ^ ((mp >> 2) << 1);
-                    const int at = (kk * 32 + kr) * (TN * 2) + piece * 16 + (mp & 1) * 8;
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lb + at));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lb + at + 4 * TN * 2));
-                    bf[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                if constexpr (!TRA) {
-                    af[i] = *(const s16x8*)(la + a_n[kk] + i * 4 * 128);
-                } else {
-                    const int piece = (wm * 16 + (mp & 3) * 4 + (i >> 1)) ^ (mp >> 2);
-                    const int at = (kk * 32 + kr) * (TM * 2) + piece * 16 + (i & 1) * 8;
-                    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(la + at));
-                    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(la + at + 4 * TM * 2));
-                    af[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < MI; ++i)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) acc[i][j] = vg_mma<DT>(af[i], bf[j], acc[i][j]);
+    for (int kk = 0; kk < 2; ++kk) {
+        a_n[kk] = row_a * (BK * 2) + (((kk * 4 + g4) ^ vg_swizzle_a(row_a)) << 4);
+        b_n[kk] = row_b * (BK * 2) + (((kk * 4 + g4) ^ vg_swizzle_b(row_b)) << 4);
+    }
+    const int kr = g4 * 8 + (mp >> 2);     // across rows: the k row this lane addresses (+ 32 kk, + 4 for the upper half)
+
+    // Operands of half a slice in registers: a row tile's are replaced by the next half's as soon as its products are
+    // issued; the column tiles', which all row tiles use, have a second set.
+    s16x8 af[MI], bf[NJ], bn[NJ];
+    auto read_a = [&](int i, const char* la, int kk) {
+        if constexpr (!TRA) {
+            af[i] = *(const s16x8*)(la + a_n[kk] + i * 4 * BK * 2);
+        } else {
+            const int piece = (wm * 16 + (mp & 3) * 4 + (i >> 1)) ^ (mp >> 2);
+            const int at = (kk * 32 + kr) * (TM * 2) + piece * 16 + (i & 1) * 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(la + at));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(la + at + 4 * TM * 2));
+            af[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    auto read_b = [&](int j, const char* lb, int kk) {
+        if constexpr (!TRB) {
+            bn[j] = *(const s16x8*)(lb + b_n[kk] + j * 16 * BK * 2);
+        } else {
+            const int piece = (wn * 2 * NJ + j * 2 + ((mp & 3) >> 1)) ^ ((mp >> 2) << 1);
+            const int at = (kk * 32 + kr) * (TN * 2) + piece * 16 + (mp & 1) * 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lb + at));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lb + at + 4 * TN * 2));
+            bn[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
     };
 
     if (steps > 0) {
-        int pair = 0, k = 0;
-        issue(0, 0, 0);
-        vg_wait_loads();
-        __syncthreads();
+        const char *la = lds, *lb = lds + NA * A_BYTES;
+        // the first half slice's operands
+        vg_wait_loads<0>();
+        vg_barrier();
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) read_b(j, lb, 0);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) read_a(i, la, 0);
+        int slot_a = 0, slot_b = 0;
         for (int s = 0; s < steps; ++s) {
-            if (++k == ks) { k = 0; ++pair; }
-            if (s + 1 < steps) issue((s + 1) & 1, pair, k);
-            compute(s & 1);
-            vg_wait_loads();
-            __syncthreads();
+            // Half a slice is multiplied from registers while the next half is read from LDS and later slices' loads are
+            // started, each BETWEEN the matrix instructions, a few cycles behind every NJ of them: the loads of a slice
+            // in one go would hold up the wave until the address unit has taken them all.
+            //
+            // First half: reads the second half of slice s; starts the loads of a's slice s+2 (NA = 3), whose slot held
+            // slice s-1: all its readers have used it before the barrier.
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) bf[j] = bn[j];
+            vg_barrier();
+            const bool more_a = NA == 3 && s > 0 && s + 2 < steps;
+            if (more_a) next_a();
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = vg_mma<DT>(af[i], bf[j], acc[i][j]);
+                if (i < NJ) read_b(i, lb, 1);
+                read_a(i, la, 1);
+                if (more_a) {
+#pragma unroll
+                    for (int q = 0; q < QA; ++q)
+                        if (q * MI / QA == i) load_a(q);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            // Second half: reads the first half of slice s+1, for which every wave has waited for its own loads before the
+            // barrier; starts the loads of b's slice s+2 (and a's, NA = 2) into the slots of slice s.  b's last reads of
+            // slice s are waited for before the barrier; a's are used by products issued below, so with NA = 2 its
+            // loads go behind them and a second barrier.
+            __builtin_amdgcn_sched_barrier(0);
+            vg_wait_lds<(MI - NJ) * (TRA ? 2 : 1)>();   // b's reads come before the last MI - NJ of a's
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) bf[j] = bn[j];
+            if (more_a) vg_wait_loads<QA>();
+            else vg_wait_loads<0>();
+            vg_barrier();
+            const bool more = s + 2 < steps;
+            if (more) next_b();
+            slot_a = slot_a + 1 == NA ? 0 : slot_a + 1;
+            slot_b ^= 1;
+            la = lds + slot_a * A_BYTES;                // behind the last slice a slot is read that nothing needs
+            lb = lds + NA * A_BYTES + slot_b * B_BYTES;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) acc[i][j] = vg_mma<DT>(af[i], bf[j], acc[i][j]);
+                if (i < NJ) read_b(i, lb, 0);
+                read_a(i, la, 0);
+                if (more) {
+#pragma unroll
+                    for (int q = 0; q < QB; ++q)
+                        if (q * MI / QB == i) load_b(q);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (NA == 2 && more) {
+                vg_barrier();
+                load_slice_a();
+            }
         }
     }
+    __syncthreads();
 
-    // ---- epilogues.  This lane holds, for column n = n0 + 16 (NJ wn + j) + mp, the rows m = mb + 4 i + r.
-    const int64_t mb = m0 + wm * 128 + g4 * 32;
-    const int nb = wn * 16 * NJ + mp;
-    if constexpr (EPI == VG_LSE || EPI == VG_GRAD) {
-        float bias[MI][4];
+    // ---- epilogues
+    if constexpr (EPI == VG_LSE) {
+        float2* red = (float2*)lds;                     // [WM][TN]; the last barrier has passed
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-            const f32x4 v = *(const f32x4*)(p.bias + mb + 4 * i);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) bias[i][r] = v[r];
-        }
-        if constexpr (EPI == VG_LSE) {
-            float2* red = (float2*)lds;                 // [WM][TN]; the last barrier has passed
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int64_t n = n0 + nb + j * 16;
-                const bool there = n < n_lim;
-                const int64_t rel = there ? (int64_t)p.tgt[n] - p.v0 - mb : -1;
-                float top = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        acc[i][j][r] += bias[i][r];
-                        top = fmaxf(top, acc[i][j][r]);
-                    }
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float ref = top == -INFINITY ? 0.f : top;
-                float sum = 0.f, hit = 0.f;
-                bool any = false;
-#pragma unroll
-                for (int i = 0; i < MI; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        sum += lvae_exp2((acc[i][j][r] - ref) * LVAE_LOG2E);
-                        const bool is = rel == 4 * i + r;
-                        hit = is ? acc[i][j][r] : hit;
-                        any |= is;
-                    }
-                sum += __shfl_xor(sum, 16, 64);
-                sum += __shfl_xor(sum, 32, 64);
-                if (any) p.picked[n] = hit;
-                if (g4 == 0) red[wm * TN + nb + j * 16] = make_float2(top, sum);
-            }
-            __syncthreads();
-            for (int c = threadIdx.x; c < TN; c += 64 * W) {
-                if (n0 + c >= n_lim) continue;
-                float2 x = red[c];
-#pragma unroll
-                for (int w = 1; w < WM; ++w) {
-                    const float2 y = red[w * TN + c];
-                    const float top = fmaxf(x.x, y.x), ref = top == -INFINITY ? 0.f : top;
-                    x.y = x.y * lvae_exp2((x.x - ref) * LVAE_LOG2E) + y.y * lvae_exp2((y.x - ref) * LVAE_LOG2E);
-                    x.x = top;
-                }
-                p.part[(int64_t)tm * p.ldp + n0 + c] = x;
-            }
-        } else {
-            float colsum[MI][4];
+        for (int j = 0; j < NJ; ++j) {
+            const int64_t n = n0 + nb + j * 16;
+            const int64_t rel = n < n_lim ? (int64_t)p.tgt[n] - p.v0 - mb : -1;
+            float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) colsum[i][r] = 0.f;
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, acc[i][j][r]);
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float ref = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int64_t n = n0 + nb + j * 16;
-                const bool there = n < n_lim;           // rows behind the last kept token are written as zeros
-                const int64_t rel = there ? (int64_t)p.tgt[n] - p.v0 - mb : -1;
-                const float lse = there ? p.lse[n] : 0.f, gy = there ? p.gy[n] : 0.f;
-                uint16_t* row = p.g + n * p.ldg + mb;
+            for (int i = 0; i < MI; ++i)
 #pragma unroll
-                for (int i = 0; i < MI; i += 2) {
-                    s16x8 o[3];
+                for (int r = 0; r < 4; ++r) sum += lvae_exp2((acc[i][j][r] - ref) * LVAE_LOG2E);
+            sum += __shfl_xor(sum, 16, 64);
+            sum += __shfl_xor(sum, 32, 64);
+            if (__any(rel >= 0 && rel < 32)) {          // few tiles hold a target of theirs
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int ii = i + (e >> 2), r = e & 3;
-                        float x = lvae_exp2((acc[ii][j][r] + bias[ii][r] - lse) * LVAE_LOG2E);
-                        x = (rel == 4 * ii + r ? x - 1.f : x) * gy;
-                        x = there ? x : 0.f;
-                        colsum[ii][r] += x;
-                        if constexpr (DT == LVAE_F32) {
-                            uint16_t l[3];
-                            vg_limbs(x, l);
-                            o[0][e] = l[0]; o[1][e] = l[1]; o[2][e] = l[2];
-                        } else {
-                            // G is rounded once to the operand type, half a step of each element: the products need a
-                            // 16-bit operand, and the gradients are rounded to the same type themselves
-                            o[0][e] = vg_round<DT>(x);
-                        }
-                    }
+                for (int i = 0; i < MI; ++i)
 #pragma unroll
-                    for (int l = 0; l < (DT == LVAE_F32 ? 3 : 1); ++l) *(s16x8*)(row + l * p.plane_g + 4 * i) = o[l];
-                }
+                    for (int r = 0; r < 4; ++r)
+                        if (rel == 4 * i + r) p.picked[n] = acc[i][j][r];
             }
-            if (p.dbias) {
-                float* d = p.dbias + ((int64_t)tn * WN + wn) * p.ldg + mb;
+            if (g4 == 0) red[wm * TN + nb + j * 16] = make_float2(top, sum);
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < TN; c += 64 * W) {
+            if (n0 + c >= n_lim) continue;
+            float2 x = red[c];
 #pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    f32x4 v;
+            for (int w = 1; w < WM; ++w) {
+                const float2 y = red[w * TN + c];
+                const float top = fmaxf(x.x, y.x), ref = top == -INFINITY ? 0.f : top;
+                x.y = x.y * lvae_exp2((x.x - ref) * LVAE_LOG2E) + y.y * lvae_exp2((y.x - ref) * LVAE_LOG2E);
+                x.x = top;
+            }
+            p.part[(int64_t)tm * p.ldp + n0 + c] = x;
+        }
+    } else if constexpr (EPI == VG_GRAD) {
+        f32x4 colsum[MI];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = vg_row_sum(colsum[i][r]);
-                    if (mp == 0) *(f32x4*)(d + 4 * i) = v;
+        for (int i = 0; i < MI; ++i) colsum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int64_t n = n0 + nb + j * 16;
+            const bool there = n < n_lim;               // rows behind the last kept token are written as zeros
+            const int64_t rel = there ? (int64_t)p.tgt[n] - p.v0 - mb : -1;
+            const float lse = there ? p.lse[n] : 0.f, gy = there ? p.gy[n] : 0.f;
+            const bool all = n0 + (wn + 1) * 16 * NJ <= n_lim;
+            const bool hit = __any(rel >= 0 && rel < 32);
+            uint16_t* row = p.g + n * p.ldg + mb;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = lvae_exp2((acc[i][j][r] - lse) * LVAE_LOG2E);
+            }
+            if (hit) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] -= rel == 4 * i + r ? 1.f : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < MI; i += 2) {
+                s16x8 o[3];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int ii = i + (e >> 2), r = e & 3;
+                    float x = acc[ii][j][r] * gy;
+                    if (!all) x = there ? x : 0.f;
+                    colsum[ii][r] += x;
+                    if constexpr (DT == LVAE_F32) {
+                        uint16_t l[3];
+                        vg_limbs(x, l);
+                        o[0][e] = l[0]; o[1][e] = l[1]; o[2][e] = l[2];
+                    } else {
+                        // G is rounded once to the operand type, half a step of each element: the products need a
+                        // 16-bit operand, and the gradients are rounded to the same type themselves
+                        o[0][e] = vg_round<DT>(x);
+                    }
                 }
+#pragma unroll
+                for (int l = 0; l < (DT == LVAE_F32 ? 3 : 1); ++l) *(s16x8*)(row + l * p.plane_g + 4 * i) = o[l];
+            }
+        }
+        if (p.dbias) {
+            float* d = p.dbias + ((int64_t)tn * WN + wn) * p.ldg + mb;
+#pragma unroll
+            for (int i = 0; i < MI; ++i) {
+                f32x4 v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = vg_row_sum(colsum[i][r]);
+                if (mp == 0) *(f32x4*)(d + 4 * i) = v;
             }
         }
     } else if constexpr (EPI == VG_SLAB) {

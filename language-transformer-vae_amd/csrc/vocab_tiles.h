@@ -1,24 +1,25 @@
 // Launchers of the tile products of one element type; each vocab_tiles_*.hip defines VG_DT and VG_NAME and includes this.
 #include "vocab_gemm.h"
 
-template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ>
+
+template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
 static int vg_start(const VgArgs& p, hipStream_t st) {
     const int64_t blocks = lvae_round_up((int64_t)p.tiles_m * p.tiles_n * p.splits, 8);
-    vg_kernel<DT, TRA, TRB, EPI, WM, WN, NJ><<<dim3((unsigned)blocks), dim3(64 * WM * WN), 0, st>>>(p);
+    vg_kernel<DT, TRA, TRB, EPI, WM, WN, NJ, NA><<<dim3((unsigned)blocks), dim3(64 * WM * WN), 0, st>>>(p);
     LVAE_LAUNCH_CHECK();
     return LVAE_OK;
 }
 
-template <int DT, int WM, int WN, int NJ> static int vg_mode(int mode, const VgArgs& p, hipStream_t st) {
+template <int DT, int WM, int WN, int NJ, int NA> static int vg_mode(int mode, const VgArgs& p, hipStream_t st) {
     switch (mode) {
-        case VG_LOGITS_LSE: return vg_start<DT, false, false, VG_LSE, WM, WN, NJ>(p, st);
-        case VG_LOGITS_GRAD: return vg_start<DT, false, false, VG_GRAD, WM, WN, NJ>(p, st);
-        case VG_DHIDDEN: return vg_start<DT, true, false, VG_SLAB, WM, WN, NJ>(p, st);
-        case VG_DWEIGHT_SLAB: return vg_start<DT, true, true, VG_SLAB, WM, WN, NJ>(p, st);
-        default: return vg_start<DT, true, true, VG_OUT, WM, WN, NJ>(p, st);
+        case VG_LOGITS_LSE: return vg_start<DT, false, false, VG_LSE, WM, WN, NJ, NA>(p, st);
+        case VG_LOGITS_GRAD: return vg_start<DT, false, false, VG_GRAD, WM, WN, NJ, NA>(p, st);
+        case VG_DHIDDEN: return vg_start<DT, true, false, VG_SLAB, WM, WN, NJ, NA>(p, st);
+        case VG_DWEIGHT_SLAB: return vg_start<DT, true, true, VG_SLAB, WM, WN, NJ, NA>(p, st);
+        default: return vg_start<DT, true, true, VG_OUT, WM, WN, NJ, NA>(p, st);
     }
 }
 
 int VG_NAME(int mode, int narrow, const VgArgs& p, hipStream_t st) {
-    return narrow ? vg_mode<VG_DT, 2, 2, 2>(mode, p, st) : vg_mode<VG_DT, 2, 4, 4>(mode, p, st);
+    return narrow ? vg_mode<VG_DT, 2, 2, 2, 2>(mode, p, st) : vg_mode<VG_DT, 2, 4, 4, 3>(mode, p, st);
 }
