@@ -1,23 +1,25 @@
-// Norm of many tensors together, and clipping by it, in two launches per list (of up to 112 tensors a launch).
+// Norm of many tensors together, and clipping by it, in two launches.
 //
-//   1. norm_kernel: every workgroup takes a contiguous run of 8,192-element chunks of the list and leaves one partial
+//   1. norm_kernel: every workgroup takes a contiguous run of 2,048-element chunks of the list and leaves one partial
 //      (sum of squares in float64: no overflow or underflow of any float32 gradient, and an order of its own that never
 //      changes; or the largest magnitude).
 //   2. scale_kernel: every workgroup adds up all partials itself, in one order, so that no third launch or atomic is
 //      needed; where the factor is 1 nothing is read or written in place.
 //
 // Bound by memory: one read of all gradients for the norm, one read and write more where they are scaled.  The tensor
-// table travels as a kernel argument: no copy to the device, nothing to keep alive, and a captured graph holds it.
+// table travels as kernel arguments, so that nothing is copied from host memory and a captured graph holds it: up to 112
+// tensors in the arguments of the two kernels themselves; longer lists are first written to the workspace by launches
+// that only do that (2 us each), because one full launch over all tensors beats several of a part of the GPU each
+// (264 tensors, 60 M bfloat16 elements into float32: BEFORE us with a launch for each 112, AFTER us so).
 #include <stdlib.h>
 
 #include "vocab_gemm.h"
 
 namespace {
 
-constexpr int MAX_TENSORS = 112;            // 36 bytes each: below 4 KiB of kernel arguments
-constexpr int CHUNK = 8192;
-constexpr int BLOCKS = 2048;                // workgroups (and partials) over all launches of a list, or a few more
-constexpr int MIN_BLOCKS = 32;
+constexpr int MAX_TENSORS = 112;            // 33 bytes each: below 4 KiB of kernel arguments
+constexpr int CHUNK = 2048;                 // 8 elements a thread
+constexpr int BLOCKS = 2048;                // workgroups, and partials: 8 a CU
 
 struct Table {
     const void* src[MAX_TENSORS];
@@ -27,46 +29,67 @@ struct Table {
     uint8_t type[MAX_TENSORS];              // source type | destination type << 4
     int32_t count;
     uint32_t chunks;
+    int32_t out;                // whether some tensor goes elsewhere
 };
 static_assert(sizeof(Table) <= 4032, "kernel arguments");
 
-// eight elements from any element-aligned address (the compiler emits unaligned 16-byte accesses)
-typedef f32x4 __attribute__((aligned(4))) f32x4_u;
-typedef s16x8 __attribute__((aligned(2))) s16x8_u;
+// the same in the workspace
+struct LongTable {
+    const void** src;
+    void** dst;
+    int64_t* n;
+    uint32_t* first;
+    uint8_t* type;
+    int32_t count;
+    uint32_t chunks;
+    int32_t out;                // whether some tensor goes elsewhere
+};
 
-__device__ __forceinline__ void load8(const void* p, int64_t i, int dt, float x[8]) {
-    if (dt == LVAE_F32) {
-        const f32x4_u* q = (const f32x4_u*)((const float*)p + i);
-        const f32x4 a = q[0], b = q[1];
+__global__ __launch_bounds__(128) void table_kernel(Table t, LongTable l, int at) {
+    const int i = threadIdx.x;
+    if (i >= t.count) return;
+    l.src[at + i] = t.src[i];
+    l.dst[at + i] = t.dst[i];
+    l.n[at + i] = t.n[i];
+    l.first[at + i] = t.first[i];
+    l.type[at + i] = t.type[i];
+}
+
+// Eight elements of a full chunk: this thread's four of either half, so that the lanes of an access are neighbours in
+// float32 (16 bytes a lane) and in 16 bits (8 bytes).  Any element-aligned address (the compiler emits unaligned accesses).
+typedef f32x4 __attribute__((aligned(4))) f32x4_u;
+typedef s16x4 __attribute__((aligned(2))) s16x4_u;
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ void load8(const void* p, int64_t i0, int dt, float x[8]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
-    } else {
-        const s16x8 v = *(const s16x8_u*)((const uint16_t*)p + i);
-        if (dt == LVAE_BF16) {
+    for (int h = 0; h < 2; ++h) {
+        const int64_t i = i0 + h * (CHUNK / 2) + threadIdx.x * 4;
+        if (dt == LVAE_F32) {
+            const f32x4 a = *(const f32x4_u*)((const float*)p + i);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = vg_bf16((uint16_t)v[e]);
+            for (int e = 0; e < 4; ++e) x[4 * h + e] = a[e];
         } else {
-            const f16x8 h = __builtin_bit_cast(f16x8, v);
+            const s16x4 v = *(const s16x4_u*)((const uint16_t*)p + i);
+            const f16x4 f = __builtin_bit_cast(f16x4, v);      // the vector: a bit cast of its element reads element 0
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = (float)h[e];
+            for (int e = 0; e < 4; ++e) x[4 * h + e] = dt == LVAE_BF16 ? vg_bf16((uint16_t)v[e]) : (float)f[e];
         }
     }
 }
-__device__ __forceinline__ void store8(void* p, int64_t i, int dt, const float x[8]) {
-    if (dt == LVAE_F32) {
-        f32x4_u* q = (f32x4_u*)((float*)p + i);
-        q[0] = f32x4{x[0], x[1], x[2], x[3]};
-        q[1] = f32x4{x[4], x[5], x[6], x[7]};
-    } else {
-        s16x8 v;
-        if (dt == LVAE_BF16) {
+__device__ __forceinline__ void store8(void* p, int64_t i0, int dt, const float x[8]) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = vg_round<LVAE_BF16>(x[e]);
+    for (int h = 0; h < 2; ++h) {
+        const int64_t i = i0 + h * (CHUNK / 2) + threadIdx.x * 4;
+        if (dt == LVAE_F32) {
+            *(f32x4_u*)((float*)p + i) = f32x4{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
         } else {
+            s16x4 v;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = vg_round<LVAE_F16>(x[e]);
+            for (int e = 0; e < 4; ++e)
+                v[e] = (short)(dt == LVAE_BF16 ? vg_round<LVAE_BF16>(x[4 * h + e]) : vg_round<LVAE_F16>(x[4 * h + e]));
+            *(s16x4_u*)((uint16_t*)p + i) = v;
         }
-        *(s16x8_u*)((uint16_t*)p + i) = v;
     }
 }
 __device__ __forceinline__ float load1(const void* p, int64_t i, int dt) {
@@ -92,7 +115,7 @@ template <bool INF> __device__ __forceinline__ double block_join(double v, doubl
 }
 
 // the tensor that chunk c belongs to
-__device__ __forceinline__ int find(const Table& t, uint32_t c) {
+template <class T> __device__ __forceinline__ int find(const T& t, uint32_t c) {
     int lo = 0, hi = t.count - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -103,13 +126,13 @@ __device__ __forceinline__ int find(const Table& t, uint32_t c) {
 }
 
 // this workgroup's chunks, the same share for each
-__device__ __forceinline__ void my_chunks(const Table& t, uint32_t& c0, uint32_t& c1) {
+template <class T> __device__ __forceinline__ void my_chunks(const T& t, uint32_t& c0, uint32_t& c1) {
     const uint32_t each = t.chunks / gridDim.x, rest = t.chunks % gridDim.x, b = blockIdx.x;
     c0 = b * each + min(b, rest);
     c1 = c0 + each + (b < rest ? 1 : 0);
 }
 
-template <bool INF> __global__ __launch_bounds__(256) void norm_kernel(Table t, double* part) {
+template <bool INF, class T> __global__ __launch_bounds__(256) void norm_kernel(T t, double* part) {
     __shared__ double red[4];
     uint32_t c, c1;
     my_chunks(t, c, c1);
@@ -122,15 +145,12 @@ template <bool INF> __global__ __launch_bounds__(256) void norm_kernel(Table t, 
             const int dt = t.type[e] & 15;
             const int64_t i0 = (int64_t)(c - t.first[e]) * CHUNK, n = t.n[e];
             if (i0 + CHUNK <= n) {
+                float x[8];
+                load8(src, i0, dt, x);
 #pragma unroll
-                for (int u = 0; u < CHUNK / 2048; ++u) {
-                    float x[8];
-                    load8(src, i0 + u * 2048 + threadIdx.x * 8, dt, x);
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        if constexpr (INF) acc[k & 1] = nan_max(acc[k & 1], (double)fabsf(x[k]));
-                        else acc[k & 1] = fma((double)x[k], (double)x[k], acc[k & 1]);
-                    }
+                for (int k = 0; k < 8; ++k) {
+                    if constexpr (INF) acc[k & 1] = nan_max(acc[k & 1], (double)fabsf(x[k]));
+                    else acc[k & 1] = fma((double)x[k], (double)x[k], acc[k & 1]);
                 }
             } else {
                 for (int64_t i = i0 + threadIdx.x; i < n; i += 256) {
@@ -157,8 +177,8 @@ template <bool INF> __global__ __launch_bounds__(256) void total_kernel(const do
     if (threadIdx.x == 0) norm[0] = n;
 }
 
-template <bool INF> __global__ __launch_bounds__(256) void scale_kernel(Table t, const double* part, int parts, float max_norm,
-                                                                        float* norm) {
+template <bool INF, class T> __global__ __launch_bounds__(256) void scale_kernel(T t, const double* part, int parts, float max_norm,
+                                                                                 float* norm) {
     __shared__ double red[4];
     const float n_all = total<INF>(part, parts, red);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = n_all;
@@ -166,35 +186,27 @@ template <bool INF> __global__ __launch_bounds__(256) void scale_kernel(Table t,
     f = f > 1.f ? 1.f : f;                   // NaN stays
     uint32_t c, c1;
     my_chunks(t, c, c1);
-    if (c >= c1) return;
-    int e = find(t, c);
-    for (; c < c1; ++c) {
-        while (e + 1 < t.count && t.first[e + 1] <= c) ++e;
+    if (c >= c1 || (f == 1.f && !t.out)) return;
+    // backwards: what the norm has read last is still in the memory-side cache
+    int e = find(t, c1 - 1);
+    for (uint32_t k = c1; k > c;) {
+        --k;
+        while (t.first[e] > k) --e;
         const void* src = t.src[e];
         void* dst = t.dst[e];
         if (f == 1.f && dst == src) continue;
         const int dt = t.type[e] & 15, ot = t.type[e] >> 4;
-        const int64_t i0 = (int64_t)(c - t.first[e]) * CHUNK, n = t.n[e];
+        const int64_t i0 = (int64_t)(k - t.first[e]) * CHUNK, n = t.n[e];
         if (i0 + CHUNK <= n) {
+            float x[8];
+            load8(src, i0, dt, x);
 #pragma unroll
-            for (int u = 0; u < CHUNK / 2048; ++u) {
-                const int64_t i = i0 + u * 2048 + threadIdx.x * 8;
-                float x[8];
-                load8(src, i, dt, x);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] *= f;
-                store8(dst, i, ot, x);
-            }
+            for (int j = 0; j < 8; ++j) x[j] *= f;
+            store8(dst, i0, ot, x);
         } else {
             for (int64_t i = i0 + threadIdx.x; i < n; i += 256) store1(dst, i, ot, load1(src, i, dt) * f);
         }
     }
-}
-
-int64_t batches_of(int64_t count) { return count > 0 ? lvae_ceil_div(count, MAX_TENSORS) : 1; }
-int64_t blocks_of(int64_t count) {
-    const int64_t b = BLOCKS / batches_of(count);
-    return b < MIN_BLOCKS ? MIN_BLOCKS : b;
 }
 
 struct Span {
@@ -207,63 +219,88 @@ int by_start(const void* x, const void* y) {
     return p->a < q->a ? -1 : p->a > q->a;
 }
 
+void sort_spans(Span* s, int64_t n) {
+    for (int64_t i = 1; i < n; ++i)
+        if (s[i].a < s[i - 1].a) {
+            qsort(s, (size_t)n, sizeof(Span), by_start);
+            return;
+        }
+}
+
 int64_t size_of(int dt) { return dt == LVAE_F32 ? 4 : 2; }
 
 // no element that is written may belong to a second entry
 int check_overlap(const lvae_grad_entry* list, int64_t count, int scale) {
     if (!scale) return LVAE_OK;
-    Span* s = (Span*)malloc((size_t)(2 * count + 1) * sizeof(Span));
-    if (!s) return lvae_set_error(LVAE_ERR_INVALID, "out of host memory for %lld tensors", (long long)count);
-    int64_t m = 0;
+    // sources and destinations apart: either list is mostly in order already (views of one buffer), and needs no sorting
+    Span* buf = (Span*)malloc((size_t)(2 * count + 1) * sizeof(Span));
+    if (!buf) return lvae_set_error(LVAE_ERR_INVALID, "out of host memory for %lld tensors", (long long)count);
+    Span *s = buf, *d = buf + count;
+    int64_t ns = 0, nd = 0;
     for (int64_t i = 0; i < count; ++i) {
         if (list[i].n == 0) continue;
         const bool in_place = !list[i].dst || list[i].dst == list[i].src;
-        const uintptr_t p = (uintptr_t)list[i].src, d = (uintptr_t)list[i].dst;
-        s[m++] = Span{p, p + (uintptr_t)(list[i].n * size_of(list[i].dtype)), i, in_place};
-        if (!in_place) s[m++] = Span{d, d + (uintptr_t)(list[i].n * size_of(list[i].out_dtype)), i, 1};
+        const uintptr_t p = (uintptr_t)list[i].src, q = (uintptr_t)list[i].dst;
+        s[ns++] = Span{p, p + (uintptr_t)(list[i].n * size_of(list[i].dtype)), i, in_place};
+        if (!in_place) d[nd++] = Span{q, q + (uintptr_t)(list[i].n * size_of(list[i].out_dtype)), i, 1};
     }
-    qsort(s, (size_t)m, sizeof(Span), by_start);
+    sort_spans(s, ns);
+    sort_spans(d, nd);
     int64_t a = -1, b = -1;
     uintptr_t end = 0, end_w = 0;                          // of what lies before: anything, what is written
     int64_t who = -1, who_w = -1;
-    for (int64_t i = 0; i < m && a < 0; ++i) {
-        if (s[i].writes && end > s[i].a) { a = who; b = s[i].entry; }
-        else if (end_w > s[i].a) { a = who_w; b = s[i].entry; }
-        if (s[i].b > end) { end = s[i].b; who = s[i].entry; }
-        if (s[i].writes && s[i].b > end_w) { end_w = s[i].b; who_w = s[i].entry; }
+    for (int64_t i = 0, j = 0; i + j < ns + nd && a < 0;) {
+        const Span& x = j >= nd || (i < ns && s[i].a <= d[j].a) ? s[i++] : d[j++];
+        if (x.writes && end > x.a) { a = who; b = x.entry; }
+        else if (end_w > x.a) { a = who_w; b = x.entry; }
+        if (x.b > end) { end = x.b; who = x.entry; }
+        if (x.writes && x.b > end_w) { end_w = x.b; who_w = x.entry; }
     }
-    free(s);
+    free(buf);
     if (a >= 0) return lvae_set_error(LVAE_ERR_INVALID, "tensors %lld and %lld share memory that is written", (long long)a, (long long)b);
     return LVAE_OK;
 }
 
-// the table of entries [i0, ...) that fit one launch; returns the next entry
-int64_t fill(const lvae_grad_entry* list, int64_t count, int64_t i0, Table* t) {
+// the next entries from i0 on, at most MAX_TENSORS; chunks are counted over the whole list.  Returns the next entry.
+int64_t fill(const lvae_grad_entry* list, int64_t count, int64_t i0, uint32_t* chunks, Table* t) {
     t->count = 0;
-    t->chunks = 0;
     int64_t i = i0;
     for (; i < count && t->count < MAX_TENSORS; ++i) {
         const lvae_grad_entry& x = list[i];
         if (x.n == 0) continue;
-        const int64_t chunks = lvae_ceil_div(x.n, CHUNK);
-        if (t->count && (int64_t)t->chunks + chunks > 0x7FFFFFFF) break;
         const int k = t->count++;
         t->src[k] = x.src;
         t->dst[k] = x.dst ? x.dst : (void*)x.src;
         t->n[k] = x.n;
-        t->first[k] = t->chunks;
+        t->first[k] = *chunks;
         t->type[k] = (uint8_t)(x.dtype | (x.dst ? x.out_dtype : x.dtype) << 4);
-        t->chunks += (uint32_t)chunks;
+        *chunks += (uint32_t)lvae_ceil_div(x.n, CHUNK);
     }
+    t->chunks = *chunks;
+    t->out = 0;
+    for (int k = 0; k < t->count; ++k) t->out |= t->dst[k] != t->src[k];
     return i;
+}
+
+constexpr int64_t PART_BYTES = BLOCKS * 8;
+int64_t long_bytes(int64_t count) { return lvae_round_up(count * (8 + 8 + 8 + 4 + 1) + 256, 256); }
+
+template <bool INF, class T>
+int launch(const T& t, int scale, float max_norm, double* part, float* norm, hipStream_t st) {
+    const int g = (int)(t.chunks < BLOCKS ? t.chunks : BLOCKS);
+    norm_kernel<INF, T><<<dim3((unsigned)g), 256, 0, st>>>(t, part);
+    LVAE_LAUNCH_CHECK();
+    if (scale) scale_kernel<INF, T><<<dim3((unsigned)g), 256, 0, st>>>(t, part, g, max_norm, norm);
+    else total_kernel<INF><<<1, 256, 0, st>>>(part, g, norm);
+    LVAE_LAUNCH_CHECK();
+    return LVAE_OK;
 }
 
 }  // namespace
 
 extern "C" int lvae_clip_workspace_bytes(int64_t count, int64_t* out_bytes) {
-    LVAE_CHECK_ARG(out_bytes && count >= 0, "bad arguments: count=%lld", (long long)count);
-    // one launch more than the count says, should a table end early at its chunk limit
-    *out_bytes = lvae_round_up((batches_of(count) * 2 + 1) * blocks_of(count) * 8, 256);
+    LVAE_CHECK_ARG(out_bytes && count >= 0 && count <= (1 << 24), "bad arguments: count=%lld", (long long)count);
+    *out_bytes = PART_BYTES + (count > MAX_TENSORS ? long_bytes(count) : 0);
     return LVAE_OK;
 }
 
@@ -275,6 +312,7 @@ extern "C" int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int i
     LVAE_CHECK_ARG(count == 0 || list, "list must be non-NULL");
     LVAE_CHECK_ARG(norm, "norm must be non-NULL");
     LVAE_CHECK_ARG(!scale || max_norm >= 0.0, "max_norm must not be negative or NaN");
+    int64_t chunks = 0;
     for (int64_t i = 0; i < count; ++i) {
         const lvae_grad_entry& x = list[i];
         LVAE_CHECK_ARG(x.n >= 0 && x.n < (1ll << 43), "tensor %lld: bad size %lld", (long long)i, (long long)x.n);
@@ -284,7 +322,9 @@ extern "C" int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int i
         LVAE_CHECK_ARG(x.dst != x.src || x.out_dtype == x.dtype, "tensor %lld: in place in another type", (long long)i);
         LVAE_CHECK_ARG(((uintptr_t)x.src % size_of(x.dtype)) == 0 && (!x.dst || ((uintptr_t)x.dst % size_of(x.out_dtype)) == 0),
                        "tensor %lld: not aligned to its elements", (long long)i);
+        chunks += lvae_ceil_div(x.n, CHUNK);
     }
+    LVAE_CHECK_ARG(chunks < (1ll << 31), "too many elements");
     const int rc2 = check_overlap(list, count, scale);
     if (rc2 != LVAE_OK) return rc2;
     if (!ws) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace is NULL (%lld bytes needed)", (long long)need);
@@ -292,35 +332,35 @@ extern "C" int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int i
     if (ws_bytes < need) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace too small: %lld < %lld bytes", (long long)ws_bytes, (long long)need);
     hipStream_t st = (hipStream_t)stream;
     double* part = (double*)ws;
-    const int64_t blocks = blocks_of(count), room = need / 8;
-    int64_t parts = 0;
+    const float bound = (float)max_norm;
     Table t;
-    for (int64_t i = 0; i < count;) {
-        i = fill(list, count, i, &t);
-        if (t.count == 0) continue;
-        const int64_t g = t.chunks < blocks ? t.chunks : blocks;
-        if (parts + g > room) return lvae_set_error(LVAE_ERR_UNSUPPORTED, "more than 2^31 chunks of gradients in one list");
-        if (inf_norm) norm_kernel<true><<<dim3((unsigned)g), 256, 0, st>>>(t, part + parts);
-        else norm_kernel<false><<<dim3((unsigned)g), 256, 0, st>>>(t, part + parts);
+    uint32_t at = 0;
+    int64_t i = fill(list, count, 0, &at, &t);
+    if (t.count == 0) {                                    // nothing but empty tensors
+        total_kernel<false><<<1, 256, 0, st>>>(part, 0, norm);
         LVAE_LAUNCH_CHECK();
-        parts += g;
+        return LVAE_OK;
     }
-    bool said = false;
-    if (scale)
-        for (int64_t i = 0; i < count;) {
-            i = fill(list, count, i, &t);
-            if (t.count == 0) continue;
-            const int64_t g = t.chunks < blocks ? t.chunks : blocks;
-            float* out = said ? nullptr : norm;
-            said = true;
-            if (inf_norm) scale_kernel<true><<<dim3((unsigned)g), 256, 0, st>>>(t, part, (int)parts, (float)max_norm, out);
-            else scale_kernel<false><<<dim3((unsigned)g), 256, 0, st>>>(t, part, (int)parts, (float)max_norm, out);
+    if (i == count)
+        return inf_norm ? launch<true>(t, scale, bound, part, norm, st) : launch<false>(t, scale, bound, part, norm, st);
+    char* p = (char*)ws + PART_BYTES;
+    LongTable l;
+    l.src = (const void**)p;
+    l.dst = (void**)(p + count * 8);
+    l.n = (int64_t*)(p + count * 16);
+    l.first = (uint32_t*)(p + count * 24);
+    l.type = (uint8_t*)(p + count * 28);
+    l.count = l.out = 0;
+    for (;;) {
+        if (t.count) {
+            table_kernel<<<1, 128, 0, st>>>(t, l, l.count);
             LVAE_LAUNCH_CHECK();
+            l.count += t.count;
+            l.out |= t.out;
         }
-    if (!said) {
-        if (inf_norm) total_kernel<true><<<1, 256, 0, st>>>(part, (int)parts, norm);
-        else total_kernel<false><<<1, 256, 0, st>>>(part, (int)parts, norm);
-        LVAE_LAUNCH_CHECK();
+        if (i == count) break;
+        i = fill(list, count, i, &at, &t);
     }
-    return LVAE_OK;
+    l.chunks = at;
+    return inf_norm ? launch<true>(l, scale, bound, part, norm, st) : launch<false>(l, scale, bound, part, norm, st);
 }
