@@ -57,8 +57,6 @@ __global__ __launch_bounds__(128) void table_kernel(Table t, LongTable l, int at
 
 // Eight elements of a full chunk: this thread's four of either half, so that the lanes of an access are neighbours in
 // float32 (16 bytes a lane) and in 16 bits (8 bytes).  Any element-aligned address (the compiler emits unaligned accesses).
-typedef f32x4 __attribute__((aligned(4))) f32x4_u;
-typedef s16x4 __attribute__((aligned(2))) s16x4_u;
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ void load8(const void* p, int64_t i0, int dt, float x[8]) {

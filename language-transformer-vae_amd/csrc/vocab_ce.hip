@@ -13,6 +13,13 @@
 int lvae_vg_launch_bf16(int mode, int narrow, const VgArgs& p, hipStream_t st);
 int lvae_vg_launch_f16(int mode, int narrow, const VgArgs& p, hipStream_t st);
 int lvae_vg_launch_f32(int mode, int narrow, const VgArgs& p, hipStream_t st);
+int lvae_vg_launch_both_bf16(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st);
+int lvae_vg_launch_both_f16(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st);
+int lvae_vg_launch_both_f32(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st);
+
+#ifndef VOCAB_G_MIB
+#define VOCAB_G_MIB 512ll
+#endif
 
 namespace {
 
@@ -24,8 +31,9 @@ struct Axes {
     int64_t size[3], stride[3];
 };
 __device__ __forceinline__ int64_t at_axes(const Axes& a, int64_t t) {
-    const int64_t k = t % a.size[2], r = t / a.size[2];
-    return (r / a.size[1]) * a.stride[0] + (r % a.size[1]) * a.stride[1] + k * a.stride[2];
+    // there are fewer than 2^31 tokens: 32-bit divisions
+    const unsigned u = (unsigned)t, s2 = (unsigned)a.size[2], s1 = (unsigned)a.size[1], r = u / s2, q = r / s1;
+    return q * a.stride[0] + (r - q * s1) * a.stride[1] + (u - r * s2) * a.stride[2];
 }
 
 template <int DT> __device__ __forceinline__ float load_as_float(const void* p, int64_t i) {
@@ -66,11 +74,21 @@ struct RowsArgs {
     float *lse_of, *gy_of, *unscale;
     float *ll, *lse_out;        // forward: zeros for tokens that do not count
     int* n_rows;
+    // the other workgroups of the launch
+    int row_blocks, bias_blocks;
+    const void* bias;
+    float* bias_out;
+    int bias_dtype;
+    int64_t Vpad;
+    const void* weight;         // copied where the tiles cannot read it as it lies, or NULL
+    uint16_t* wpack;
+    int64_t wstride;
+    int H, Kp;
 };
 
 // One workgroup per 1,024 tokens.  Each counts the kept tokens before its own by itself (targets are 8 bytes a token
 // and stay in L2; at 65,536 tokens the last workgroup reads 512 KB) instead of a second launch for the prefix.
-__global__ __launch_bounds__(1024) void rows_kernel(RowsArgs p) {
+__device__ __forceinline__ void list_rows(const RowsArgs& p) {
     __shared__ int red[16];
     __shared__ float redf[16];
     const int64_t first = (int64_t)blockIdx.x * 1024;
@@ -125,39 +143,24 @@ __global__ __launch_bounds__(1024) void rows_kernel(RowsArgs p) {
             if (p.lse_out) p.lse_out[t] = 0.f;
         }
     }
-    if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) p.n_rows[0] = before + all;
+    if ((int)blockIdx.x == p.row_blocks - 1 && threadIdx.x == 0) p.n_rows[0] = before + all;
 }
 
-// Rows of hidden (listed, zeros behind the last up to a whole tile) or of W (strided) as the tile products read them:
-// Kp columns, zero behind H; float32 as three limb planes.  One wave per row.
-template <int DT> __global__ __launch_bounds__(256) void pack_kernel(const void* src, const int64_t* off, int64_t stride,
-                                                                     const int* n_rows, int64_t rows, int H, int Kp,
-                                                                     uint16_t* out, int64_t plane) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= rows) return;
-    const int lane = threadIdx.x & 63;
-    bool there = true;
-    if (off) {
-        const int64_t n = n_rows[0];
-        if (r >= (n + 255) / 256 * 256) return;
-        there = r < n;
-    }
-    const int64_t base = there ? (off ? off[r] : r * stride) : 0;
-    uint16_t* o = out + r * Kp;
-    constexpr int SZ = DT == LVAE_F32 ? 4 : 2;
-    const bool vec = ((((uintptr_t)src + base * SZ) & 15) == 0) && H % 8 == 0;       // of this row
-    for (int k = lane * 8; k < Kp; k += 512) {
-        float x[8];
-        s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+// Row r of hidden (listed, zeros behind the last up to a whole tile) or of W as the tile products read it: Kp columns, zero
+// behind H; float32 as three limb planes.  One wave per row.
+template <int DT> __device__ __forceinline__ void pack_row(const void* src, int64_t base, bool there, int H, int Kp, uint16_t* o, int64_t plane) {
+    for (int k = (threadIdx.x & 63) * 8; k < Kp; k += 512) {
         if constexpr (DT == LVAE_F32) {
+            const float* q = (const float*)src + base + k;
+            float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = 0.f;
-            if (there && vec && k < H) {
-                const f32x4 a = *(const f32x4*)((const float*)src + base + k), b = *(const f32x4*)((const float*)src + base + k + 4);
+            if (there && k + 8 <= H) {
+                const f32x4 a = *(const f32x4_u*)q, b = *(const f32x4_u*)(q + 4);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
             } else if (there) {
-                for (int e = 0; e < 8; ++e) if (k + e < H) x[e] = ((const float*)src)[base + k + e];
+                for (int e = 0; e < 8; ++e) if (k + e < H) x[e] = q[e];
             }
             s16x8 w[3];
 #pragma unroll
@@ -169,19 +172,37 @@ template <int DT> __global__ __launch_bounds__(256) void pack_kernel(const void*
 #pragma unroll
             for (int l = 0; l < 3; ++l) *(s16x8*)(o + l * plane + k) = w[l];
         } else {
-            if (there && vec && k < H) v = *(const s16x8*)((const uint16_t*)src + base + k);
+            const uint16_t* q = (const uint16_t*)src + base + k;
+            s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (there && k + 8 <= H) v = *(const s16x8_u*)q;
             else if (there) {
-                for (int e = 0; e < 8; ++e) if (k + e < H) v[e] = ((const uint16_t*)src)[base + k + e];
+                for (int e = 0; e < 8; ++e) if (k + e < H) v[e] = q[e];
             }
             *(s16x8*)(o + k) = v;
         }
     }
 }
 
-// bias in float32, -inf behind the vocabulary: what the tiles add, so that no word beyond the last can count
-__global__ __launch_bounds__(256) void bias_kernel(const void* bias, int dt, int64_t V, int64_t Vpad, float* out) {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v < Vpad) out[v] = v >= V ? -INFINITY : bias ? load_any(bias, v, dt) : 0.f;
+template <int DT> __global__ __launch_bounds__(256) void pack_kernel(const void* src, const int64_t* off, const int* n_rows, int64_t rows,
+                                                                     int H, int Kp, uint16_t* out, int64_t plane) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = n_rows[0];
+    if (r >= rows || r >= (n + 255) / 256 * 256) return;
+    const bool there = r < n;
+    pack_row<DT>(src, there ? off[r] : 0, there, H, Kp, out + r * Kp, plane);
+}
+
+// What the products need and does not depend on each other, in one launch: the list of tokens, the bias in float32 with
+// -inf behind the vocabulary (no word beyond the last can count), and the padded copy of W where one is needed.
+template <int DT> __global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
+    if ((int)blockIdx.x < p.row_blocks) {
+        list_rows(p);
+    } else if ((int)blockIdx.x < p.row_blocks + p.bias_blocks) {
+        const int64_t v = (int64_t)(blockIdx.x - p.row_blocks) * 1024 + threadIdx.x;
+        if (v < p.Vpad) p.bias_out[v] = v >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v, p.bias_dtype) : 0.f;
+    } else {
+        const int64_t r = (int64_t)(blockIdx.x - p.row_blocks - p.bias_blocks) * 16 + (threadIdx.x >> 6);
+        if (r < p.V) pack_row<DT>(p.weight, r * p.wstride, true, p.H, p.Kp, p.wpack + r * p.Kp, p.V * p.Kp);
+    }
 }
 
 __device__ __forceinline__ float2 merge_lse(float2 a, float2 b) {
@@ -189,21 +210,28 @@ __device__ __forceinline__ float2 merge_lse(float2 a, float2 b) {
     return make_float2(top, a.y * lvae_exp2((a.x - ref) * LVAE_LOG2E) + b.y * lvae_exp2((b.x - ref) * LVAE_LOG2E));
 }
 
-// LSE of each kept token from its partials [tiles][ldp]; 32 tokens a workgroup, 8 threads a token
+// LSE of each kept token from its partials [tiles][ldp]; 16 tokens a workgroup, 16 threads a token
 __global__ __launch_bounds__(256) void finish_kernel(const float2* part, int tiles, int64_t ldp, const float* picked,
                                                      const int* tok, const int* tgt, const int* n_rows, float* ll,
                                                      float* lse) {
-    __shared__ float2 red[8][32];
-    const int64_t j = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int g = threadIdx.x >> 5;
+    __shared__ float2 red[16][16];
+    const int64_t j = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+    const int g = threadIdx.x >> 4;
     const int64_t n = n_rows[0];
     float2 x = make_float2(-INFINITY, 0.f);
     if (j < n)
-        for (int i = g; i < tiles; i += 8) x = merge_lse(x, part[(int64_t)i * ldp + j]);
-    red[g][threadIdx.x & 31] = x;
+        for (int i = g; i < tiles; i += 64) {
+            float2 y[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                y[u] = i + 16 * u < tiles ? part[(int64_t)(i + 16 * u) * ldp + j] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x = merge_lse(x, y[u]);
+        }
+    red[g][threadIdx.x & 15] = x;
     __syncthreads();
     if (g == 0 && j < n) {
-        for (int i = 1; i < 8; ++i) x = merge_lse(x, red[i][threadIdx.x]);
+        for (int i = 1; i < 16; ++i) x = merge_lse(x, red[i][threadIdx.x]);
         float l = x.x + logf(x.y);
         const bool bad = tgt[j] < 0;
         if (bad) l = NAN;
@@ -213,9 +241,11 @@ __global__ __launch_bounds__(256) void finish_kernel(const float2* part, int til
 }
 
 // ---- few tokens: W streamed once -------------------------------------------------------------------------------
-// A wave owns 16 words; its A operand comes from memory in registers (a lane reads 32 consecutive bytes of its word's
-// row: 128 bytes a row and step), the tokens' rows are its B operand.  The order of the summed index inside a step is
-// the lanes' own (the same on both sides).  Bound by the read of W.
+// A wave owns 16 words, whose rows come from memory into registers as they lie in the instruction's operand (a lane reads
+// 32 consecutive bytes of its word's row: 128 bytes a row and step), four steps ahead of their use.  The tokens' rows go
+// through LDS, four steps at a time, shared by the four waves: read from memory by every wave they cost more accesses of
+// the first-level cache than W (24 float32 tokens: 66 us so, 48 us through LDS).  The order of the summed index inside
+// a step is the lanes' own, the same on both sides.  Bound by the read of W.
 template <int DT> struct FewStep {
     static constexpr int K = DT == LVAE_F32 ? 32 : 64, LANE = K / 4;       // elements a step, and a lane's share
 };
@@ -231,12 +261,16 @@ template <int DT, bool ALIGNED> __device__ __forceinline__ void few_load(const v
             const f32x4 v = *(const f32x4*)((const char*)row + (at < H ? at : 0) * SZ);
             out[h] = at < H ? v : out[h];
         } else if constexpr (DT == LVAE_F32) {
+            if (at + 4 <= H) out[h] = *(const f32x4_u*)((const float*)row + at);
+            else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) if (at + e < H) out[h][e] = ((const float*)row)[at + e];
+                for (int e = 0; e < 4; ++e) if (at + e < H) out[h][e] = ((const float*)row)[at + e];
         } else {
             s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (at + 8 <= H) v = *(const s16x8_u*)((const uint16_t*)row + at);
+            else
 #pragma unroll
-            for (int e = 0; e < 8; ++e) if (at + e < H) v[e] = ((const uint16_t*)row)[at + e];
+                for (int e = 0; e < 8; ++e) if (at + e < H) v[e] = ((const uint16_t*)row)[at + e];
             out[h] = __builtin_bit_cast(f32x4, v);
         }
     }
@@ -266,44 +300,71 @@ struct FewArgs {
 
 template <int DT, int NT, bool ALIGNED> __global__ __launch_bounds__(256) void few_kernel(FewArgs p) {
     constexpr int SZ = DT == LVAE_F32 ? 4 : 2, KS = FewStep<DT>::K, KL = FewStep<DT>::LANE;
+    constexpr int U = 4, PITCH = U * 128 + 16;          // steps a round; a token's bytes of one in LDS
     __shared__ float2 red[4][NT * 16];
+    __shared__ __align__(16) char tok[2][NT * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mp = lane & 15, g4 = lane >> 4;
     const int64_t vw = ((int64_t)blockIdx.x * 4 + wave) * 16;
     const char* wrow = (const char*)p.weight + min(vw + mp, p.V - 1) * p.wstride * SZ;
-    const char* hrow[NT];
+    const char* trow[NT];                   // rows that this thread brings into LDS: 32 bytes of each a round
 #pragma unroll
-    for (int n = 0; n < NT; ++n) hrow[n] = (const char*)p.hidden + at_axes(p.hid, min(n * 16 + mp, p.T - 1)) * SZ;
+    for (int i = 0; i < NT; ++i)
+        trow[i] = (const char*)p.hidden + at_axes(p.hid, min(i * 16 + (int)(threadIdx.x >> 4), p.T - 1)) * SZ;
     f32x4 acc[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    constexpr int U = ALIGNED ? 4 : 1;      // steps whose loads of W are in flight together
-    for (int k0 = 0; k0 < p.H; k0 += U * KS) {
-        f32x4 a[U][2];
+
+    f32x4 a[U][2], an[U][2], bt[NT][2];
+    auto load_w = [&](int k0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) few_load<DT, ALIGNED>(wrow, k0 + u * KS + g4 * KL, p.H, a[u]);
+        for (int u = 0; u < U; ++u) few_load<DT, ALIGNED>(wrow, k0 + u * KS + g4 * KL, p.H, an[u]);
+    };
+    auto load_t = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) few_load<DT, ALIGNED>(trow[i], k0 + (threadIdx.x & 15) * KL, p.H, bt[i]);
+    };
+    auto store_t = [&](int to) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            char* q = tok[to] + (i * 16 + (threadIdx.x >> 4)) * PITCH + (threadIdx.x & 15) * 32;
+            *(f32x4*)q = bt[i][0];
+            *(f32x4*)(q + 16) = bt[i][1];
+        }
+    };
+    load_t(0);
+    load_w(0);
+    store_t(0);
+    int buf = 0;
+    for (int k0 = 0; k0 < p.H; k0 += U * KS) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) { a[u][0] = an[u][0]; a[u][1] = an[u][1]; }
+        __syncthreads();
+        const bool more = k0 + U * KS < p.H;
+        if (more) { load_t(k0 + U * KS); load_w(k0 + U * KS); }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                f32x4 b[2];
-                few_load<DT, ALIGNED>(hrow[n], k0 + u * KS + g4 * KL, p.H, b);
+                const char* q = tok[buf] + (n * 16 + mp) * PITCH + u * 128 + g4 * 32;
+                const f32x4 b[2] = {*(const f32x4*)q, *(const f32x4*)(q + 16)};
                 acc[n] = few_mma<DT>(a[u], b, acc[n]);
             }
+        buf ^= 1;
+        if (more) store_t(buf);             // the other buffer: its readers have passed the barrier above
     }
     const int64_t v0 = vw + g4 * 4;
     float bias[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) bias[r] = v0 + r >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v0 + r, p.bias_dtype) : 0.f;
+    for (int r = 0; r < 4; ++r) bias[r] = v0 + r < p.V && p.bias ? load_any(p.bias, v0 + r, p.bias_dtype) : 0.f;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int t = n * 16 + mp;
-        const int64_t rel = t < p.T ? p.targets[at_axes(p.tgt, t)] - v0 : -1;
+        const int64_t y = t < p.T ? p.targets[at_axes(p.tgt, t)] : -1;
         float x[4], top = -INFINITY;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            x[r] = acc[n][r] + bias[r];
-            if (v0 + r >= p.V) x[r] = -INFINITY;
-            if (rel == r && v0 + r < p.V) p.picked[t] = x[r];
+            x[r] = v0 + r < p.V ? acc[n][r] + bias[r] : -INFINITY;
+            if (y == v0 + r && v0 + r < p.V) p.picked[t] = x[r];
             top = fmaxf(top, x[r]);
         }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
@@ -355,31 +416,57 @@ __global__ __launch_bounds__(256) void few_finish_kernel(const float2* part, int
 }
 
 // ---- backward: sums of the partial products ----------------------------------------------------------------------
-// d_hidden of every token: the slabs of its row, in order; zeros where the token does not count
-__global__ __launch_bounds__(256) void dhidden_kernel(const float* slab, int splits, int64_t slab_stride, int64_t ld,
-                                                      const int* inv, int64_t T, int H, const float* unscale, void* out,
-                                                      int dt) {
-    const int per = (H + 3) / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= T * per) return;
-    const int64_t t = i / per;
-    const int h = (int)(i - t * per) * 4;
-    const int j = inv[t];
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (j >= 0) {
-        for (int s = 0; s < splits; ++s) x += *(const f32x4*)(slab + s * slab_stride + j * ld + h);
-        if (unscale) x *= unscale[0];
-    }
-    const int64_t o = t * H + h;
-    if (H % 4 == 0 && dt == LVAE_F32) { *(f32x4*)((float*)out + o) = x; return; }
-    if (H % 4 == 0) {
-        s16x4 v;
+struct FinalArgs {
+    const float* slab;          // d_hidden: the slabs of a token's row, in order; zeros where the token does not count
+    int64_t slab_stride, ld, T;
+    const int* inv;
+    int splits, H, dt, hidden_blocks;
+    void* d_hidden;
+    const float* part;          // d_bias: the partial column sums of the tiles that hold kept tokens
+    int64_t ld_part, V;
+    int per_tile, tile_rows, bias_dt;
+    void* d_bias;
+    const int* n_rows;
+    const float* unscale;
+};
+__global__ __launch_bounds__(256) void final_kernel(FinalArgs p) {
+    __shared__ double red[8][32];
+    if ((int)blockIdx.x < p.hidden_blocks) {
+        const unsigned per = (p.H + 3) / 4;
+        const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+        if (i >= p.T * per) return;
+        const int64_t t = i / per;
+        const int h = (int)(i - t * per) * 4, j = p.inv[t];
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        if (j >= 0) {
+            for (int s = 0; s < p.splits; ++s) x += *(const f32x4*)(p.slab + s * p.slab_stride + j * p.ld + h);
+            if (p.unscale) x *= p.unscale[0];
+        }
+        const int64_t o = t * p.H + h;
+        if (h + 4 > p.H) {
+            for (int e = 0; e < 4; ++e) if (h + e < p.H) store_any(p.d_hidden, o + e, x[e], p.dt);
+        } else if (p.dt == LVAE_F32) {
+            *(f32x4_u*)((float*)p.d_hidden + o) = x;
+        } else {
+            s16x4 v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = dt == LVAE_BF16 ? vg_round<LVAE_BF16>(x[e]) : vg_round<LVAE_F16>(x[e]);
-        *(s16x4*)((uint16_t*)out + o) = v;
+            for (int e = 0; e < 4; ++e) v[e] = p.dt == LVAE_BF16 ? vg_round<LVAE_BF16>(x[e]) : vg_round<LVAE_F16>(x[e]);
+            *(s16x4_u*)((uint16_t*)p.d_hidden + o) = v;
+        }
         return;
     }
-    for (int e = 0; e < 4; ++e) if (h + e < H) store_any(out, o + e, x[e], dt);
+    const int64_t v = (int64_t)(blockIdx.x - p.hidden_blocks) * 32 + (threadIdx.x & 31);
+    const int g = threadIdx.x >> 5;
+    const int n = (p.n_rows[0] + p.tile_rows - 1) / p.tile_rows * p.per_tile;
+    double x = 0.0;
+    if (v < p.V)
+        for (int i = g; i < n; i += 8) x += p.part[(int64_t)i * p.ld_part + v];
+    red[g][threadIdx.x & 31] = x;
+    __syncthreads();
+    if (g || v >= p.V) return;
+    for (int i = 1; i < 8; ++i) x += red[i][threadIdx.x];
+    const float f = (float)x;
+    store_any(p.d_bias, v, p.unscale ? f * p.unscale[0] : f, p.bias_dt);
 }
 
 // rows [0, rows) of the split weight gradient
@@ -392,24 +479,6 @@ __global__ __launch_bounds__(256) void dweight_kernel(const float* slab, int spl
     float x = 0.f;
     for (int s = 0; s < splits; ++s) x += slab[s * slab_stride + v * ld + h];
     store_any(out, i, unscale ? x * unscale[0] : x, dt);
-}
-
-// d_bias of a piece: the partial column sums of the tiles that hold kept tokens
-__global__ __launch_bounds__(256) void dbias_kernel(const float* part, int64_t ld, int per_tile, int tile_rows, const int* n_rows,
-                                                    int64_t rows, const float* unscale, void* out, int dt, int64_t v0) {
-    __shared__ double red[8][32];
-    const int64_t v = (int64_t)blockIdx.x * 32 + (threadIdx.x & 31);
-    const int g = threadIdx.x >> 5;
-    const int n = (n_rows[0] + tile_rows - 1) / tile_rows * per_tile;
-    double x = 0.0;
-    if (v < rows)
-        for (int i = g; i < n; i += 8) x += part[(int64_t)i * ld + v];
-    red[g][threadIdx.x & 31] = x;
-    __syncthreads();
-    if (g || v >= rows) return;
-    for (int i = 1; i < 8; ++i) x += red[i][threadIdx.x];
-    const float f = (float)x;
-    store_any(out, v0 + v, unscale ? f * unscale[0] : f, dt);
 }
 
 __global__ __launch_bounds__(256) void segment_sum_kernel(const float* x, int64_t n, int64_t len, float* out) {
@@ -527,31 +596,35 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     pl->inv = take(at, pl->T * 4);
     pl->lse = take(at, pl->Tpad * 4);
     pl->gy = take(at, pl->Tpad * 4);
-    // pieces of the vocabulary: G of one piece takes at most 512 MiB, and every piece is as large as the others
+    // pieces of the vocabulary: G of one piece takes at most 512 MiB, and every piece is as large as the others.  Fewer
+    // pieces mean fewer rounds of tiles that do not fill the GPU, and fewer additions to the slabs of dHidden
     const int64_t per_word = pl->Tpad * pl->planes * 2;
-    int64_t piece = (512ll << 20) / per_word / 256 * 256;
+    int64_t piece = (VOCAB_G_MIB << 20) / per_word / 256 * 256;
     if (piece < 1024) piece = 1024;
-    if (piece > 32768) piece = 32768;
+    if (piece > 1 << 20) piece = 1 << 20;
     const int64_t pieces = lvae_ceil_div(pl->Vpad, piece);
     pl->piece = lvae_round_up(lvae_ceil_div(pl->V, pieces), 256);
     pl->g = take(at, pl->planes * pl->Tpad * pl->piece * 2);
     const int64_t th = lvae_ceil_div(pl->H, 256);
-    // few output tiles and a long sum: the sum is split so that the launch fills the 256 CUs
+    // the sum of d_hidden runs over the whole piece: it is split so that no tile takes more than 0.6 of a CU's share of the
+    // launch that holds both products
     const int64_t tiles_h = th * lvae_ceil_div(pl->T, pl->tile_n), tiles_w = th * lvae_ceil_div(pl->piece, 256);
-    pl->splits_h = (int)lvae_ceil_div(256, tiles_h);
-    const int64_t most_h = lvae_ceil_div(pl->piece, 512);
-    if (pl->splits_h > most_h) pl->splits_h = (int)most_h;
+    const int64_t ks_h = lvae_ceil_div(pl->piece, VG_BK), ks_w = lvae_ceil_div(pl->T, VG_BK);
+    const int64_t share = (tiles_h * ks_h + tiles_w * ks_w) / 256 + 1;      // slices a CU, both products
+    int64_t most = share * 6 / 10;
+    if (most < 16) most = 16;
+    pl->splits_h = (int)lvae_ceil_div(ks_h, most);
     if (pl->splits_h > 32) pl->splits_h = 32;
+    // the weight gradient's sum is split only where both products together leave CUs without a tile: its slabs are as
+    // large as the gradient itself
     pl->splits_w = 1;
-    if (tiles_w <= 128 && pl->T >= 1024) {
-        pl->splits_w = (int)(256 / tiles_w);
-        const int64_t most_w = pl->T / 512;
-        if (pl->splits_w > most_w) pl->splits_w = (int)most_w;
+    if (tiles_w + tiles_h * pl->splits_h < 192 && ks_w > most) {
+        pl->splits_w = (int)lvae_ceil_div(ks_w, most);
         if (pl->splits_w > 32) pl->splits_w = 32;
     }
     pl->slab = want_h ? take(at, pl->splits_h * pl->Tpad * pl->Kp * 4) : 0;
     pl->slab_w = want_w && pl->splits_w > 1 ? take(at, pl->splits_w * pl->piece * pl->Kp * 4) : 0;
-    pl->dbias = want_b ? take(at, pl->Tpad / pl->tile_n * 4 * pl->piece * 4) : 0;
+    pl->dbias = want_b ? take(at, pl->Tpad / pl->tile_n * (pl->narrow ? 2 : 4) * pl->Vpad * 4) : 0;
     pl->bytes = at;
 }
 
@@ -582,38 +655,50 @@ int launch_tiles(int dtype, int mode, int narrow, const VgArgs& a, hipStream_t s
          : dtype == LVAE_BF16 ? lvae_vg_launch_bf16(mode, narrow, a, st) : lvae_vg_launch_f16(mode, narrow, a, st);
 }
 
-int launch_pack(int dtype, const void* src, const int64_t* off, int64_t stride, const int* n_rows, int64_t rows, int H, int Kp,
-                uint16_t* out, hipStream_t st) {
-    const dim3 grid((unsigned)lvae_ceil_div(rows, 4));
-    const int64_t plane = rows * Kp;
-    if (dtype == LVAE_F32) pack_kernel<LVAE_F32><<<grid, 256, 0, st>>>(src, off, stride, n_rows, rows, H, Kp, out, plane);
-    else pack_kernel<LVAE_BF16><<<grid, 256, 0, st>>>(src, off, stride, n_rows, rows, H, Kp, out, plane);
-    LVAE_LAUNCH_CHECK();
-    return LVAE_OK;
-}
-
 #define RUN(call)                    \
     do {                             \
         const int rc__ = (call);     \
         if (rc__ != LVAE_OK) return rc__; \
     } while (0)
 
-// rows, packed hidden, packed weight and bias; fills the operands of the logits' product
-int launch_operands(const lvae_vocab_problem* q, const Plan& pl, const RowsArgs& rows, char* ws, VgArgs* a, hipStream_t st) {
-    rows_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 1024)), 1024, 0, st>>>(rows);
-    LVAE_LAUNCH_CHECK();
+int launch_both(int dtype, int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st) {
+    return dtype == LVAE_F32 ? lvae_vg_launch_both_f32(mode_w, h, w, h_first, st)
+         : dtype == LVAE_BF16 ? lvae_vg_launch_both_bf16(mode_w, h, w, h_first, st) : lvae_vg_launch_both_f16(mode_w, h, w, h_first, st);
+}
+
+// rows, bias, W and hidden as the products read them; fills the operands of the logits' product
+int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows, char* ws, VgArgs* a, hipStream_t st) {
     uint16_t* hp = (uint16_t*)(ws + pl.hpack);
-    RUN(launch_pack(q->dtype, q->hidden, rows.off, 0, rows.n_rows, pl.Tpad, (int)pl.H, (int)pl.Kp, hp, st));
+    uint16_t* wp = pl.direct_w ? nullptr : (uint16_t*)(ws + pl.wpack);
     float* bias = (float*)(ws + pl.bias);
-    bias_kernel<<<dim3((unsigned)(pl.Vpad / 256)), 256, 0, st>>>(q->bias, q->bias_dtype, pl.V, pl.Vpad, bias);
+    rows.row_blocks = (int)lvae_ceil_div(pl.T, 1024);
+    rows.bias_blocks = (int)lvae_ceil_div(pl.Vpad, 1024);
+    rows.bias = q->bias;
+    rows.bias_out = bias;
+    rows.bias_dtype = q->bias_dtype;
+    rows.Vpad = pl.Vpad;
+    rows.weight = q->weight;
+    rows.wpack = wp;
+    rows.wstride = q->weight_stride;
+    rows.H = q->H;
+    rows.Kp = (int)pl.Kp;
+    const int64_t blocks = rows.row_blocks + rows.bias_blocks + (wp ? lvae_ceil_div(pl.V, 16) : 0);
+    const dim3 grid((unsigned)blocks), pack((unsigned)lvae_ceil_div(pl.Tpad, 4));
+    if (q->dtype == LVAE_F32) {
+        prepare_kernel<LVAE_F32><<<grid, 1024, 0, st>>>(rows);
+        LVAE_LAUNCH_CHECK();
+        pack_kernel<LVAE_F32><<<pack, 256, 0, st>>>(q->hidden, rows.off, rows.n_rows, pl.Tpad, q->H, (int)pl.Kp, hp, pl.Tpad * pl.Kp);
+    } else {                                             // 16 bits are 16 bits
+        prepare_kernel<LVAE_BF16><<<grid, 1024, 0, st>>>(rows);
+        LVAE_LAUNCH_CHECK();
+        pack_kernel<LVAE_BF16><<<pack, 256, 0, st>>>(q->hidden, rows.off, rows.n_rows, pl.Tpad, q->H, (int)pl.Kp, hp, pl.Tpad * pl.Kp);
+    }
     LVAE_LAUNCH_CHECK();
     *a = VgArgs{};
     a->a = (const uint16_t*)q->weight;
     a->lda = q->weight_stride;
     a->a_cols = pl.H;
-    if (!pl.direct_w) {
-        uint16_t* wp = (uint16_t*)(ws + pl.wpack);
-        RUN(launch_pack(q->dtype, q->weight, nullptr, q->weight_stride, nullptr, pl.V, (int)pl.H, (int)pl.Kp, wp, st));
+    if (wp) {
         a->a = wp;
         a->lda = a->a_cols = pl.Kp;
         a->plane_a = pl.V * pl.Kp;
@@ -717,7 +802,7 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     a.ldp = pl.Tpad;
     a.picked = picked;
     RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow, a, st));
-    finish_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 32)), 256, 0, st>>>(part, a.tiles_m, pl.Tpad, picked, rows.tok, rows.tgt_of,
+    finish_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 16)), 256, 0, st>>>(part, a.tiles_m, pl.Tpad, picked, rows.tok, rows.tgt_of,
                                                                           rows.n_rows, ll, lse);
     LVAE_LAUNCH_CHECK();
     return LVAE_OK;
@@ -757,90 +842,100 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     VgArgs a;
     RUN(launch_operands(q, pl, rows, ws, &a, st));
     const float* unscale = rows.g_scale_to > 0.f ? rows.unscale : nullptr;
-    const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2, th = lvae_ceil_div(pl.H, 256);
-    const uint16_t* w0 = a.a;
-    const uint16_t* hp = a.b;
+    const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2;
+    const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow ? 2 : 4;
     uint16_t* gbuf = (uint16_t*)(ws + pl.g);
-    const int64_t plane_g = pl.Tpad * pl.piece;
-    const int waves_n = pl.narrow ? 2 : 4;
+    VgArgs dl = a;                                       // the gradient of the logits
+    dl.lse = rows.lse_of;
+    dl.gy = rows.gy_of;
+    dl.g = gbuf;
+    dl.ldg = pl.piece;
+    dl.plane_g = pl.Tpad * pl.piece;
+    dl.ld_dbias = pl.Vpad;
+    VgArgs h = {};                                       // dHidden
+    h.lda = a.lda;
+    h.plane_a = a.plane_a;
+    h.a_cols = a.a_cols;
+    h.b = gbuf;
+    h.ldb = pl.piece;
+    h.plane_b = dl.plane_g;
+    h.M = pl.H;
+    h.N = pl.T;
+    h.n_rows = rows.n_rows;
+    h.tiles_m = th;
+    h.tiles_n = a.tiles_n;
+    h.splits = pl.splits_h;
+    h.slab = (float*)(ws + pl.slab);
+    h.ld_slab = pl.Kp;
+    h.slab_stride = pl.Tpad * pl.Kp;
+    VgArgs w = {};                                       // dWeight
+    w.a = a.b;
+    w.lda = pl.Kp;
+    w.plane_a = a.plane_b;
+    w.a_cols = pl.Kp;
+    w.b = gbuf;
+    w.ldb = pl.piece;
+    w.plane_b = dl.plane_g;
+    w.M = pl.H;
+    w.n_rows = rows.n_rows;
+    w.tiles_m = th;
+    w.splits = pl.splits_w;
+    w.slab = (float*)(ws + pl.slab_w);
+    w.ld_slab = pl.Kp;
+    w.slab_stride = pl.piece * pl.Kp;
+    w.ld_out = pl.H;
+    w.unscale = unscale;
+    const int mode_w = pl.splits_w > 1 ? VG_DWEIGHT_SLAB : VG_DWEIGHT;
     for (int64_t v0 = 0; v0 < pl.V; v0 += pl.piece) {
         const int64_t words = pl.V - v0 < pl.piece ? pl.V - v0 : pl.piece;
-        VgArgs l = a;                                    // G of this piece
-        l.a = w0 + v0 * a.lda;
-        l.M = words;
-        l.tiles_m = (int)lvae_ceil_div(words, 256);
-        l.bias = a.bias + v0;
-        l.v0 = v0;
-        l.lse = rows.lse_of;
-        l.gy = rows.gy_of;
-        l.g = gbuf;
-        l.ldg = pl.piece;
-        l.plane_g = plane_g;
-        l.dbias = d_bias ? (float*)(ws + pl.dbias) : nullptr;
-        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, l, st));
-        if (d_bias) {
-            dbias_kernel<<<dim3((unsigned)lvae_ceil_div(words, 32)), 256, 0, st>>>(l.dbias, pl.piece, waves_n, pl.tile_n, rows.n_rows,
-                                                                                   words, unscale, d_bias, q->bias_dtype, v0);
+        dl.a = a.a + v0 * a.lda;
+        dl.M = words;
+        dl.tiles_m = (int)lvae_ceil_div(words, 256);
+        dl.bias = a.bias + v0;
+        dl.v0 = v0;
+        dl.dbias = d_bias ? (float*)(ws + pl.dbias) + v0 : nullptr;
+        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, dl, st));
+        h.a = dl.a;
+        h.K = words;
+        h.slab_add = v0 > 0;
+        w.N = words;
+        w.tiles_n = dl.tiles_m;
+        w.out = (char*)d_weight + v0 * pl.H * esz;
+        if (d_hidden && d_weight && !pl.narrow) {
+            const int64_t ks_h = lvae_ceil_div(words, VG_BK) / pl.splits_h, ks_w = lvae_ceil_div(pl.T, VG_BK) / pl.splits_w;
+            RUN(launch_both(q->dtype, mode_w, h, w, ks_h >= ks_w, st));
+        } else {
+            if (d_hidden) RUN(launch_tiles(q->dtype, VG_DHIDDEN, pl.narrow, h, st));
+            if (d_weight) RUN(launch_tiles(q->dtype, mode_w, 0, w, st));
+        }
+        if (d_weight && pl.splits_w > 1) {
+            dweight_kernel<<<dim3((unsigned)lvae_ceil_div(words * pl.H, 256)), 256, 0, st>>>(
+                w.slab, pl.splits_w, w.slab_stride, w.ld_slab, words, (int)pl.H, unscale, w.out, q->dtype);
             LVAE_LAUNCH_CHECK();
         }
-        if (d_hidden) {
-            VgArgs h = {};
-            h.a = w0 + v0 * a.lda;
-            h.lda = a.lda;
-            h.plane_a = a.plane_a;
-            h.a_cols = a.a_cols;
-            h.b = gbuf;
-            h.ldb = pl.piece;
-            h.plane_b = plane_g;
-            h.M = pl.H;
-            h.N = pl.T;
-            h.K = words;
-            h.n_rows = rows.n_rows;
-            h.tiles_m = (int)th;
-            h.tiles_n = a.tiles_n;
-            h.splits = pl.splits_h;
-            h.slab = (float*)(ws + pl.slab);
-            h.ld_slab = pl.Kp;
-            h.slab_stride = pl.Tpad * pl.Kp;
-            h.slab_add = v0 > 0;
-            RUN(launch_tiles(q->dtype, VG_DHIDDEN, pl.narrow, h, st));
-        }
-        if (d_weight) {
-            VgArgs w = {};
-            w.a = hp;
-            w.lda = pl.Kp;
-            w.plane_a = a.plane_b;
-            w.a_cols = pl.Kp;
-            w.b = gbuf;
-            w.ldb = pl.piece;
-            w.plane_b = plane_g;
-            w.M = pl.H;
-            w.N = words;
-            w.n_rows = rows.n_rows;
-            w.tiles_m = (int)th;
-            w.tiles_n = (int)lvae_ceil_div(words, 256);
-            w.splits = pl.splits_w;
-            char* out = (char*)d_weight + v0 * pl.H * esz;
-            if (pl.splits_w > 1) {
-                w.slab = (float*)(ws + pl.slab_w);
-                w.ld_slab = pl.Kp;
-                w.slab_stride = pl.piece * pl.Kp;
-                RUN(launch_tiles(q->dtype, VG_DWEIGHT_SLAB, 0, w, st));
-                dweight_kernel<<<dim3((unsigned)lvae_ceil_div(words * pl.H, 256)), 256, 0, st>>>(
-                    w.slab, pl.splits_w, w.slab_stride, w.ld_slab, words, (int)pl.H, unscale, out, q->dtype);
-                LVAE_LAUNCH_CHECK();
-            } else {
-                w.out = out;
-                w.ld_out = pl.H;
-                w.unscale = unscale;
-                RUN(launch_tiles(q->dtype, VG_DWEIGHT, 0, w, st));
-            }
-        }
     }
-    if (d_hidden) {
-        const int64_t n = pl.T * ((pl.H + 3) / 4);
-        dhidden_kernel<<<dim3((unsigned)lvae_ceil_div(n, 256)), 256, 0, st>>>((float*)(ws + pl.slab), pl.splits_h, pl.Tpad * pl.Kp, pl.Kp,
-                                                                             rows.inv, pl.T, (int)pl.H, unscale, d_hidden, q->dtype);
+    if (d_hidden || d_bias) {
+        FinalArgs f = {};
+        f.slab = h.slab;
+        f.slab_stride = h.slab_stride;
+        f.ld = h.ld_slab;
+        f.T = pl.T;
+        f.inv = rows.inv;
+        f.splits = pl.splits_h;
+        f.H = q->H;
+        f.dt = q->dtype;
+        f.hidden_blocks = d_hidden ? (int)lvae_ceil_div(pl.T * ((pl.H + 3) / 4), 256) : 0;
+        f.d_hidden = d_hidden;
+        f.part = (float*)(ws + pl.dbias);
+        f.ld_part = pl.Vpad;
+        f.V = pl.V;
+        f.per_tile = waves_n;
+        f.tile_rows = pl.tile_n;
+        f.bias_dt = q->bias_dtype;
+        f.d_bias = d_bias;
+        f.n_rows = rows.n_rows;
+        f.unscale = unscale;
+        final_kernel<<<dim3((unsigned)(f.hidden_blocks + (d_bias ? lvae_ceil_div(pl.V, 32) : 0))), 256, 0, st>>>(f);
         LVAE_LAUNCH_CHECK();
     }
     return LVAE_OK;

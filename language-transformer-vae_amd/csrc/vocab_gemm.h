@@ -29,6 +29,10 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+// in memory, aligned to their elements alone (the compiler emits unaligned 16-byte accesses)
+typedef f32x4 __attribute__((aligned(4))) f32x4_u;
+typedef s16x4 __attribute__((aligned(2))) s16x4_u;
+typedef s16x8 __attribute__((aligned(2))) s16x8_u;
 
 #define VG_BK 64               // a slice of the summed index: rows of 128 bytes, whole cache lines (64-byte rows load at half the rate)
 
@@ -55,7 +59,8 @@ struct VgArgs {
     float* picked;              // logit of the target
     uint16_t* g;                // [planes][rows][ldg] gradient of the logits
     int64_t ldg, plane_g;
-    float* dbias;               // [tiles_n * waves along n][ldg] partial column sums, or NULL
+    float* dbias;               // [tiles_n * waves along n][ld_dbias] partial column sums, or NULL
+    int64_t ld_dbias;
     float* slab;                // [splits][slab_rows][ld_slab] float32 partial products
     int64_t ld_slab, slab_stride;
     int slab_add;               // add to what the slab holds
@@ -147,13 +152,14 @@ __device__ __forceinline__ float vg_row_sum(float v) {
 
 // TRA / TRB: the operand is stored [k][m] / [k][n].  WM x WN waves, each 128 x (16 NJ); NA slices of a and
 // two of b in LDS at a time.
+template <int WM, int WN, int NJ, int NA> constexpr int vg_lds_bytes() { return (NA * 128 * WM + 2 * 16 * NJ * WN) * VG_BK * 2; }
+
 template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
-__global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
+__device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* lds) {
     constexpr int W = WM * WN, MI = 8, TM = 128 * WM, TN = 16 * NJ * WN, BK = VG_BK;
     constexpr int A_BYTES = TM * BK * 2, B_BYTES = TN * BK * 2;
     constexpr int QA = A_BYTES / 1024 / W, QB = B_BYTES / 1024 / W;
     static_assert(QA * W * 1024 == A_BYTES && QB * W * 1024 == B_BYTES, "whole loads");
-    __shared__ __align__(1024) char lds[NA * A_BYTES + 2 * B_BYTES];
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -165,7 +171,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
     int tm, tn, split;
     {
         const int per = p.tiles_m * p.tiles_n, total = per * p.splits;
-        const int each = total / 8, rest = total % 8, x = blockIdx.x & 7, l = blockIdx.x >> 3;
+        const int each = total / 8, rest = total % 8, x = block & 7, l = block >> 3;
         int id = x * each + min(x, rest) + l;
         if (l >= each + (x < rest ? 1 : 0)) return;
         split = id / per;
@@ -484,7 +490,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
             }
         }
         if (p.dbias) {
-            float* d = p.dbias + ((int64_t)tn * WN + wn) * p.ldg + mb;
+            float* d = p.dbias + ((int64_t)tn * WN + wn) * p.ld_dbias + mb;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
                 f32x4 v;
@@ -509,7 +515,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
         }
     } else {
         const float f = p.unscale ? p.unscale[0] : 1.f;
-        const bool whole = mb + 32 <= p.M && (p.ld_out & 7) == 0;
+        const bool whole = mb + 32 <= p.M;              // rows of any alignment: the stores need that of an element alone
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int64_t n = n0 + nb + j * 16;
@@ -518,7 +524,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
                 float* row = (float*)p.out + n * p.ld_out + mb;
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    if (whole) *(f32x4*)(row + 4 * i) = acc[i][j];
+                    if (whole) *(f32x4_u*)(row + 4 * i) = acc[i][j];
                     else
                         for (int r = 0; r < 4; ++r)
                             if (mb + 4 * i + r < p.M) row[4 * i + r] = acc[i][j][r];
@@ -530,7 +536,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
                     s16x8 o;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) o[e] = vg_round<DT>(acc[i + (e >> 2)][j][e & 3] * f);
-                    if (whole) *(s16x8*)(row + 4 * i) = o;
+                    if (whole) *(s16x8_u*)(row + 4 * i) = o;
                     else
                         for (int e = 0; e < 8; ++e)
                             if (mb + 4 * i + e < p.M) row[4 * i + e] = o[e];
@@ -538,4 +544,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
             }
         }
     }
+}
+
+template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
+__global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
+    __shared__ __align__(1024) char lds[vg_lds_bytes<WM, WN, NJ, NA>()];
+    vg_tile<DT, TRA, TRB, EPI, WM, WN, NJ, NA>(p, blockIdx.x, lds);
+}
+
+// Both products of a piece's G in one launch, so that the tiles of one fill the CUs that the last round of the other
+// leaves idle; the longer tiles come first.
+template <int DT, int EPI_W, int WM, int WN, int NJ, int NA>
+__global__ __launch_bounds__(64 * WM * WN, 2) void vg_both_kernel(VgArgs h, VgArgs w, unsigned blocks_h, unsigned blocks_w, int h_first) {
+    __shared__ __align__(1024) char lds[vg_lds_bytes<WM, WN, NJ, NA>()];
+    const unsigned b = blockIdx.x;
+    if (h_first ? b < blocks_h : b >= blocks_w)
+        vg_tile<DT, true, false, VG_SLAB, WM, WN, NJ, NA>(h, h_first ? b : b - blocks_w, lds);
+    else
+        vg_tile<DT, true, true, EPI_W, WM, WN, NJ, NA>(w, h_first ? b - blocks_h : b, lds);
 }

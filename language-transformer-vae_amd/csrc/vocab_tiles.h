@@ -1,4 +1,4 @@
-// Launchers of the tile products of one element type; each vocab_tiles_*.hip defines VG_DT and VG_NAME and includes this.
+// Launchers of the tile products of one element type; each vocab_tiles_*.hip defines VG_DT, VG_NAME and VG_NAME_BOTH and includes this.
 #include "vocab_gemm.h"
 
 
@@ -20,6 +20,18 @@ template <int DT, int WM, int WN, int NJ, int NA> static int vg_mode(int mode, c
     }
 }
 
+#define VG_WIDE 2, 4, 4, 3
+#define VG_NARROW 2, 2, 2, 2
+
 int VG_NAME(int mode, int narrow, const VgArgs& p, hipStream_t st) {
-    return narrow ? vg_mode<VG_DT, 2, 2, 2, 2>(mode, p, st) : vg_mode<VG_DT, 2, 4, 4, 3>(mode, p, st);
+    return narrow ? vg_mode<VG_DT, VG_NARROW>(mode, p, st) : vg_mode<VG_DT, VG_WIDE>(mode, p, st);
+}
+
+int VG_NAME_BOTH(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st) {
+    const int64_t bh = lvae_round_up((int64_t)h.tiles_m * h.tiles_n * h.splits, 8), bw = lvae_round_up((int64_t)w.tiles_m * w.tiles_n * w.splits, 8);
+    const dim3 grid((unsigned)(bh + bw));
+    if (mode_w == VG_DWEIGHT_SLAB) vg_both_kernel<VG_DT, VG_SLAB, VG_WIDE><<<grid, 512, 0, st>>>(h, w, (unsigned)bh, (unsigned)bw, h_first);
+    else vg_both_kernel<VG_DT, VG_OUT, VG_WIDE><<<grid, 512, 0, st>>>(h, w, (unsigned)bh, (unsigned)bw, h_first);
+    LVAE_LAUNCH_CHECK();
+    return LVAE_OK;
 }
