@@ -459,10 +459,10 @@ int lvae_vocab_ll_bwd(const lvae_vocab_problem* problem, const float* lse, const
                       const float* g_scale, void* d_hidden, void* d_weight, void* d_bias, void* ws, int64_t ws_bytes,
                       void* stream);
 
-/* loss[0] = factor * sum(ll); with mean != 0, over max(1, tokens whose target is not ignore_index).  loss[1] is the
- * factor of each ll in it (the g_scale of the backward).  One workgroup, float64. */
+/* loss = factor * sum(ll); with mean != 0, over max(1, tokens whose target is not ignore_index).  each: the factor of
+ * each ll in it (the g_scale of the backward).  Both float32 on the device; one workgroup, float64. */
 int lvae_vocab_loss_f32(const lvae_vocab_problem* problem, const float* ll, int mean, float factor, float* loss,
-                        void* stream);
+                        float* each, void* stream);
 
 /* out[i] = sum_k x[i * len + k], float64 inside; len may be 0. */
 int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream);

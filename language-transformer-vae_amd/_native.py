@@ -3,6 +3,7 @@
 There is no fallback: if the shared library is missing or a call fails, this raises.  PyTorch is used
 only to own device memory and to name the current HIP stream.
 """
+import contextlib
 import ctypes
 import os
 
@@ -126,7 +127,7 @@ _SIGNATURES = {
     "lvae_vocab_ll_bwd": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.POINTER(_i64), _c_f32p,
                                  ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _i64,
                                  ctypes.c_void_p]),
-    "lvae_vocab_loss_f32": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _int, _f32, _c_f32p, ctypes.c_void_p]),
+    "lvae_vocab_loss_f32": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _int, _f32, _c_f32p, _c_f32p, ctypes.c_void_p]),
     "lvae_segment_sum_f32": (_int, [_c_f32p, _i64, _i64, _c_f32p, ctypes.c_void_p]),
     "lvae_clip_workspace_bytes": (_int, [_i64, ctypes.POINTER(_i64)]),
     "lvae_clip_grads": (_int, [ctypes.c_void_p, _i64, _int, _int, ctypes.c_double, _c_f32p, ctypes.c_void_p, _i64,
@@ -176,6 +177,22 @@ def ptr(t):
 
 def stream_ptr(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+# The two below are what stream_ptr() and torch.cuda.device() do, without the objects that these make: a call of a few
+# microseconds on the GPU is otherwise bound by them.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_NO_GUARD = contextlib.nullcontext()
+
+
+def raw_stream(index):
+    """Handle of the current stream of GPU ``index``, as an int."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def on_device(index):
+    """Context in which GPU ``index`` is the current one."""
+    return _NO_GUARD if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def as_f32(t, name):

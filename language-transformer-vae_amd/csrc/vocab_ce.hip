@@ -491,7 +491,8 @@ __global__ __launch_bounds__(256) void segment_sum_kernel(const float* x, int64_
 }
 
 __global__ __launch_bounds__(1024) void loss_kernel(const int64_t* targets, Axes tgt, int64_t T, int64_t ignore,
-                                                    const float* ll, int mean, float factor, float* out) {
+                                                    const float* ll, int mean, float factor, float* loss,
+                                                    float* each) {
     __shared__ double red[16];
     __shared__ int redi[16];
     double a = 0.0;
@@ -508,8 +509,8 @@ __global__ __launch_bounds__(1024) void loss_kernel(const int64_t* targets, Axes
         double s = 0.0;
         for (int w = 0; w < 16; ++w) s += red[w];
         const double f = (double)factor / (mean ? (double)max(1, c) : 1.0);
-        out[0] = (float)(s * f);
-        out[1] = (float)f;
+        loss[0] = (float)(s * f);
+        each[0] = (float)f;
     }
 }
 
@@ -523,7 +524,7 @@ struct Plan {
     int splits_h, splits_w;
     // offsets into the workspace, bytes
     int64_t off, tok, tgt, inv, lse, gy, head, bias, hpack, wpack, part, picked, g, slab, slab_w, dbias, bytes;
-    int64_t few_blocks;
+    int64_t few_blocks, ld_dbias;
 };
 
 int check_problem(const lvae_vocab_problem* q, Plan* pl) {
@@ -624,7 +625,10 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     }
     pl->slab = want_h ? take(at, pl->splits_h * pl->Tpad * pl->Kp * 4) : 0;
     pl->slab_w = want_w && pl->splits_w > 1 ? take(at, pl->splits_w * pl->piece * pl->Kp * 4) : 0;
-    pl->dbias = want_b ? take(at, pl->Tpad / pl->tile_n * (pl->narrow ? 2 : 4) * pl->Vpad * 4) : 0;
+    // column sums of all pieces for one reduction at the end, or of one piece where that would take over 256 MiB
+    const int64_t parts = pl->Tpad / pl->tile_n * (pl->narrow ? 2 : 4);
+    pl->ld_dbias = parts * pl->Vpad * 4 <= 256ll << 20 ? pl->Vpad : pl->piece;
+    pl->dbias = want_b ? take(at, parts * pl->ld_dbias * 4) : 0;
     pl->bytes = at;
 }
 
@@ -851,7 +855,8 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     dl.g = gbuf;
     dl.ldg = pl.piece;
     dl.plane_g = pl.Tpad * pl.piece;
-    dl.ld_dbias = pl.Vpad;
+    dl.ld_dbias = pl.ld_dbias;
+    const bool bias_whole = pl.ld_dbias >= pl.Vpad;
     VgArgs h = {};                                       // dHidden
     h.lda = a.lda;
     h.plane_a = a.plane_a;
@@ -886,6 +891,16 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     w.ld_out = pl.H;
     w.unscale = unscale;
     const int mode_w = pl.splits_w > 1 ? VG_DWEIGHT_SLAB : VG_DWEIGHT;
+    FinalArgs f = {};
+    f.part = (float*)(ws + pl.dbias);
+    f.ld_part = pl.ld_dbias;
+    f.V = d_bias ? pl.V : 0;
+    f.per_tile = waves_n;
+    f.tile_rows = pl.tile_n;
+    f.bias_dt = q->bias_dtype;
+    f.d_bias = d_bias;
+    f.n_rows = rows.n_rows;
+    f.unscale = unscale;
     for (int64_t v0 = 0; v0 < pl.V; v0 += pl.piece) {
         const int64_t words = pl.V - v0 < pl.piece ? pl.V - v0 : pl.piece;
         dl.a = a.a + v0 * a.lda;
@@ -893,8 +908,15 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         dl.tiles_m = (int)lvae_ceil_div(words, 256);
         dl.bias = a.bias + v0;
         dl.v0 = v0;
-        dl.dbias = d_bias ? (float*)(ws + pl.dbias) + v0 : nullptr;
+        dl.dbias = d_bias ? (float*)(ws + pl.dbias) + (bias_whole ? v0 : 0) : nullptr;
         RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, dl, st));
+        if (d_bias && !bias_whole) {
+            FinalArgs b = f;
+            b.V = words;
+            b.d_bias = (char*)d_bias + v0 * (q->bias_dtype == LVAE_F32 ? 4 : 2);
+            final_kernel<<<dim3((unsigned)lvae_ceil_div(words, 32)), 256, 0, st>>>(b);
+            LVAE_LAUNCH_CHECK();
+        }
         h.a = dl.a;
         h.K = words;
         h.slab_add = v0 > 0;
@@ -914,38 +936,31 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
             LVAE_LAUNCH_CHECK();
         }
     }
-    if (d_hidden || d_bias) {
-        FinalArgs f = {};
-        f.slab = h.slab;
-        f.slab_stride = h.slab_stride;
-        f.ld = h.ld_slab;
-        f.T = pl.T;
-        f.inv = rows.inv;
-        f.splits = pl.splits_h;
-        f.H = q->H;
-        f.dt = q->dtype;
-        f.hidden_blocks = d_hidden ? (int)lvae_ceil_div(pl.T * ((pl.H + 3) / 4), 256) : 0;
-        f.d_hidden = d_hidden;
-        f.part = (float*)(ws + pl.dbias);
-        f.ld_part = pl.Vpad;
-        f.V = pl.V;
-        f.per_tile = waves_n;
-        f.tile_rows = pl.tile_n;
-        f.bias_dt = q->bias_dtype;
-        f.d_bias = d_bias;
-        f.n_rows = rows.n_rows;
-        f.unscale = unscale;
-        final_kernel<<<dim3((unsigned)(f.hidden_blocks + (d_bias ? lvae_ceil_div(pl.V, 32) : 0))), 256, 0, st>>>(f);
+    f.slab = h.slab;
+    f.slab_stride = h.slab_stride;
+    f.ld = h.ld_slab;
+    f.T = pl.T;
+    f.inv = rows.inv;
+    f.splits = pl.splits_h;
+    f.H = q->H;
+    f.dt = q->dtype;
+    f.hidden_blocks = d_hidden ? (int)lvae_ceil_div(pl.T * ((pl.H + 3) / 4), 256) : 0;
+    f.d_hidden = d_hidden;
+    if (!bias_whole) f.V = 0;
+    const int64_t blocks = f.hidden_blocks + lvae_ceil_div(f.V, 32);
+    if (blocks) {
+        final_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(f);
         LVAE_LAUNCH_CHECK();
     }
     return LVAE_OK;
 }
 
-extern "C" int lvae_vocab_loss_f32(const lvae_vocab_problem* q, const float* ll, int mean, float factor, float* loss, void* stream) {
+extern "C" int lvae_vocab_loss_f32(const lvae_vocab_problem* q, const float* ll, int mean, float factor, float* loss, float* each,
+                                   void* stream) {
     Plan pl = {};
     RUN(check_problem(q, &pl));
-    LVAE_CHECK_ARG(ll && loss && q->targets, "ll, loss and targets must be non-NULL");
-    loss_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(q->targets, axes_of(q, q->target_stride), pl.T, q->ignore_index, ll, mean, factor, loss);
+    LVAE_CHECK_ARG(ll && loss && each && q->targets, "ll, loss, each and targets must be non-NULL");
+    loss_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(q->targets, axes_of(q, q->target_stride), pl.T, q->ignore_index, ll, mean, factor, loss, each);
     LVAE_LAUNCH_CHECK();
     return LVAE_OK;
 }

@@ -41,51 +41,79 @@ class _Problem:
     """Checked arguments of one call: the C structure and what keeps its pointers alive."""
 
     def __init__(self, hidden, weight, targets, bias, ignore_index):
-        for t, name in ((hidden, "hidden"), (weight, "weight"), (targets, "targets")) + (((bias, "bias"),) if bias is not None else ()):
+        named = [(hidden, "hidden"), (weight, "weight"), (targets, "targets")]
+        if bias is not None:
+            named.append((bias, "bias"))
+        for t, name in named:
             if not isinstance(t, torch.Tensor):
                 raise TypeError(f"{name} must be a torch.Tensor")
             if not t.is_cuda:
                 raise N.LvaeError(f"{name} is on {t.device}: the HIP path needs a GPU tensor (no CPU fallback)")
-            if t.device != hidden.device:
-                raise ValueError(f"{name} is on {t.device}, hidden on {hidden.device}")
-        if hidden.dtype not in N.DTYPES or weight.dtype != hidden.dtype:
+        index = hidden.get_device()
+        if weight.get_device() != index or targets.get_device() != index or (bias is not None and bias.get_device() != index):
+            raise ValueError(f"hidden, weight, targets and bias must be on one device: {[str(t.device) for t, _ in named]}")
+        dtype = N.DTYPES.get(hidden.dtype)
+        if dtype is None or weight.dtype != hidden.dtype:
             raise TypeError(f"hidden and weight must be of one type, float32, bfloat16 or float16: {hidden.dtype}, {weight.dtype}")
         if bias is not None and bias.dtype not in N.DTYPES:
             raise TypeError(f"bias must be float32, bfloat16 or float16: {bias.dtype}")
         if targets.dtype != torch.int64:
             raise TypeError(f"targets must be int64: {targets.dtype}")
-        if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
-            raise ValueError(f"shape mismatch: hidden {tuple(hidden.shape)}, weight {tuple(weight.shape)}")
+        shape = hidden.shape
+        if not shape or weight.dim() != 2 or weight.shape[1] != shape[-1]:
+            raise ValueError(f"shape mismatch: hidden {tuple(shape)}, weight {tuple(weight.shape)}")
         V, H = weight.shape
         if V < 1 or H < 1:
             raise ValueError(f"weight {tuple(weight.shape)} is empty")
         if bias is not None and bias.shape != (V,):
             raise ValueError(f"bias {tuple(bias.shape)} must be ({V},)")
-        self.shape = hidden.shape[:-1]
-        if targets.shape != self.shape:
+        self.shape = shape = shape[:-1]
+        if targets.shape != shape:
             try:
-                targets = targets.expand(self.shape)
+                targets = targets.expand(shape)
             except RuntimeError:
-                raise ValueError(f"targets {tuple(targets.shape)} do not expand to {tuple(self.shape)}") from None
-        if hidden.stride(-1) != 1 and H > 1:
+                raise ValueError(f"targets {tuple(targets.shape)} do not expand to {tuple(shape)}") from None
+        hs, (w0, w1) = hidden.stride(), weight.stride()
+        if hs[-1] != 1 and H > 1:
             hidden = hidden.contiguous()
-        if (weight.stride(1) != 1 and H > 1) or (weight.stride(0) < H and V > 1):
+            hs = hidden.stride()
+        if (w1 != 1 and H > 1) or (w0 < H and V > 1):
             weight = weight.contiguous()
+            w0 = H
         if bias is not None and not bias.is_contiguous():
             bias = bias.contiguous()
-        axes = _common_axes(self.shape, [hidden.stride()[:-1], targets.stride()])
+        axes = _common_axes(shape, (hs[:-1], targets.stride()))
         if axes is None:
             hidden, targets = hidden.contiguous(), targets.contiguous()
-            axes = _common_axes(self.shape, [hidden.stride()[:-1], targets.stride()])
+            axes = _common_axes(shape, (hidden.stride()[:-1], targets.stride()))
         self.tensors = (hidden, weight, targets, bias)
-        self.device = hidden.device
+        self.pointers = _pointers(self.tensors)
+        self.device, self.index = hidden.device, index
         self.T = targets.numel()
+        self.ignore_index = ignore_index
         size, (hs, ts) = axes
-        three = N._i64 * 3
-        self.c = N.VocabProblem(hidden.data_ptr(), weight.data_ptr(), None if bias is None else bias.data_ptr(),
-                                targets.data_ptr(), three(*size), three(*hs), three(*ts), V,
-                                weight.stride(0) if V > 1 else H, int(ignore_index), H, N.DTYPES[hidden.dtype],
-                                0 if bias is None else N.DTYPES[bias.dtype], 0)
+        h, w, y, b = self.pointers
+        self.c = N.VocabProblem(h, w, b, y, _Three(*size), _Three(*hs), _Three(*ts), V, w0 if V > 1 else H,
+                                int(ignore_index), H, dtype, 0 if bias is None else N.DTYPES[bias.dtype], 0)
+
+    def without_tensors(self):
+        """(tensors, plan that does not hold them): for the backward, whose tensors autograd keeps."""
+        tensors, self.tensors = self.tensors, None
+        return tensors, self
+
+    def at(self, tensors):
+        """The plan for tensors that autograd has kept: itself, unless a hook of the saved tensors has moved them."""
+        if _pointers(tensors) == self.pointers:
+            return self
+        h, w, y, b = tensors
+        return _Problem(h, w, y, b, self.ignore_index)
+
+
+_Three = N._i64 * 3
+
+
+def _pointers(tensors):
+    return [None if t is None else t.data_ptr() for t in tensors]
 
 
 def _forward(q, want_lse):
@@ -95,38 +123,39 @@ def _forward(q, want_lse):
     lse = torch.empty(q.shape, dtype=torch.float32, device=dev) if want_lse else None
     if q.T:
         nbytes = N._i64(0)
-        with torch.cuda.device(dev):
+        with N.on_device(q.index):
             lib = N.lib()
             N.check(lib.lvae_vocab_ll_workspace_bytes(q.c, nbytes))
             ws = N.workspace(nbytes.value, dev)
-            N.check(lib.lvae_vocab_ll(q.c, N.ptr(ll), N.ptr(lse), N.ptr(ws), nbytes.value, N.stream_ptr(dev)))
+            N.check(lib.lvae_vocab_ll(q.c, ll.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(),
+                                      nbytes.value, N.raw_stream(q.index)))
     return ll, lse
 
 
-def _backward(q, needs, lse, g, g_axes_strides, g_scale):
+def _backward(q, tensors, needs, lse, g, g_strides, g_scale):
     """Gradients of hidden, weight, bias (None where not needed); g is read with the strides given, one per token axis
     of the problem."""
-    hidden, weight, _, bias = q.tensors
+    hidden, weight, _, bias = tensors
     dev = q.device
+    new = torch.empty if q.T else torch.zeros
     d_h = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if needs[0] else None
-    if not q.T:
-        return (d_h, torch.zeros(weight.shape, dtype=weight.dtype, device=dev) if needs[1] else None,
-                torch.zeros(bias.shape, dtype=bias.dtype, device=dev) if needs[2] else None)
-    d_w = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if needs[1] else None
-    d_b = torch.empty(bias.shape, dtype=bias.dtype, device=dev) if needs[2] else None
-    nbytes = N._i64(0)
-    with torch.cuda.device(dev):
-        lib = N.lib()
-        N.check(lib.lvae_vocab_ll_bwd_workspace_bytes(q.c, int(needs[0]), int(needs[1]), int(needs[2]), nbytes))
-        ws = N.workspace(nbytes.value, dev)
-        N.check(lib.lvae_vocab_ll_bwd(q.c, N.ptr(lse), N.ptr(g), (N._i64 * 3)(*g_axes_strides), N.ptr(g_scale),
-                                      N.ptr(d_h), N.ptr(d_w), N.ptr(d_b), N.ptr(ws), nbytes.value, N.stream_ptr(dev)))
+    d_w = new(weight.shape, dtype=weight.dtype, device=dev) if needs[1] else None
+    d_b = new(bias.shape, dtype=bias.dtype, device=dev) if needs[2] else None
+    if q.T:
+        nbytes = N._i64(0)
+        with N.on_device(q.index):
+            lib = N.lib()
+            N.check(lib.lvae_vocab_ll_bwd_workspace_bytes(q.c, needs[0], needs[1], needs[2], nbytes))
+            ws = N.workspace(nbytes.value, dev)
+            p = _pointers((lse, g, g_scale, d_h, d_w, d_b))
+            N.check(lib.lvae_vocab_ll_bwd(q.c, p[0], p[1], _Three(*g_strides), p[2], p[3], p[4], p[5], ws.data_ptr(),
+                                          nbytes.value, N.raw_stream(q.index)))
     return d_h, d_w, d_b
 
 
 def _token_strides(q):
     """Strides of a contiguous [tokens] tensor on the problem's three axes."""
-    a, b, c = q.c.size
+    _, b, c = q.c.size
     return (b * c, c, 1)
 
 
@@ -142,16 +171,17 @@ def _put_together(q, ll, how):
     if how == _SEQUENCES:
         out = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
         if out.numel():
-            with torch.cuda.device(dev):
-                N.check(N.lib().lvae_segment_sum_f32(N.ptr(ll), out.numel(), q.shape[-1], N.ptr(out), N.stream_ptr(dev)))
+            with N.on_device(q.index):
+                N.check(N.lib().lvae_segment_sum_f32(ll.data_ptr(), out.numel(), q.shape[-1], out.data_ptr(),
+                                                     N.raw_stream(q.index)))
         return out, None
     if not q.T:
-        out = torch.zeros(2, dtype=torch.float32, device=dev)
-    else:
-        out = torch.empty(2, dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            N.check(N.lib().lvae_vocab_loss_f32(q.c, N.ptr(ll), int(how == _MEAN), -1.0, N.ptr(out), N.stream_ptr(dev)))
-    return out[0], out[1]
+        return torch.zeros((), device=dev), torch.zeros((), device=dev)
+    loss, each = torch.empty((), device=dev, dtype=torch.float32), torch.empty((), device=dev, dtype=torch.float32)
+    with N.on_device(q.index):
+        N.check(N.lib().lvae_vocab_loss_f32(q.c, ll.data_ptr(), how == _MEAN, -1.0, loss.data_ptr(), each.data_ptr(),
+                                            N.raw_stream(q.index)))
+    return loss, each
 
 
 class _VocabLL(torch.autograd.Function):
@@ -163,35 +193,34 @@ class _VocabLL(torch.autograd.Function):
         q = _Problem(hidden.detach(), weight.detach(), targets, None if bias is None else bias.detach(), ignore_index)
         ll, lse = _forward(q, True)
         out, factor = _put_together(q, ll, how)
-        ctx.save_for_backward(hidden, weight, bias, targets, lse, factor)
-        ctx.ignore_index, ctx.how = ignore_index, how
+        tensors, ctx.plan = q.without_tensors()
+        ctx.save_for_backward(*tensors, lse, factor)
+        ctx.how = how
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        hidden, weight, bias, targets, lse, factor = ctx.saved_tensors
+        *tensors, lse, factor = ctx.saved_tensors
         needs = ctx.needs_input_grad[:3]
         if not any(needs):
             return None, None, None, None, None, None
-        q = _Problem(hidden.detach(), weight.detach(), targets, None if bias is None else bias.detach(), ctx.ignore_index)
+        q = ctx.plan.at(tensors)
         if g.dtype != torch.float32:
             g = g.float()
-        if ctx.how in (_MEAN, _SUM):
+        if ctx.how >= _MEAN:
             strides = (0, 0, 0)
         else:
             # sequences: one value for all positions of a sentence; the problem's axes join dimensions, so spread it out
             g = (g if ctx.how == _TOKENS else g.unsqueeze(-1).expand(q.shape)).contiguous()
             strides = _token_strides(q)
-        d_h, d_w, d_b = _backward(q, needs, lse, g, strides, factor)
-        return d_h, d_w, d_b, None, None, None
+        return (*_backward(q, tensors, needs, lse, g, strides, factor), None, None, None)
 
 
 def _run(hidden, weight, targets, bias, ignore_index, how):
     if _needs_grad(hidden, weight, bias):
         return _VocabLL.apply(hidden, weight, bias, targets, ignore_index, how)
-    det = lambda t: t.detach() if isinstance(t, torch.Tensor) else t
-    q = _Problem(det(hidden), det(weight), targets, det(bias), ignore_index)
+    q = _Problem(hidden, weight, targets, bias, ignore_index)
     return _put_together(q, _forward(q, False)[0], how)[0]
 
 

@@ -41,14 +41,14 @@ def _call(src, dst, norm_type, scale, max_norm):
         table = _table(src2, None if dst is None else copies)[0]
     count = len(src)
     nbytes = N._i64(0)
-    dev = torch.device("cuda", index)
-    with torch.cuda.device(index):
+    dev = src[0].device
+    with N.on_device(index):
         lib = N.lib()
         N.check(lib.lvae_clip_workspace_bytes(count, nbytes))
         ws = N.workspace(nbytes.value, dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        N.check(lib.lvae_clip_grads(table, count, int(norm_type == float("inf")), int(scale), float(max_norm), N.ptr(norm),
-                                    N.ptr(ws), nbytes.value, N.stream_ptr(dev)))
+        N.check(lib.lvae_clip_grads(table, count, int(norm_type == float("inf")), int(scale), float(max_norm), norm.data_ptr(),
+                                    ws.data_ptr(), nbytes.value, N.raw_stream(index)))
     if scale:
         for i in odd:
             (src if dst is None else dst)[i].detach().copy_(copies[i])

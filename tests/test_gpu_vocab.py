@@ -389,3 +389,23 @@ def test_training_step_of_the_text_model():
     assert abs(norm.item() - want) <= 4 * U * want
     for p, q in zip(params, before):
         assert torch.allclose(p.grad, q * 0.5, rtol=1e-6, atol=0)
+
+
+def test_bias_gradient_piece_by_piece():
+    """So many tokens and words that the bias gradient's column sums are reduced after every piece of the vocabulary."""
+    from lvae import decoder_ops as D
+    T, V, H = 66000, 65000, 16
+    g = torch.Generator(device="cuda").manual_seed(0)
+    h = torch.randn(T, H, device="cuda", generator=g).bfloat16()
+    w = (torch.randn(V, H, device="cuda", generator=g) / 4).bfloat16()
+    b = torch.zeros(V, device="cuda", requires_grad=True)
+    y = torch.randint(0, V, (T,), device="cuda", generator=g)
+    D.vocab_cross_entropy(h, w, y, b, reduction="sum").backward()
+    want, mass = torch.zeros(V, device="cuda", dtype=torch.float64), torch.zeros(V, device="cuda", dtype=torch.float64)
+    for rows in range(0, T, 2000):
+        p = torch.softmax(h[rows:rows + 2000].double() @ w.double().t(), 1)
+        mass += p.sum(0)
+    want = mass - torch.bincount(y, minlength=V)
+    tol = 2 * (H + 16) * 2 * U * 40 + 2.0 ** -20 + 8 * U * 10      # of a logit; S below 40: |h| < 5, |w| < 1.3, 16 terms of mean 0.16
+    bound = mass * (2 * tol + 2.0 ** -21) + 64 * U * (mass + torch.bincount(y, minlength=V)) + U * want.abs()
+    assert ((b.grad.double() - want).abs() <= bound).all()

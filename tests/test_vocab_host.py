@@ -67,7 +67,7 @@ def test_call_refusals():
     assert b"no gradient" in lib.lvae_last_error()
     assert lib.lvae_vocab_ll_bwd(problem(), None, 256, s, None, 256, None, None, 256, 1 << 40, None) == -1
     assert lib.lvae_vocab_ll_bwd(problem(), 256, 256, s, None, 256, None, None, 256, 16, None) == -2
-    assert lib.lvae_vocab_loss_f32(problem(), None, 1, -1.0, 256, None) == -1
+    assert lib.lvae_vocab_loss_f32(problem(), None, 1, -1.0, 256, 256, None) == -1
     assert lib.lvae_segment_sum_f32(None, 3, 3, 256, None) == -1 and lib.lvae_segment_sum_f32(256, 3, -1, 256, None) == -1
 
 
