@@ -25,7 +25,8 @@ namespace {
 
 // G in 16 bits is kept relative to the largest upstream gradient: the -1 of a target is then exact (with the 1 / n of a
 // mean inside, all targets would share one rounding error), and fp16, with the largest at 2^14, holds what is 2^-28 of it
-constexpr float F16_G_SCALE = 16384.f;
+constexpr float F16_G_SCALE = 16384.f;       // also of the limbs of float32
+constexpr int MAX_PARTS = 512;              // workgroups that look for the largest magnitude of W, and of H
 
 struct Axes {
     int64_t size[3], stride[3];
@@ -68,7 +69,7 @@ struct RowsArgs {
     const float* gy;            // backward: upstream gradient
     const float* g_scale;
     int64_t T, V, ignore;
-    float g_scale_to;           // what the largest |g| becomes; 0: gradients stay as they are
+    float g_scale_to;           // what the largest |g| becomes
     int64_t* off;               // place of the kept token's hidden state
     int *tok, *tgt_of, *inv;    // its number, its target; and back (-1: not kept)
     float *lse_of, *gy_of, *unscale;
@@ -83,7 +84,11 @@ struct RowsArgs {
     const void* weight;         // copied where the tiles cannot read it as it lies, or NULL
     uint16_t* wpack;
     int64_t wstride;
-    int H, Kp;
+    const void* hidden;
+    int H, Kp, dtype;
+    float* largest;             // limbs: [2][MAX_PARTS] largest magnitudes, of H and of W
+    int h_blocks, w_blocks;
+    int* exponents;
 };
 
 // One workgroup per 1,024 tokens.  Each counts the kept tokens before its own by itself (targets are 8 bytes a token
@@ -98,7 +103,7 @@ __device__ __forceinline__ void list_rows(const RowsArgs& p) {
     float factor = 1.f;
     if (p.gy_of && p.g_scale) factor = p.g_scale[0];
     float norm = 1.f;
-    if (p.gy_of && p.g_scale_to > 0.f) {                              // the same in every workgroup
+    if (p.gy_of) {                              // the same in every workgroup
         float top = 0.f;
         for (int64_t u = threadIdx.x; u < p.T; u += 1024)
             if (p.targets[at_axes(p.tgt, u)] != p.ignore) {
@@ -136,7 +141,7 @@ __device__ __forceinline__ void list_rows(const RowsArgs& p) {
             if (p.lse_of) {
                 p.lse_of[j] = p.lse[t];
                 const float g = -(p.gy[at_axes(p.g, t)] * factor);     // on the negative log-likelihood: G = (softmax - onehot) g
-                p.gy_of[j] = p.g_scale_to > 0.f ? (g / norm) * p.g_scale_to : g;
+                p.gy_of[j] = (g / norm) * p.g_scale_to;
             }
         } else {
             if (p.ll) p.ll[t] = 0.f;
@@ -147,61 +152,119 @@ __device__ __forceinline__ void list_rows(const RowsArgs& p) {
 }
 
 // Row r of hidden (listed, zeros behind the last up to a whole tile) or of W as the tile products read it: Kp columns, zero
-// behind H; float32 as three limb planes.  One wave per row.
-template <int DT> __device__ __forceinline__ void pack_row(const void* src, int64_t base, bool there, int H, int Kp, uint16_t* o, int64_t plane) {
+// behind H; float32 as two limb planes of x 2^e.  One wave per row.
+template <int DT> __device__ __forceinline__ void pack_row(const void* src, int64_t base, bool there, int H, int Kp, int e, uint16_t* o, int64_t plane) {
     for (int k = (threadIdx.x & 63) * 8; k < Kp; k += 512) {
         if constexpr (DT == LVAE_F32) {
             const float* q = (const float*)src + base + k;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = 0.f;
+            for (int i = 0; i < 8; ++i) x[i] = 0.f;
             if (there && k + 8 <= H) {
                 const f32x4 a = *(const f32x4_u*)q, b = *(const f32x4_u*)(q + 4);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) { x[e] = a[e]; x[4 + e] = b[e]; }
+                for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
             } else if (there) {
-                for (int e = 0; e < 8; ++e) if (k + e < H) x[e] = q[e];
+                for (int i = 0; i < 8; ++i) if (k + i < H) x[i] = q[i];
             }
-            s16x8 w[3];
+            s16x8 w[2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                uint16_t l[3];
-                vg_limbs(x[e], l);
-                w[0][e] = l[0]; w[1][e] = l[1]; w[2][e] = l[2];
+            for (int i = 0; i < 8; ++i) {
+                uint16_t l[2];
+                vg_limbs(ldexpf(x[i], e), l);
+                w[0][i] = l[0]; w[1][i] = l[1];
             }
-#pragma unroll
-            for (int l = 0; l < 3; ++l) *(s16x8*)(o + l * plane + k) = w[l];
+            *(s16x8*)(o + k) = w[0];
+            *(s16x8*)(o + plane + k) = w[1];
         } else {
             const uint16_t* q = (const uint16_t*)src + base + k;
             s16x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
             if (there && k + 8 <= H) v = *(const s16x8_u*)q;
             else if (there) {
-                for (int e = 0; e < 8; ++e) if (k + e < H) v[e] = q[e];
+                for (int i = 0; i < 8; ++i) if (k + i < H) v[i] = q[i];
             }
             *(s16x8*)(o + k) = v;
         }
     }
 }
 
-template <int DT> __global__ __launch_bounds__(256) void pack_kernel(const void* src, const int64_t* off, const int* n_rows, int64_t rows,
-                                                                     int H, int Kp, uint16_t* out, int64_t plane) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), n = n_rows[0];
-    if (r >= rows || r >= (n + 255) / 256 * 256) return;
-    const bool there = r < n;
-    pack_row<DT>(src, there ? off[r] : 0, there, H, Kp, out + r * Kp, plane);
+// largest finite magnitude of a float32 row; one wave
+__device__ __forceinline__ float row_largest(const float* row, int H, float top) {
+    const int lane = threadIdx.x & 63;
+    auto take = [&](float x) { const float a = fabsf(x); if (a > top && a < INFINITY) top = a; };
+    int k = lane * 4;
+    for (; k + 4 <= H; k += 256) {
+        const f32x4 v = *(const f32x4_u*)(row + k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) take(v[i]);
+    }
+    for (; k < H; ++k) take(row[k]);
+    return top;
+}
+__device__ __forceinline__ void store_largest(float top, float* to) {        // of 1024 threads
+    __shared__ float red[16];
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) top = fmaxf(top, red[w]);
+        to[0] = top;
+    }
+}
+// e with 2^14 <= largest 2^e < 2^15, from the parts; every thread of a wave gets it
+__device__ __forceinline__ int exponent_for(const float* parts, int n) {
+    float top = 0.f;
+    for (int i = threadIdx.x & 63; i < n; i += 64) top = fmaxf(top, parts[i]);
+    top = wave_max(top);
+    return top > 0.f ? 14 - ilogbf(top) : 0;
 }
 
 // What the products need and does not depend on each other, in one launch: the list of tokens, the bias in float32 with
-// -inf behind the vocabulary (no word beyond the last can count), and the padded copy of W where one is needed.
-template <int DT> __global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
-    if ((int)blockIdx.x < p.row_blocks) {
+// -inf behind the vocabulary (no word beyond the last can count), and for float32 the largest magnitudes of W and of the
+// hidden states that count.
+__global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
+    int b = blockIdx.x;
+    if (b < p.row_blocks) {
         list_rows(p);
-    } else if ((int)blockIdx.x < p.row_blocks + p.bias_blocks) {
-        const int64_t v = (int64_t)(blockIdx.x - p.row_blocks) * 1024 + threadIdx.x;
+        return;
+    }
+    b -= p.row_blocks;
+    if (b < p.bias_blocks) {
+        const int64_t v = (int64_t)b * 1024 + threadIdx.x;
         if (v < p.Vpad) p.bias_out[v] = v >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v, p.bias_dtype) : 0.f;
+        return;
+    }
+    b -= p.bias_blocks;
+    const int wave = threadIdx.x >> 6;
+    float top = 0.f;
+    if (b < p.h_blocks) {
+        for (int64_t t = (int64_t)b * 16 + wave; t < p.T; t += (int64_t)p.h_blocks * 16)
+            if (p.targets[at_axes(p.tgt, t)] != p.ignore) top = row_largest((const float*)p.hidden + at_axes(p.hid, t), p.H, top);
+        store_largest(top, p.largest + b);
     } else {
-        const int64_t r = (int64_t)(blockIdx.x - p.row_blocks - p.bias_blocks) * 16 + (threadIdx.x >> 6);
-        if (r < p.V) pack_row<DT>(p.weight, r * p.wstride, true, p.H, p.Kp, p.wpack + r * p.Kp, p.V * p.Kp);
+        b -= p.h_blocks;
+        for (int64_t v = (int64_t)b * 16 + wave; v < p.V; v += (int64_t)p.w_blocks * 16)
+            top = row_largest((const float*)p.weight + v * p.wstride, p.H, top);
+        store_largest(top, p.largest + MAX_PARTS + b);
+    }
+}
+
+// The operands as the products read them: the listed hidden states, and W where its rows do not serve as they lie.
+template <int DT> __global__ __launch_bounds__(256) void pack_kernel(RowsArgs p, int64_t Tpad, uint16_t* hpack) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    int e = 0;
+    if (DT == LVAE_F32) {
+        e = exponent_for(p.largest + (r < Tpad ? 0 : MAX_PARTS), r < Tpad ? p.h_blocks : p.w_blocks);
+        if (threadIdx.x == 0 && (r == 0 || r == Tpad)) p.exponents[r == 0 ? 0 : 1] = e;
+    }
+    if (r < Tpad) {
+        const int64_t n = p.n_rows[0];
+        if (r >= (n + 255) / 256 * 256) return;
+        const bool there = r < n;
+        pack_row<DT>(p.hidden, there ? p.off[r] : 0, there, p.H, p.Kp, e, hpack + r * p.Kp, Tpad * p.Kp);
+    } else if (r - Tpad < p.V) {
+        const int64_t v = r - Tpad;
+        pack_row<DT>(p.weight, v * p.wstride, true, p.H, p.Kp, e, p.wpack + v * p.Kp, p.V * p.Kp);
     }
 }
 
@@ -428,6 +491,7 @@ struct FinalArgs {
     void* d_bias;
     const int* n_rows;
     const float* unscale;
+    const int* exponents;       // d_hidden of limbs carries that of W
 };
 __global__ __launch_bounds__(256) void final_kernel(FinalArgs p) {
     __shared__ double red[8][32];
@@ -440,7 +504,11 @@ __global__ __launch_bounds__(256) void final_kernel(FinalArgs p) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
         if (j >= 0) {
             for (int s = 0; s < p.splits; ++s) x += *(const f32x4*)(p.slab + s * p.slab_stride + j * p.ld + h);
-            if (p.unscale) x *= p.unscale[0];
+            x *= p.unscale[0];
+            if (p.dt == LVAE_F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = ldexpf(x[e], -p.exponents[1]);
+            }
         }
         const int64_t o = t * p.H + h;
         if (h + 4 > p.H) {
@@ -466,19 +534,20 @@ __global__ __launch_bounds__(256) void final_kernel(FinalArgs p) {
     if (g || v >= p.V) return;
     for (int i = 1; i < 8; ++i) x += red[i][threadIdx.x];
     const float f = (float)x;
-    store_any(p.d_bias, v, p.unscale ? f * p.unscale[0] : f, p.bias_dt);
+    store_any(p.d_bias, v, f * p.unscale[0], p.bias_dt);
 }
 
 // rows [0, rows) of the split weight gradient
 __global__ __launch_bounds__(256) void dweight_kernel(const float* slab, int splits, int64_t slab_stride, int64_t ld,
-                                                      int64_t rows, int H, const float* unscale, void* out, int dt) {
+                                                      int64_t rows, int H, const float* unscale, const int* exponents, void* out, int dt) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= rows * H) return;
     const int64_t v = i / H;
     const int h = (int)(i - v * H);
     float x = 0.f;
     for (int s = 0; s < splits; ++s) x += slab[s * slab_stride + v * ld + h];
-    store_any(out, i, unscale ? x * unscale[0] : x, dt);
+    x *= unscale[0];
+    store_any(out, i, dt == LVAE_F32 ? ldexpf(x, -exponents[0]) : x, dt);
 }
 
 __global__ __launch_bounds__(256) void segment_sum_kernel(const float* x, int64_t n, int64_t len, float* out) {
@@ -523,7 +592,7 @@ struct Plan {
     int64_t piece;              // words of the vocabulary a time (backward)
     int splits_h, splits_w;
     // offsets into the workspace, bytes
-    int64_t off, tok, tgt, inv, lse, gy, head, bias, hpack, wpack, part, picked, g, slab, slab_w, dbias, bytes;
+    int64_t off, tok, tgt, inv, lse, gy, head, largest, bias, hpack, wpack, part, picked, g, slab, slab_w, dbias, bytes;
     int64_t few_blocks, ld_dbias;
 };
 
@@ -546,7 +615,7 @@ int check_problem(const lvae_vocab_problem* q, Plan* pl) {
     pl->Vpad = lvae_round_up(q->V, 256);
     pl->H = q->H;
     pl->Kp = lvae_round_up(q->H, VG_BK);
-    pl->planes = q->dtype == LVAE_F32 ? 3 : 1;
+    pl->planes = q->dtype == LVAE_F32 ? 2 : 1;
     // the tiles read W where it lies if its rows are whole 128-byte slices on 16-byte boundaries; else a padded copy
     pl->direct_w = q->dtype != LVAE_F32 && q->H % VG_BK == 0 && q->weight_stride % 8 == 0 &&
                    q->weight_stride < (1 << 22) && ((uintptr_t)q->weight & 15) == 0;
@@ -564,7 +633,8 @@ int64_t take(int64_t& at, int64_t bytes) {
 
 void plan_common(Plan* pl) {
     int64_t at = 0;
-    pl->head = take(at, 256);                            // n_rows, unscale
+    pl->head = take(at, 256);                            // n_rows, unscale, exponents
+    pl->largest = take(at, 2 * MAX_PARTS * 4);
     pl->off = take(at, pl->Tpad * 8);
     pl->tok = take(at, pl->Tpad * 4);
     pl->tgt = take(at, pl->Tpad * 4);
@@ -686,17 +756,20 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     rows.wstride = q->weight_stride;
     rows.H = q->H;
     rows.Kp = (int)pl.Kp;
-    const int64_t blocks = rows.row_blocks + rows.bias_blocks + (wp ? lvae_ceil_div(pl.V, 16) : 0);
-    const dim3 grid((unsigned)blocks), pack((unsigned)lvae_ceil_div(pl.Tpad, 4));
+    rows.hidden = q->hidden;
+    rows.largest = (float*)(ws + pl.largest);
+    rows.exponents = (int*)(ws + pl.head + 128);
     if (q->dtype == LVAE_F32) {
-        prepare_kernel<LVAE_F32><<<grid, 1024, 0, st>>>(rows);
-        LVAE_LAUNCH_CHECK();
-        pack_kernel<LVAE_F32><<<pack, 256, 0, st>>>(q->hidden, rows.off, rows.n_rows, pl.Tpad, q->H, (int)pl.Kp, hp, pl.Tpad * pl.Kp);
-    } else {                                             // 16 bits are 16 bits
-        prepare_kernel<LVAE_BF16><<<grid, 1024, 0, st>>>(rows);
-        LVAE_LAUNCH_CHECK();
-        pack_kernel<LVAE_BF16><<<pack, 256, 0, st>>>(q->hidden, rows.off, rows.n_rows, pl.Tpad, q->H, (int)pl.Kp, hp, pl.Tpad * pl.Kp);
+        rows.h_blocks = (int)lvae_ceil_div(pl.T, 16);
+        rows.w_blocks = (int)lvae_ceil_div(pl.V, 16);
+        if (rows.h_blocks > MAX_PARTS) rows.h_blocks = MAX_PARTS;
+        if (rows.w_blocks > MAX_PARTS) rows.w_blocks = MAX_PARTS;
     }
+    prepare_kernel<<<dim3((unsigned)(rows.row_blocks + rows.bias_blocks + rows.h_blocks + rows.w_blocks)), 1024, 0, st>>>(rows);
+    LVAE_LAUNCH_CHECK();
+    const dim3 pack((unsigned)lvae_ceil_div(pl.Tpad + (wp ? pl.V : 0), 4));
+    if (q->dtype == LVAE_F32) pack_kernel<LVAE_F32><<<pack, 256, 0, st>>>(rows, pl.Tpad, hp);
+    else pack_kernel<LVAE_BF16><<<pack, 256, 0, st>>>(rows, pl.Tpad, hp);       // 16 bits are 16 bits
     LVAE_LAUNCH_CHECK();
     *a = VgArgs{};
     a->a = (const uint16_t*)q->weight;
@@ -717,6 +790,7 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     a->splits = 1;
     a->bias = bias;
     a->tgt = rows.tgt_of;
+    a->exponents = rows.exponents;
     return LVAE_OK;
 }
 
@@ -839,13 +913,13 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     rows.lse = lse;
     rows.gy = g;
     rows.g_scale = g_scale;
-    rows.g_scale_to = q->dtype == LVAE_F16 ? F16_G_SCALE : q->dtype == LVAE_BF16 ? 1.f : 0.f;
+    rows.g_scale_to = q->dtype == LVAE_BF16 ? 1.f : F16_G_SCALE;
     rows.inv = (int*)(ws + pl.inv);
     rows.lse_of = (float*)(ws + pl.lse);
     rows.gy_of = (float*)(ws + pl.gy);
     VgArgs a;
     RUN(launch_operands(q, pl, rows, ws, &a, st));
-    const float* unscale = rows.g_scale_to > 0.f ? rows.unscale : nullptr;
+    const float* unscale = rows.unscale;
     const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2;
     const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow ? 2 : 4;
     uint16_t* gbuf = (uint16_t*)(ws + pl.g);
@@ -889,6 +963,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     w.ld_slab = pl.Kp;
     w.slab_stride = pl.piece * pl.Kp;
     w.ld_out = pl.H;
+    w.exponents = a.exponents;                           // dWeight carries that of H
     w.unscale = unscale;
     const int mode_w = pl.splits_w > 1 ? VG_DWEIGHT_SLAB : VG_DWEIGHT;
     FinalArgs f = {};
@@ -901,6 +976,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     f.d_bias = d_bias;
     f.n_rows = rows.n_rows;
     f.unscale = unscale;
+    f.exponents = a.exponents;
     for (int64_t v0 = 0; v0 < pl.V; v0 += pl.piece) {
         const int64_t words = pl.V - v0 < pl.piece ? pl.V - v0 : pl.piece;
         dl.a = a.a + v0 * a.lda;
@@ -932,7 +1008,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         }
         if (d_weight && pl.splits_w > 1) {
             dweight_kernel<<<dim3((unsigned)lvae_ceil_div(words * pl.H, 256)), 256, 0, st>>>(
-                w.slab, pl.splits_w, w.slab_stride, w.ld_slab, words, (int)pl.H, unscale, w.out, q->dtype);
+                w.slab, pl.splits_w, w.slab_stride, w.ld_slab, words, (int)pl.H, unscale, a.exponents, w.out, q->dtype);
             LVAE_LAUNCH_CHECK();
         }
     }

@@ -10,9 +10,13 @@
 // an operand stored [k][m] is staged as it lies and read with ds_read_b64_tr_b16, which hands each lane four k values of
 // its own column.
 //
-// float32 operands are three bf16 limbs (x = x1 + x2 + x3, 8 bits each, exact to 2^-24): six limb products, smallest
-// first, on the same code by walking the summed index once per product.  The products left out are below 2^-24 of
-// |a||b|, the rounding of a float32 product itself.
+// float32 operands are two fp16 limbs, x 2^e = x1 + 2^-11 x2 with x1 and x2 rounded to 11 bits each, and e such that the
+// tensor's largest magnitude is just below 2^15: good to 2^-22 of every element down to 2^-29 of the largest, and to an
+// absolute 2^-51 of that below (subnormals).  Three products on the same code by walking the summed index three times:
+// x1 y2 + x2 y1 first, then the sums times 2^-11, then x1 y1; x2 y2, below 2^-22 of |x||y|, is left out.  With the upper
+// limb's own scale the lower one keeps its bits where a plain fp16 remainder would be subnormal (softmax values of
+// unlikely words).  Against three bf16 limbs and six products: half the matrix instructions and two thirds of the bytes
+// (4,096 tokens, width 768, 50,265 words: 1,317 us so, AFTER us with two limbs).
 //
 // Row order.  A lane of the 16x16x32 instruction ends up with rows 4g..4g+3 (g = lane / 16) of each of its eight row
 // tiles.  The rows of W that feed row tile i are chosen as m = 32 g + 4 i + r, so that a lane's 8 x 4 results are 32
@@ -64,18 +68,20 @@ struct VgArgs {
     float* slab;                // [splits][slab_rows][ld_slab] float32 partial products
     int64_t ld_slab, slab_stride;
     int slab_add;               // add to what the slab holds
-    void* out;                  // direct output [N][ld_out] of the operand type (float32 for three limbs)
+    void* out;                  // direct output [N][ld_out] of the operand type (float32 for limbs)
     int64_t ld_out;
     const float* unscale;       // device factor of the outputs, or NULL
+    const int* exponents;       // limbs: e of the hidden states and of the weights
+    int exponent_of;            // which of the two the outputs carry
 };
 
 enum { VG_LSE = 0, VG_GRAD = 1, VG_SLAB = 2, VG_OUT = 3 };
 // the products as launched
 enum { VG_LOGITS_LSE = 0, VG_LOGITS_GRAD = 1, VG_DHIDDEN = 2, VG_DWEIGHT_SLAB = 3, VG_DWEIGHT = 4 };
-// element types: LVAE_F32 (three bf16 limbs), LVAE_BF16, LVAE_F16
+// element types: LVAE_F32 (two fp16 limbs), LVAE_BF16, LVAE_F16
 
 template <int DT> __device__ __forceinline__ f32x4 vg_mma(s16x8 a, s16x8 b, f32x4 c) {
-    if constexpr (DT == LVAE_F16)
+    if constexpr (DT != LVAE_BF16)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -88,13 +94,13 @@ template <int DT> __device__ __forceinline__ uint16_t vg_round(float x) {
 }
 __device__ __forceinline__ float vg_bf16(uint16_t x) { return __uint_as_float((unsigned)x << 16); }
 
-// x as three bf16 limbs; an infinity or NaN stays in the first one
-__device__ __forceinline__ void vg_limbs(float x, uint16_t l[3]) {
-    l[0] = vg_round<LVAE_BF16>(x);
-    float r = x - vg_bf16(l[0]);
-    if (!(fabsf(x) < INFINITY) || !(fabsf(r) < INFINITY)) r = 0.f;
-    l[1] = vg_round<LVAE_BF16>(r);
-    l[2] = vg_round<LVAE_BF16>(r - vg_bf16(l[1]));
+// x as two fp16 limbs, the lower one times 2^11; an infinity or NaN stays in the upper one
+__device__ __forceinline__ void vg_limbs(float x, uint16_t l[2]) {
+    const _Float16 hi = (_Float16)x;
+    float r = (x - (float)hi) * 2048.f;
+    if (!(fabsf((float)hi) < INFINITY)) r = 0.f;
+    l[0] = __builtin_bit_cast(uint16_t, hi);
+    l[1] = vg_round<LVAE_F16>(r);
 }
 
 // 16 bytes a lane from base + off (bytes) to LDS at the wave-uniform byte address lds (+ 16 lane).  As inline assembly:
@@ -186,7 +192,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
     if (N_TOKENS && n0 >= n_lim) return;                // uniform: every wave leaves
     const int64_t k_lim = TRB ? (int64_t)n_kept : p.K;
 
-    constexpr int NP = DT == LVAE_F32 ? 6 : 1;
+    constexpr int NP = DT == LVAE_F32 ? 3 : 1;
     const int ks_all = (int)((k_lim + BK - 1) / BK);
     const int ks_per = (ks_all + p.splits - 1) / p.splits;
     const int ks0 = min(split * ks_per, ks_all), ks = min(ks_per, ks_all - ks0);
@@ -241,9 +247,9 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
     const void *l_a = nullptr, *l_b = nullptr;
     unsigned l_dst_a = 0, l_dst_b = 0;
     bool l_last = false;
-    // limb planes of the six products, smallest first: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+    // limb planes of the three products: (0,1) (1,0) (0,0)
     auto next_a = [&]() {
-        const int limb = na.pair == 1 ? 2 : na.pair == 2 || na.pair == 4 ? 1 : 0;
+        const int limb = na.pair == 1;
         const int64_t kk = (int64_t)(ks0 + na.k) * BK;
         l_a = vg_uniform(abase + limb * p.plane_a + (TRA ? kk * p.lda : kk));
         l_last = TRA && !TRB && (ks0 + na.k == ks_all - 1);
@@ -252,7 +258,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
         na.slot = na.slot + 1 == NA ? 0 : na.slot + 1;
     };
     auto next_b = [&]() {
-        const int limb = DT != LVAE_F32 ? 0 : nb_.pair == 0 ? 2 : nb_.pair == 2 || nb_.pair == 3 ? 1 : 0;
+        const int limb = DT == LVAE_F32 && nb_.pair == 0;
         const int64_t kk = (int64_t)(ks0 + nb_.k) * BK;
         l_b = vg_uniform(bbase + limb * p.plane_b + (TRB ? kk * p.ldb : kk));
         l_dst_b = __builtin_amdgcn_readfirstlane(lds0 + NA * A_BYTES + nb_.slot * B_BYTES + wave * 1024);
@@ -284,7 +290,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        if constexpr (EPI == VG_LSE || EPI == VG_GRAD) x = *(const f32x4*)(p.bias + mb + 4 * i);
+        if constexpr (DT != LVAE_F32 && (EPI == VG_LSE || EPI == VG_GRAD)) x = *(const f32x4*)(p.bias + mb + 4 * i);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) acc[i][j] = x;
     }
@@ -336,6 +342,12 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
         for (int i = 0; i < MI; ++i) read_a(i, la, 0);
         int slot_a = 0, slot_b = 0;
         for (int s = 0; s < steps; ++s) {
+            if (DT == LVAE_F32 && s == 2 * ks) {            // the mixed products are complete
+#pragma unroll
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) acc[i][j] *= 1.f / 2048;
+            }
             // Half a slice is multiplied from registers while the next half is read from LDS and later slices' loads are
             // started, each BETWEEN the matrix instructions, a few cycles behind every NJ of them: the loads of a slice
             // in one go would hold up the wave until the address unit has taken them all.
@@ -399,6 +411,17 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
     __syncthreads();
 
     // ---- epilogues
+    if constexpr (DT == LVAE_F32 && (EPI == VG_LSE || EPI == VG_GRAD)) {
+        const int e = -(p.exponents[0] + p.exponents[1]);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const f32x4 b = *(const f32x4*)(p.bias + mb + 4 * i);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[i][j][r] = ldexpf(acc[i][j][r], e) + b[r];
+        }
+    }
     if constexpr (EPI == VG_LSE) {
         float2* red = (float2*)lds;                     // [WM][TN]; the last barrier has passed
 #pragma unroll
@@ -468,7 +491,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
             }
 #pragma unroll
             for (int i = 0; i < MI; i += 2) {
-                s16x8 o[3];
+                s16x8 o[2];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int ii = i + (e >> 2), r = e & 3;
@@ -476,9 +499,9 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
                     if (!all) x = there ? x : 0.f;
                     colsum[ii][r] += x;
                     if constexpr (DT == LVAE_F32) {
-                        uint16_t l[3];
+                        uint16_t l[2];
                         vg_limbs(x, l);
-                        o[0][e] = l[0]; o[1][e] = l[1]; o[2][e] = l[2];
+                        o[0][e] = l[0]; o[1][e] = l[1];
                     } else {
                         // G is rounded once to the operand type, half a step of each element: the products need a
                         // 16-bit operand, and the gradients are rounded to the same type themselves
@@ -486,7 +509,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
                     }
                 }
 #pragma unroll
-                for (int l = 0; l < (DT == LVAE_F32 ? 3 : 1); ++l) *(s16x8*)(row + l * p.plane_g + 4 * i) = o[l];
+                for (int l = 0; l < (DT == LVAE_F32 ? 2 : 1); ++l) *(s16x8*)(row + l * p.plane_g + 4 * i) = o[l];
             }
         }
         if (p.dbias) {
@@ -515,6 +538,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
         }
     } else {
         const float f = p.unscale ? p.unscale[0] : 1.f;
+        const int e = DT == LVAE_F32 ? -p.exponents[p.exponent_of] : 0;
         const bool whole = mb + 32 <= p.M;              // rows of any alignment: the stores need that of an element alone
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -524,10 +548,13 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
                 float* row = (float*)p.out + n * p.ld_out + mb;
 #pragma unroll
                 for (int i = 0; i < MI; ++i) {
-                    if (whole) *(f32x4_u*)(row + 4 * i) = acc[i][j];
+                    f32x4 o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = ldexpf(acc[i][j][r] * f, e);
+                    if (whole) *(f32x4_u*)(row + 4 * i) = o;
                     else
                         for (int r = 0; r < 4; ++r)
-                            if (mb + 4 * i + r < p.M) row[4 * i + r] = acc[i][j][r];
+                            if (mb + 4 * i + r < p.M) row[4 * i + r] = o[r];
                 }
             } else {
                 uint16_t* row = (uint16_t*)p.out + n * p.ld_out + mb;
