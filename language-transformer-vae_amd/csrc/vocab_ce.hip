@@ -88,7 +88,7 @@ struct RowsArgs {
     int H, Kp, dtype;
     float* largest;             // limbs: [2][MAX_PARTS] largest magnitudes, of H and of W
     int h_blocks, w_blocks;
-    int* exponents;
+    int* exponents;             // found from these, or with no blocks already there
 };
 
 // One workgroup per 1,024 tokens.  Each counts the kept tokens before its own by itself (targets are 8 bytes a token
@@ -254,8 +254,12 @@ template <int DT> __global__ __launch_bounds__(256) void pack_kernel(RowsArgs p,
     const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
     int e = 0;
     if (DT == LVAE_F32) {
-        e = exponent_for(p.largest + (r < Tpad ? 0 : MAX_PARTS), r < Tpad ? p.h_blocks : p.w_blocks);
-        if (threadIdx.x == 0 && (r == 0 || r == Tpad)) p.exponents[r == 0 ? 0 : 1] = e;
+        if (p.w_blocks) {
+            e = exponent_for(p.largest + (r < Tpad ? 0 : MAX_PARTS), r < Tpad ? p.h_blocks : p.w_blocks);
+            if (threadIdx.x == 0 && (r == 0 || r == Tpad)) p.exponents[r == 0 ? 0 : 1] = e;
+        } else {
+            e = p.exponents[r < Tpad ? 0 : 1];
+        }
     }
     if (r < Tpad) {
         const int64_t n = p.n_rows[0];
@@ -758,8 +762,9 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     rows.Kp = (int)pl.Kp;
     rows.hidden = q->hidden;
     rows.largest = (float*)(ws + pl.largest);
-    rows.exponents = (int*)(ws + pl.head + 128);
-    if (q->dtype == LVAE_F32) {
+    const bool known = rows.exponents && rows.lse_of;        // a backward that got those of its forward
+    if (!rows.exponents) rows.exponents = (int*)(ws + pl.head + 128);
+    if (q->dtype == LVAE_F32 && !known) {
         rows.h_blocks = (int)lvae_ceil_div(pl.T, 16);
         rows.w_blocks = (int)lvae_ceil_div(pl.V, 16);
         if (rows.h_blocks > MAX_PARTS) rows.h_blocks = MAX_PARTS;
@@ -831,7 +836,8 @@ extern "C" int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* q, int64_
     return LVAE_OK;
 }
 
-extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, void* wsv, int64_t ws_bytes, void* stream) {
+extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, int32_t* exponents, void* wsv, int64_t ws_bytes,
+                             void* stream) {
     Plan pl = {};
     RUN(check_problem(q, &pl));
     RUN(check_data(q));
@@ -872,6 +878,7 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     RowsArgs rows = rows_args(q, pl, ws);
     rows.ll = ll;
     rows.lse_out = lse;
+    rows.exponents = exponents;
     VgArgs a;
     RUN(launch_operands(q, pl, rows, ws, &a, st));
     a.M = pl.V;
@@ -897,8 +904,8 @@ extern "C" int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* q, in
 }
 
 extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, const float* g, const int64_t* g_stride,
-                                 const float* g_scale, void* d_hidden, void* d_weight, void* d_bias, void* wsv,
-                                 int64_t ws_bytes, void* stream) {
+                                 const float* g_scale, const int32_t* exponents, void* d_hidden, void* d_weight,
+                                 void* d_bias, void* wsv, int64_t ws_bytes, void* stream) {
     Plan pl = {};
     RUN(check_problem(q, &pl));
     RUN(check_data(q));
@@ -917,6 +924,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     rows.inv = (int*)(ws + pl.inv);
     rows.lse_of = (float*)(ws + pl.lse);
     rows.gy_of = (float*)(ws + pl.gy);
+    rows.exponents = const_cast<int32_t*>(exponents);     // read only: w_blocks stays 0
     VgArgs a;
     RUN(launch_operands(q, pl, rows, ws, &a, st));
     const float* unscale = rows.unscale;

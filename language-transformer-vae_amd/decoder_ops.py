@@ -117,22 +117,25 @@ def _pointers(tensors):
 
 
 def _forward(q, want_lse):
-    """(ll, lse or None), both [*token dimensions] float32."""
+    """(ll, lse or None, exponents or None): [*token dimensions] float32, and what the backward of float32 operands needs
+    besides."""
     dev = q.device
     ll = torch.empty(q.shape, dtype=torch.float32, device=dev)
     lse = torch.empty(q.shape, dtype=torch.float32, device=dev) if want_lse else None
+    limbs = want_lse and q.T > N.VOCAB_FEW and q.c.dtype == N.DTYPES[torch.float32]
+    exponents = torch.empty(2, dtype=torch.int32, device=dev) if limbs else None
     if q.T:
         nbytes = N._i64(0)
         with N.on_device(q.index):
             lib = N.lib()
             N.check(lib.lvae_vocab_ll_workspace_bytes(q.c, nbytes))
             ws = N.workspace(nbytes.value, dev)
-            N.check(lib.lvae_vocab_ll(q.c, ll.data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(),
-                                      nbytes.value, N.raw_stream(q.index)))
-    return ll, lse
+            p = _pointers((ll, lse, exponents))
+            N.check(lib.lvae_vocab_ll(q.c, p[0], p[1], p[2], ws.data_ptr(), nbytes.value, N.raw_stream(q.index)))
+    return ll, lse, exponents
 
 
-def _backward(q, tensors, needs, lse, g, g_strides, g_scale):
+def _backward(q, tensors, needs, lse, g, g_strides, g_scale, exponents):
     """Gradients of hidden, weight, bias (None where not needed); g is read with the strides given, one per token axis
     of the problem."""
     hidden, weight, _, bias = tensors
@@ -147,9 +150,9 @@ def _backward(q, tensors, needs, lse, g, g_strides, g_scale):
             lib = N.lib()
             N.check(lib.lvae_vocab_ll_bwd_workspace_bytes(q.c, needs[0], needs[1], needs[2], nbytes))
             ws = N.workspace(nbytes.value, dev)
-            p = _pointers((lse, g, g_scale, d_h, d_w, d_b))
-            N.check(lib.lvae_vocab_ll_bwd(q.c, p[0], p[1], _Three(*g_strides), p[2], p[3], p[4], p[5], ws.data_ptr(),
-                                          nbytes.value, N.raw_stream(q.index)))
+            p = _pointers((lse, g, g_scale, exponents, d_h, d_w, d_b))
+            N.check(lib.lvae_vocab_ll_bwd(q.c, p[0], p[1], _Three(*g_strides), *p[2:], ws.data_ptr(), nbytes.value,
+                                          N.raw_stream(q.index)))
     return d_h, d_w, d_b
 
 
@@ -191,17 +194,17 @@ class _VocabLL(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, ignore_index, how):
         q = _Problem(hidden.detach(), weight.detach(), targets, None if bias is None else bias.detach(), ignore_index)
-        ll, lse = _forward(q, True)
+        ll, lse, exponents = _forward(q, True)
         out, factor = _put_together(q, ll, how)
         tensors, ctx.plan = q.without_tensors()
-        ctx.save_for_backward(*tensors, lse, factor)
+        ctx.save_for_backward(*tensors, lse, factor, exponents)
         ctx.how = how
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        *tensors, lse, factor = ctx.saved_tensors
+        *tensors, lse, factor, exponents = ctx.saved_tensors
         needs = ctx.needs_input_grad[:3]
         if not any(needs):
             return None, None, None, None, None, None
@@ -214,7 +217,7 @@ class _VocabLL(torch.autograd.Function):
             # sequences: one value for all positions of a sentence; the problem's axes join dimensions, so spread it out
             g = (g if ctx.how == _TOKENS else g.unsqueeze(-1).expand(q.shape)).contiguous()
             strides = _token_strides(q)
-        return (*_backward(q, tensors, needs, lse, g, strides, factor), None, None, None)
+        return (*_backward(q, tensors, needs, lse, g, strides, factor, exponents), None, None, None)
 
 
 def _run(hidden, weight, targets, bias, ignore_index, how):
