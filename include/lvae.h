@@ -447,11 +447,13 @@ typedef struct {
  * NULL.  Up to LVAE_VOCAB_FEW tokens the weights are streamed once past all tokens in registers; beyond, matrix-core
  * tiles (float32 as two fp16 limbs).  exponents [2] int32 on the device, or NULL: written by float32 calls of more than
  * LVAE_VOCAB_FEW tokens, the powers of two that hidden and weight are scaled by; handed to the backward of the same
- * inputs they save it a read of weight. */
+ * inputs they save it a read of weight.  loss, each [1] float32 on the device, or both NULL: loss = -sum(ll), with
+ * mean != 0 over max(1, tokens whose target is not ignore_index); each, the factor of each ll in it (the g_scale of the
+ * backward). */
 #define LVAE_VOCAB_FEW 64
 int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* problem, int64_t* out_bytes);
-int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, int32_t* exponents, void* ws, int64_t ws_bytes,
-                  void* stream);
+int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, int32_t* exponents, float* loss, float* each,
+                  int mean, void* ws, int64_t ws_bytes, void* stream);
 
 /* Backward: g is the upstream gradient on ll, over the token axes with strides g_stride (0: shared), times the device
  * scalar g_scale if that is given.  exponents: those of the forward, or NULL.  d_hidden [tokens, H], d_weight [V, H]
@@ -462,11 +464,6 @@ int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* problem, int wan
 int lvae_vocab_ll_bwd(const lvae_vocab_problem* problem, const float* lse, const float* g, const int64_t* g_stride,
                       const float* g_scale, const int32_t* exponents, void* d_hidden, void* d_weight, void* d_bias,
                       void* ws, int64_t ws_bytes, void* stream);
-
-/* loss = factor * sum(ll); with mean != 0, over max(1, tokens whose target is not ignore_index).  each: the factor of
- * each ll in it (the g_scale of the backward).  Both float32 on the device; one workgroup, float64. */
-int lvae_vocab_loss_f32(const lvae_vocab_problem* problem, const float* ll, int mean, float factor, float* loss,
-                        float* each, void* stream);
 
 /* out[i] = sum_k x[i * len + k], float64 inside; len may be 0. */
 int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream);

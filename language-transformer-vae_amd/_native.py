@@ -122,13 +122,12 @@ _SIGNATURES = {
     "lvae_kernel_matrix_f32": (_int, [_c_f32p, _c_f32p, _i64, _i64, _int, ctypes.POINTER(_f32), _int, _f32,
                                       _c_f32p, ctypes.c_void_p, _i64, ctypes.c_void_p]),
     "lvae_vocab_ll_workspace_bytes": (_int, [ctypes.POINTER(VocabProblem), ctypes.POINTER(_i64)]),
-    "lvae_vocab_ll": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.c_void_p, ctypes.c_void_p, _i64,
-                             ctypes.c_void_p]),
+    "lvae_vocab_ll": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.c_void_p, _c_f32p, _c_f32p, _int,
+                             ctypes.c_void_p, _i64, ctypes.c_void_p]),
     "lvae_vocab_ll_bwd_workspace_bytes": (_int, [ctypes.POINTER(VocabProblem), _int, _int, _int, ctypes.POINTER(_i64)]),
     "lvae_vocab_ll_bwd": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.POINTER(_i64), _c_f32p,
                                  ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _i64,
                                  ctypes.c_void_p]),
-    "lvae_vocab_loss_f32": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _int, _f32, _c_f32p, _c_f32p, ctypes.c_void_p]),
     "lvae_segment_sum_f32": (_int, [_c_f32p, _i64, _i64, _c_f32p, ctypes.c_void_p]),
     "lvae_clip_workspace_bytes": (_int, [_i64, ctypes.POINTER(_i64)]),
     "lvae_clip_grads": (_int, [ctypes.c_void_p, _i64, _int, _int, ctypes.c_double, _c_f32p, ctypes.c_void_p, _i64,

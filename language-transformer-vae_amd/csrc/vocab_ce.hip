@@ -70,11 +70,13 @@ struct RowsArgs {
     const float* g_scale;
     int64_t T, V, ignore;
     float g_scale_to;           // what the largest |g| becomes
-    int64_t* off;               // place of the kept token's hidden state
-    int *tok, *tgt_of, *inv;    // its number, its target; and back (-1: not kept)
+    int *tok, *tgt_of, *inv;    // of each kept token its number and its target; and back (-1: not kept)
     float *lse_of, *gy_of, *unscale;
     float *ll, *lse_out;        // forward: zeros for tokens that do not count
-    int* n_rows;
+    int* n_rows;                // [2]: kept tokens; a counter, set to 0
+    int64_t tokens;             // of a workgroup, a multiple of 16
+    uint16_t* hpack;            // their hidden states
+    int64_t hplane;
     // the other workgroups of the launch
     int row_blocks, bias_blocks;
     const void* bias;
@@ -85,74 +87,13 @@ struct RowsArgs {
     uint16_t* wpack;
     int64_t wstride;
     const void* hidden;
-    int H, Kp, dtype;
+    int H, Kp;
     float* largest;             // limbs: [2][MAX_PARTS] largest magnitudes, of H and of W
     int h_blocks, w_blocks;
     int* exponents;             // found from these, or with no blocks already there
 };
 
-// One workgroup per 1,024 tokens.  Each counts the kept tokens before its own by itself (targets are 8 bytes a token
-// and stay in L2; at 65,536 tokens the last workgroup reads 512 KB) instead of a second launch for the prefix.
-__device__ __forceinline__ void list_rows(const RowsArgs& p) {
-    __shared__ int red[16];
-    __shared__ float redf[16];
-    const int64_t first = (int64_t)blockIdx.x * 1024;
-    int before = 0;
-    for (int64_t u = threadIdx.x; u < first; u += 1024) before += p.targets[at_axes(p.tgt, u)] != p.ignore;
-    before = block_sum_int(before, red);
-    float factor = 1.f;
-    if (p.gy_of && p.g_scale) factor = p.g_scale[0];
-    float norm = 1.f;
-    if (p.gy_of) {                              // the same in every workgroup
-        float top = 0.f;
-        for (int64_t u = threadIdx.x; u < p.T; u += 1024)
-            if (p.targets[at_axes(p.tgt, u)] != p.ignore) {
-                const float a = fabsf(p.gy[at_axes(p.g, u)] * factor);
-                top = a > top ? a : top;
-            }
-        top = wave_max(top);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) redf[threadIdx.x >> 6] = top;
-        __syncthreads();
-        for (int w = 0; w < 16; ++w) norm = w == 0 ? redf[0] : fmaxf(norm, redf[w]);
-        if (!(norm > 0.f) || !(norm < INFINITY)) norm = p.g_scale_to;      // nothing to keep in range: a factor of 1
-        if (blockIdx.x == 0 && threadIdx.x == 0) p.unscale[0] = norm / p.g_scale_to;
-    }
-    const int64_t t = first + threadIdx.x;
-    const int64_t y = t < p.T ? p.targets[at_axes(p.tgt, t)] : p.ignore;
-    const bool keep = t < p.T && y != p.ignore;
-    const unsigned long long mask = __ballot(keep);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    __syncthreads();
-    if (lane == 0) red[wave] = __popcll(mask);
-    __syncthreads();
-    int64_t j = before + __popcll(mask & ((1ull << lane) - 1));
-    int all = 0;
-    for (int w = 0; w < 16; ++w) {
-        if (w < wave) j += red[w];
-        all += red[w];
-    }
-    if (t < p.T) {
-        if (p.inv) p.inv[t] = keep ? (int)j : -1;
-        if (keep) {
-            p.off[j] = at_axes(p.hid, t);
-            p.tok[j] = (int)t;
-            p.tgt_of[j] = y >= 0 && y < p.V ? (int)y : -2;
-            if (p.lse_of) {
-                p.lse_of[j] = p.lse[t];
-                const float g = -(p.gy[at_axes(p.g, t)] * factor);     // on the negative log-likelihood: G = (softmax - onehot) g
-                p.gy_of[j] = (g / norm) * p.g_scale_to;
-            }
-        } else {
-            if (p.ll) p.ll[t] = 0.f;
-            if (p.lse_out) p.lse_out[t] = 0.f;
-        }
-    }
-    if ((int)blockIdx.x == p.row_blocks - 1 && threadIdx.x == 0) p.n_rows[0] = before + all;
-}
-
-// Row r of hidden (listed, zeros behind the last up to a whole tile) or of W as the tile products read it: Kp columns, zero
-// behind H; float32 as two limb planes of x 2^e.  One wave per row.
+// A row of hidden or of W as the tile products read it: Kp columns, zero behind H; float32 as two limb planes of x 2^e.  One wave per row.
 template <int DT> __device__ __forceinline__ void pack_row(const void* src, int64_t base, bool there, int H, int Kp, int e, uint16_t* o, int64_t plane) {
     for (int k = (threadIdx.x & 63) * 8; k < Kp; k += 512) {
         if constexpr (DT == LVAE_F32) {
@@ -219,22 +160,9 @@ __device__ __forceinline__ int exponent_for(const float* parts, int n) {
     return top > 0.f ? 14 - ilogbf(top) : 0;
 }
 
-// What the products need and does not depend on each other, in one launch: the list of tokens, the bias in float32 with
-// -inf behind the vocabulary (no word beyond the last can count), and for float32 the largest magnitudes of W and of the
-// hidden states that count.
-__global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
+// For float32: the largest magnitudes of W and of the hidden states that count, from which the exponents follow.
+__global__ __launch_bounds__(1024) void largest_kernel(RowsArgs p) {
     int b = blockIdx.x;
-    if (b < p.row_blocks) {
-        list_rows(p);
-        return;
-    }
-    b -= p.row_blocks;
-    if (b < p.bias_blocks) {
-        const int64_t v = (int64_t)b * 1024 + threadIdx.x;
-        if (v < p.Vpad) p.bias_out[v] = v >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v, p.bias_dtype) : 0.f;
-        return;
-    }
-    b -= p.bias_blocks;
     const int wave = threadIdx.x >> 6;
     float top = 0.f;
     if (b < p.h_blocks) {
@@ -249,27 +177,117 @@ __global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
     }
 }
 
-// The operands as the products read them: the listed hidden states, and W where its rows do not serve as they lie.
-template <int DT> __global__ __launch_bounds__(256) void pack_kernel(RowsArgs p, int64_t Tpad, uint16_t* hpack) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    int e = 0;
-    if (DT == LVAE_F32) {
-        if (p.w_blocks) {
-            e = exponent_for(p.largest + (r < Tpad ? 0 : MAX_PARTS), r < Tpad ? p.h_blocks : p.w_blocks);
-            if (threadIdx.x == 0 && (r == 0 || r == Tpad)) p.exponents[r == 0 ? 0 : 1] = e;
+// The tokens [first, end) of one workgroup: those that count go into the list, in order, and their hidden states into the
+// operand.  How many count before `first` every workgroup finds by itself (8 bytes a token, from L2; at most 512
+// workgroups do so) instead of in a launch of its own.
+template <int DT> __device__ __forceinline__ void list_rows(const RowsArgs& p, int e) {
+    __shared__ int red[16];
+    __shared__ float redf[16];
+    __shared__ int row_of[1024];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * p.tokens, end = min(first + p.tokens, p.T);
+    int count = 0;
+    for (int64_t u = threadIdx.x; u < first; u += 1024) count += p.targets[at_axes(p.tgt, u)] != p.ignore;
+    int base = block_sum_int(count, red);
+    float factor = 1.f, norm = 1.f;
+    if (p.gy_of) {
+        if (p.g_scale) factor = p.g_scale[0];
+        float top = 0.f;                        // the largest upstream gradient, the same in every workgroup
+        if ((p.g.stride[0] | p.g.stride[1] | p.g.stride[2]) == 0) {
+            top = fabsf(p.gy[0] * factor);
+            if (!(top >= 0.f)) top = 0.f;
         } else {
-            e = p.exponents[r < Tpad ? 0 : 1];
+            for (int64_t u = threadIdx.x; u < p.T; u += 1024)
+                if (p.targets[at_axes(p.tgt, u)] != p.ignore) {
+                    const float a = fabsf(p.gy[at_axes(p.g, u)] * factor);
+                    top = a > top ? a : top;
+                }
+        }
+        top = wave_max(top);
+        __syncthreads();
+        if (lane == 0) redf[wave] = top;
+        __syncthreads();
+        norm = redf[0];
+        for (int w = 1; w < 16; ++w) norm = fmaxf(norm, redf[w]);
+        if (!(norm > 0.f) || !(norm < INFINITY)) norm = p.g_scale_to;      // nothing to keep in range: a factor of 1
+        if (blockIdx.x == 0 && threadIdx.x == 0) p.unscale[0] = norm / p.g_scale_to;
+    }
+    for (int64_t c = first; c < end; c += 1024) {
+        const int64_t t = c + threadIdx.x;
+        const int64_t y = t < end ? p.targets[at_axes(p.tgt, t)] : p.ignore;
+        const bool keep = t < end && y != p.ignore;
+        const unsigned long long mask = __ballot(keep);
+        __syncthreads();
+        if (lane == 0) red[wave] = __popcll(mask);
+        __syncthreads();
+        int j = base + __popcll(mask & ((1ull << lane) - 1));
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) j += red[w];
+            base += red[w];
+        }
+        row_of[threadIdx.x] = keep ? j : -1;
+        if (t < end) {
+            if (p.inv) p.inv[t] = keep ? j : -1;
+            if (keep) {
+                p.tok[j] = (int)t;
+                p.tgt_of[j] = y >= 0 && y < p.V ? (int)y : -2;
+                if (p.lse_of) {
+                    p.lse_of[j] = p.lse[t];
+                    const float g = -(p.gy[at_axes(p.g, t)] * factor);     // on the negative log-likelihood: G = (softmax - onehot) g
+                    p.gy_of[j] = (g / norm) * p.g_scale_to;
+                }
+            } else {
+                if (p.ll) p.ll[t] = 0.f;
+                if (p.lse_out) p.lse_out[t] = 0.f;
+            }
+        }
+        __syncthreads();
+        const int here = (int)min((int64_t)1024, end - c);
+        for (int i = wave; i < here; i += 16)
+            if (row_of[i] >= 0)
+                pack_row<DT>(p.hidden, at_axes(p.hid, c + i), true, p.H, p.Kp, e, p.hpack + (int64_t)row_of[i] * p.Kp, p.hplane);
+    }
+    if ((int)blockIdx.x == p.row_blocks - 1) {
+        // the product of dWeight reads whole slices of tokens: zeros behind the last
+        for (int64_t r = base + wave; r < (base + VG_BK - 1) / VG_BK * VG_BK; r += 16)
+            pack_row<DT>(p.hidden, 0, false, p.H, p.Kp, e, p.hpack + r * p.Kp, p.hplane);
+        if (threadIdx.x == 0) {
+            p.n_rows[0] = base;
+            p.n_rows[1] = 0;                    // the counter of finish_kernel
         }
     }
-    if (r < Tpad) {
-        const int64_t n = p.n_rows[0];
-        if (r >= (n + 255) / 256 * 256) return;
-        const bool there = r < n;
-        pack_row<DT>(p.hidden, there ? p.off[r] : 0, there, p.H, p.Kp, e, hpack + r * p.Kp, Tpad * p.Kp);
-    } else if (r - Tpad < p.V) {
-        const int64_t v = r - Tpad;
-        pack_row<DT>(p.weight, v * p.wstride, true, p.H, p.Kp, e, p.wpack + v * p.Kp, p.V * p.Kp);
+}
+
+// All operands of the products in one launch: the list of tokens and their hidden states, the bias in float32 with -inf
+// behind the vocabulary (no word beyond the last can count), and a padded copy of W where its rows do not serve as they
+// lie.
+template <int DT> __global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
+    int b = blockIdx.x, e_h = 0, e_w = 0;
+    if (DT == LVAE_F32) {
+        if (p.w_blocks) {
+            e_h = exponent_for(p.largest, p.h_blocks);
+            e_w = exponent_for(p.largest + MAX_PARTS, p.w_blocks);
+            if (b == 0 && threadIdx.x == 0) {
+                p.exponents[0] = e_h;
+                p.exponents[1] = e_w;
+            }
+        } else {
+            e_h = p.exponents[0];
+            e_w = p.exponents[1];
+        }
     }
+    if (b < p.row_blocks) {
+        list_rows<DT>(p, e_h);
+        return;
+    }
+    b -= p.row_blocks;
+    if (b < p.bias_blocks) {
+        const int64_t v = (int64_t)b * 1024 + threadIdx.x;
+        if (v < p.Vpad) p.bias_out[v] = v >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v, p.bias_dtype) : 0.f;
+        return;
+    }
+    const int64_t r = (int64_t)(b - p.bias_blocks) * 16 + (threadIdx.x >> 6);
+    if (r < p.V) pack_row<DT>(p.weight, r * p.wstride, true, p.H, p.Kp, e_w, p.wpack + r * p.Kp, p.V * p.Kp);
 }
 
 __device__ __forceinline__ float2 merge_lse(float2 a, float2 b) {
@@ -277,33 +295,70 @@ __device__ __forceinline__ float2 merge_lse(float2 a, float2 b) {
     return make_float2(top, a.y * lvae_exp2((a.x - ref) * LVAE_LOG2E) + b.y * lvae_exp2((b.x - ref) * LVAE_LOG2E));
 }
 
-// LSE of each kept token from its partials [tiles][ldp]; 16 tokens a workgroup, 16 threads a token
-__global__ __launch_bounds__(256) void finish_kernel(const float2* part, int tiles, int64_t ldp, const float* picked,
-                                                     const int* tok, const int* tgt, const int* n_rows, float* ll,
-                                                     float* lse) {
+struct FinishArgs {
+    const float2* part;         // [tiles][ldp]
+    int tiles;
+    int64_t ldp;
+    const float* picked;
+    const int *tok, *tgt;
+    int* n_rows;                // [2]: kept tokens; workgroups that are done
+    float *ll, *lse;
+    float *loss, *each;         // -sum of ll (over the kept tokens with `mean`) and the factor of each in it, or NULL
+    double* sums;               // [workgroups]
+    int mean;
+};
+// LSE of each kept token from its partials; 16 tokens a workgroup, 16 threads a token.  The loss, where one is asked for:
+// every workgroup leaves the sum of its tokens, and the last one to be done adds them up in order.
+__global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
     __shared__ float2 red[16][16];
+    __shared__ double redd[4];
+    __shared__ int last;
     const int64_t j = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
     const int g = threadIdx.x >> 4;
-    const int64_t n = n_rows[0];
+    const int64_t n = p.n_rows[0];
     float2 x = make_float2(-INFINITY, 0.f);
     if (j < n)
-        for (int i = g; i < tiles; i += 64) {
+        for (int i = g; i < p.tiles; i += 64) {
             float2 y[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                y[u] = i + 16 * u < tiles ? part[(int64_t)(i + 16 * u) * ldp + j] : make_float2(-INFINITY, 0.f);
+                y[u] = i + 16 * u < p.tiles ? p.part[(int64_t)(i + 16 * u) * p.ldp + j] : make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int u = 0; u < 4; ++u) x = merge_lse(x, y[u]);
         }
     red[g][threadIdx.x & 15] = x;
     __syncthreads();
+    double mine = 0.0;
     if (g == 0 && j < n) {
         for (int i = 1; i < 16; ++i) x = merge_lse(x, red[i][threadIdx.x]);
         float l = x.x + logf(x.y);
-        const bool bad = tgt[j] < 0;
+        const bool bad = p.tgt[j] < 0;
         if (bad) l = NAN;
-        ll[tok[j]] = bad ? NAN : picked[j] - l;
-        if (lse) lse[tok[j]] = l;
+        const float v = bad ? NAN : p.picked[j] - l;
+        p.ll[p.tok[j]] = v;
+        if (p.lse) p.lse[p.tok[j]] = l;
+        mine = v;
+    }
+    if (!p.loss) return;
+    if (threadIdx.x < 64) {
+        mine = wave_sum_d(mine);
+        if (threadIdx.x == 0) {
+            __hip_atomic_store(p.sums + blockIdx.x, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last = __hip_atomic_fetch_add(p.n_rows + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += 256)
+        s += __hip_atomic_load(p.sums + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s = wave_sum_d(s);
+    if ((threadIdx.x & 63) == 0) redd[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const double f = -1.0 / (p.mean ? (double)max((int64_t)1, n) : 1.0);
+        p.loss[0] = (float)((redd[0] + redd[1] + redd[2] + redd[3]) * f);
+        p.each[0] = (float)f;
     }
 }
 
@@ -563,25 +618,15 @@ __global__ __launch_bounds__(256) void segment_sum_kernel(const float* x, int64_
     if ((threadIdx.x & 63) == 0) out[s] = (float)a;
 }
 
-__global__ __launch_bounds__(1024) void loss_kernel(const int64_t* targets, Axes tgt, int64_t T, int64_t ignore,
-                                                    const float* ll, int mean, float factor, float* loss,
-                                                    float* each) {
-    __shared__ double red[16];
-    __shared__ int redi[16];
-    double a = 0.0;
-    int c = 0;
-    for (int64_t t = threadIdx.x; t < T; t += 1024) {
-        a += ll[t];
-        if (mean) c += targets[at_axes(tgt, t)] != ignore;
-    }
-    a = wave_sum_d(a);
-    c = block_sum_int(c, redi);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double s = 0.0;
-        for (int w = 0; w < 16; ++w) s += red[w];
-        const double f = (double)factor / (mean ? (double)max(1, c) : 1.0);
+// the loss of few tokens
+__global__ __launch_bounds__(64) void few_loss_kernel(const int64_t* targets, Axes tgt, int T, int64_t ignore, const float* ll,
+                                                      int mean, float* loss, float* each) {
+    const int t = threadIdx.x;                  // at most LVAE_VOCAB_FEW tokens
+    static_assert(LVAE_VOCAB_FEW <= 64, "one wave");
+    const double s = wave_sum_d(t < T ? (double)ll[t] : 0.0);
+    const int n = __popcll(__ballot(t < T && targets[at_axes(tgt, t < T ? t : 0)] != ignore));
+    if (t == 0) {
+        const double f = -1.0 / (mean ? (double)max(1, n) : 1.0);
         loss[0] = (float)(s * f);
         each[0] = (float)f;
     }
@@ -596,7 +641,7 @@ struct Plan {
     int64_t piece;              // words of the vocabulary a time (backward)
     int splits_h, splits_w;
     // offsets into the workspace, bytes
-    int64_t off, tok, tgt, inv, lse, gy, head, largest, bias, hpack, wpack, part, picked, g, slab, slab_w, dbias, bytes;
+    int64_t tok, tgt, inv, lse, gy, head, largest, bias, hpack, wpack, part, picked, sums, g, slab, slab_w, dbias, bytes;
     int64_t few_blocks, ld_dbias;
 };
 
@@ -639,7 +684,6 @@ void plan_common(Plan* pl) {
     int64_t at = 0;
     pl->head = take(at, 256);                            // n_rows, unscale, exponents
     pl->largest = take(at, 2 * MAX_PARTS * 4);
-    pl->off = take(at, pl->Tpad * 8);
     pl->tok = take(at, pl->Tpad * 4);
     pl->tgt = take(at, pl->Tpad * 4);
     pl->bias = take(at, pl->Vpad * 4);
@@ -662,6 +706,7 @@ void plan_forward(Plan* pl) {
     int64_t at = pl->bytes;
     pl->part = take(at, pl->Vpad / 256 * pl->Tpad * 8);
     pl->picked = take(at, pl->Tpad * 4);
+    pl->sums = take(at, pl->Tpad / 16 * 8);
     pl->bytes = at;
 }
 
@@ -749,7 +794,10 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     uint16_t* hp = (uint16_t*)(ws + pl.hpack);
     uint16_t* wp = pl.direct_w ? nullptr : (uint16_t*)(ws + pl.wpack);
     float* bias = (float*)(ws + pl.bias);
-    rows.row_blocks = (int)lvae_ceil_div(pl.T, 1024);
+    rows.tokens = lvae_round_up(lvae_ceil_div(pl.T, 512), 16);
+    rows.hpack = hp;
+    rows.hplane = pl.Tpad * pl.Kp;
+    rows.row_blocks = (int)lvae_ceil_div(pl.T, rows.tokens);
     rows.bias_blocks = (int)lvae_ceil_div(pl.Vpad, 1024);
     rows.bias = q->bias;
     rows.bias_out = bias;
@@ -769,12 +817,12 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
         rows.w_blocks = (int)lvae_ceil_div(pl.V, 16);
         if (rows.h_blocks > MAX_PARTS) rows.h_blocks = MAX_PARTS;
         if (rows.w_blocks > MAX_PARTS) rows.w_blocks = MAX_PARTS;
+        largest_kernel<<<dim3((unsigned)(rows.h_blocks + rows.w_blocks)), 1024, 0, st>>>(rows);
+        LVAE_LAUNCH_CHECK();
     }
-    prepare_kernel<<<dim3((unsigned)(rows.row_blocks + rows.bias_blocks + rows.h_blocks + rows.w_blocks)), 1024, 0, st>>>(rows);
-    LVAE_LAUNCH_CHECK();
-    const dim3 pack((unsigned)lvae_ceil_div(pl.Tpad + (wp ? pl.V : 0), 4));
-    if (q->dtype == LVAE_F32) pack_kernel<LVAE_F32><<<pack, 256, 0, st>>>(rows, pl.Tpad, hp);
-    else pack_kernel<LVAE_BF16><<<pack, 256, 0, st>>>(rows, pl.Tpad, hp);       // 16 bits are 16 bits
+    const dim3 grid((unsigned)(rows.row_blocks + rows.bias_blocks + (wp ? lvae_ceil_div(pl.V, 16) : 0)));
+    if (q->dtype == LVAE_F32) prepare_kernel<LVAE_F32><<<grid, 1024, 0, st>>>(rows);
+    else prepare_kernel<LVAE_BF16><<<grid, 1024, 0, st>>>(rows);       // 16 bits are 16 bits
     LVAE_LAUNCH_CHECK();
     *a = VgArgs{};
     a->a = (const uint16_t*)q->weight;
@@ -807,7 +855,6 @@ RowsArgs rows_args(const lvae_vocab_problem* q, const Plan& pl, char* ws) {
     r.T = pl.T;
     r.V = pl.V;
     r.ignore = q->ignore_index;
-    r.off = (int64_t*)(ws + pl.off);
     r.tok = (int*)(ws + pl.tok);
     r.tgt_of = (int*)(ws + pl.tgt);
     r.n_rows = (int*)(ws + pl.head);
@@ -836,12 +883,13 @@ extern "C" int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* q, int64_
     return LVAE_OK;
 }
 
-extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, int32_t* exponents, void* wsv, int64_t ws_bytes,
-                             void* stream) {
+extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, int32_t* exponents, float* loss, float* each,
+                             int mean, void* wsv, int64_t ws_bytes, void* stream) {
     Plan pl = {};
     RUN(check_problem(q, &pl));
     RUN(check_data(q));
     LVAE_CHECK_ARG(ll, "ll must be non-NULL");
+    LVAE_CHECK_ARG(!loss == !each, "loss and each go together");
     plan_forward(&pl);
     RUN(check_ws(pl, wsv, ws_bytes));
     hipStream_t st = (hipStream_t)stream;
@@ -873,6 +921,10 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
         LVAE_LAUNCH_CHECK();
         few_finish_kernel<<<dim3((unsigned)pl.T), 256, 0, st>>>(part, f.blocks, picked, q->targets, f.tgt, pl.V, q->ignore_index, ll, lse);
         LVAE_LAUNCH_CHECK();
+        if (loss) {
+            few_loss_kernel<<<1, 64, 0, st>>>(q->targets, f.tgt, f.T, q->ignore_index, ll, mean, loss, each);
+            LVAE_LAUNCH_CHECK();
+        }
         return LVAE_OK;
     }
     RowsArgs rows = rows_args(q, pl, ws);
@@ -887,8 +939,21 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     a.ldp = pl.Tpad;
     a.picked = picked;
     RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow, a, st));
-    finish_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 16)), 256, 0, st>>>(part, a.tiles_m, pl.Tpad, picked, rows.tok, rows.tgt_of,
-                                                                          rows.n_rows, ll, lse);
+    FinishArgs f = {};
+    f.part = part;
+    f.tiles = a.tiles_m;
+    f.ldp = pl.Tpad;
+    f.picked = picked;
+    f.tok = rows.tok;
+    f.tgt = rows.tgt_of;
+    f.n_rows = rows.n_rows;
+    f.ll = ll;
+    f.lse = lse;
+    f.loss = loss;
+    f.each = each;
+    f.sums = (double*)(ws + pl.sums);
+    f.mean = mean;
+    finish_kernel<<<dim3((unsigned)lvae_ceil_div(pl.T, 16)), 256, 0, st>>>(f);
     LVAE_LAUNCH_CHECK();
     return LVAE_OK;
 }
@@ -1036,16 +1101,6 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         final_kernel<<<dim3((unsigned)blocks), 256, 0, st>>>(f);
         LVAE_LAUNCH_CHECK();
     }
-    return LVAE_OK;
-}
-
-extern "C" int lvae_vocab_loss_f32(const lvae_vocab_problem* q, const float* ll, int mean, float factor, float* loss, float* each,
-                                   void* stream) {
-    Plan pl = {};
-    RUN(check_problem(q, &pl));
-    LVAE_CHECK_ARG(ll && loss && each && q->targets, "ll, loss, each and targets must be non-NULL");
-    loss_kernel<<<1, 1024, 0, (hipStream_t)stream>>>(q->targets, axes_of(q, q->target_stride), pl.T, q->ignore_index, ll, mean, factor, loss, each);
-    LVAE_LAUNCH_CHECK();
     return LVAE_OK;
 }
 

@@ -116,23 +116,38 @@ def _pointers(tensors):
     return [None if t is None else t.data_ptr() for t in tensors]
 
 
-def _forward(q, want_lse):
-    """(ll, lse or None, exponents or None): [*token dimensions] float32, and what the backward of float32 operands needs
-    besides."""
+# How the log-likelihoods of the tokens are put together: as they are, summed over the last axis, or one loss
+_TOKENS, _SEQUENCES, _MEAN, _SUM = range(4)
+
+
+def _forward(q, how, for_backward):
+    """(result, what the backward needs): the latter the LSE of every token, the factor of every token in a loss, and the
+    exponents of float32 operands; each None where there is none."""
     dev = q.device
     ll = torch.empty(q.shape, dtype=torch.float32, device=dev)
-    lse = torch.empty(q.shape, dtype=torch.float32, device=dev) if want_lse else None
-    limbs = want_lse and q.T > N.VOCAB_FEW and q.c.dtype == N.DTYPES[torch.float32]
+    lse = torch.empty(q.shape, dtype=torch.float32, device=dev) if for_backward else None
+    limbs = for_backward and q.T > N.VOCAB_FEW and q.c.dtype == N.DTYPES[torch.float32]
     exponents = torch.empty(2, dtype=torch.int32, device=dev) if limbs else None
-    if q.T:
-        nbytes = N._i64(0)
+    loss = each = None
+    if how >= _MEAN:
+        new = torch.empty if q.T else torch.zeros
+        loss, each = new((), dtype=torch.float32, device=dev), new((), dtype=torch.float32, device=dev)
+    out = ll if loss is None else loss
+    if how == _SEQUENCES:
+        out = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
+    if q.T or (how == _SEQUENCES and out.numel()):
+        lib = N.lib()
         with N.on_device(q.index):
-            lib = N.lib()
-            N.check(lib.lvae_vocab_ll_workspace_bytes(q.c, nbytes))
-            ws = N.workspace(nbytes.value, dev)
-            p = _pointers((ll, lse, exponents))
-            N.check(lib.lvae_vocab_ll(q.c, p[0], p[1], p[2], ws.data_ptr(), nbytes.value, N.raw_stream(q.index)))
-    return ll, lse, exponents
+            stream = N.raw_stream(q.index)
+            if q.T:
+                nbytes = N._i64(0)
+                N.check(lib.lvae_vocab_ll_workspace_bytes(q.c, nbytes))
+                ws = N.workspace(nbytes.value, dev)
+                N.check(lib.lvae_vocab_ll(q.c, *_pointers((ll, lse, exponents, loss, each)), how == _MEAN, ws.data_ptr(),
+                                          nbytes.value, stream))
+            if how == _SEQUENCES and out.numel():
+                N.check(lib.lvae_segment_sum_f32(ll.data_ptr(), out.numel(), q.shape[-1], out.data_ptr(), stream))
+    return out, (lse, each, exponents)
 
 
 def _backward(q, tensors, needs, lse, g, g_strides, g_scale, exponents):
@@ -162,31 +177,6 @@ def _token_strides(q):
     return (b * c, c, 1)
 
 
-# How the log-likelihoods of the tokens are put together: as they are, summed over the last axis, or one loss
-_TOKENS, _SEQUENCES, _MEAN, _SUM = range(4)
-
-
-def _put_together(q, ll, how):
-    """(result, device factor of every ll in it or None)."""
-    if how == _TOKENS:
-        return ll, None
-    dev = q.device
-    if how == _SEQUENCES:
-        out = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev)
-        if out.numel():
-            with N.on_device(q.index):
-                N.check(N.lib().lvae_segment_sum_f32(ll.data_ptr(), out.numel(), q.shape[-1], out.data_ptr(),
-                                                     N.raw_stream(q.index)))
-        return out, None
-    if not q.T:
-        return torch.zeros((), device=dev), torch.zeros((), device=dev)
-    loss, each = torch.empty((), device=dev, dtype=torch.float32), torch.empty((), device=dev, dtype=torch.float32)
-    with N.on_device(q.index):
-        N.check(N.lib().lvae_vocab_loss_f32(q.c, ll.data_ptr(), how == _MEAN, -1.0, loss.data_ptr(), each.data_ptr(),
-                                            N.raw_stream(q.index)))
-    return loss, each
-
-
 class _VocabLL(torch.autograd.Function):
     """Token log-likelihoods, put together, with a HIP backward (lvae_vocab_ll_bwd): the softmax is computed again from
     the saved LSE, a piece of the vocabulary at a time."""
@@ -194,10 +184,9 @@ class _VocabLL(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, ignore_index, how):
         q = _Problem(hidden.detach(), weight.detach(), targets, None if bias is None else bias.detach(), ignore_index)
-        ll, lse, exponents = _forward(q, True)
-        out, factor = _put_together(q, ll, how)
+        out, saved = _forward(q, how, True)
         tensors, ctx.plan = q.without_tensors()
-        ctx.save_for_backward(*tensors, lse, factor, exponents)
+        ctx.save_for_backward(*tensors, *saved)
         ctx.how = how
         return out
 
@@ -224,7 +213,7 @@ def _run(hidden, weight, targets, bias, ignore_index, how):
     if _needs_grad(hidden, weight, bias):
         return _VocabLL.apply(hidden, weight, bias, targets, ignore_index, how)
     q = _Problem(hidden, weight, targets, bias, ignore_index)
-    return _put_together(q, _forward(q, False)[0], how)[0]
+    return _forward(q, how, False)[0]
 
 
 def token_log_likelihood(hidden, weight, targets, bias=None, ignore_index=-100):

@@ -48,7 +48,7 @@ def test_problem_refusals(kw, text):
     from lvae import _native as N
     lib, out = N.lib(), ctypes.c_int64(0)
     assert lib.lvae_vocab_ll_workspace_bytes(problem(**kw), out) == -1 and text in lib.lvae_last_error()
-    assert lib.lvae_vocab_ll(problem(**kw), 256, None, None, 256, 1 << 40, None) == -1
+    assert lib.lvae_vocab_ll(problem(**kw), 256, None, None, None, None, 0, 256, 1 << 40, None) == -1
     assert lib.lvae_vocab_ll_bwd(problem(**kw), 256, 256, (ctypes.c_int64 * 3)(), None, None, 256, None, None, 256, 1 << 40, None) == -1
 
 
@@ -57,17 +57,18 @@ def test_call_refusals():
     lib, out, s = N.lib(), ctypes.c_int64(0), (ctypes.c_int64 * 3)()
     assert lib.lvae_vocab_ll_workspace_bytes(None, out) == -1 and lib.lvae_vocab_ll_workspace_bytes(problem(), None) == -1
     for kw in (dict(hidden=None), dict(weight=None), dict(targets=None)):
-        assert lib.lvae_vocab_ll(problem(**kw), 256, None, None, 256, 1 << 40, None) == -1
-    assert lib.lvae_vocab_ll(problem(), None, None, None, 256, 1 << 40, None) == -1
+        assert lib.lvae_vocab_ll(problem(**kw), 256, None, None, None, None, 0, 256, 1 << 40, None) == -1
+    assert lib.lvae_vocab_ll(problem(), None, None, None, None, None, 0, 256, 1 << 40, None) == -1
     assert lib.lvae_vocab_ll_workspace_bytes(problem(), out) == 0
-    assert lib.lvae_vocab_ll(problem(), 256, None, None, None, 0, None) == -2 and b"NULL" in lib.lvae_last_error()
-    assert lib.lvae_vocab_ll(problem(), 256, None, None, 260, 1 << 40, None) == -2 and b"aligned" in lib.lvae_last_error()
-    assert lib.lvae_vocab_ll(problem(), 256, None, None, 256, out.value - 1, None) == -2 and b"too small" in lib.lvae_last_error()
+    assert lib.lvae_vocab_ll(problem(), 256, None, None, None, None, 0, None, 0, None) == -2 and b"NULL" in lib.lvae_last_error()
+    assert lib.lvae_vocab_ll(problem(), 256, None, None, None, None, 0, 260, 1 << 40, None) == -2 and b"aligned" in lib.lvae_last_error()
+    assert lib.lvae_vocab_ll(problem(), 256, None, None, None, None, 0, 256, out.value - 1, None) == -2 and b"too small" in lib.lvae_last_error()
     assert lib.lvae_vocab_ll_bwd(problem(), 256, 256, s, None, None, None, None, None, 256, 1 << 40, None) == -1
     assert b"no gradient" in lib.lvae_last_error()
     assert lib.lvae_vocab_ll_bwd(problem(), None, 256, s, None, None, 256, None, None, 256, 1 << 40, None) == -1
     assert lib.lvae_vocab_ll_bwd(problem(), 256, 256, s, None, None, 256, None, None, 256, 16, None) == -2
-    assert lib.lvae_vocab_loss_f32(problem(), None, 1, -1.0, 256, 256, None) == -1
+    assert lib.lvae_vocab_ll(problem(), 256, None, None, 256, None, 1, 256, 1 << 40, None) == -1
+    assert b"go together" in lib.lvae_last_error()
     assert lib.lvae_segment_sum_f32(None, 3, 3, 256, None) == -1 and lib.lvae_segment_sum_f32(256, 3, -1, 256, None) == -1
 
 
