@@ -17,10 +17,6 @@ int lvae_vg_launch_both_bf16(int mode_w, const VgArgs& h, const VgArgs& w, int h
 int lvae_vg_launch_both_f16(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st);
 int lvae_vg_launch_both_f32(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st);
 
-#ifndef VOCAB_G_MIB
-#define VOCAB_G_MIB 512ll
-#endif
-
 namespace {
 
 // G in 16 bits is kept relative to the largest upstream gradient: the -1 of a target is then exact (with the 1 / n of a
@@ -637,7 +633,8 @@ struct Plan {
     int64_t T, Tpad, V, Vpad, H, Kp;
     int planes;
     bool few, direct_w;
-    int narrow, tile_n;
+    int narrow, tile_n;         // of dHidden
+    int narrow_l, tile_l;       // of the logits
     int64_t piece;              // words of the vocabulary a time (backward)
     int splits_h, splits_w;
     // offsets into the workspace, bytes
@@ -668,9 +665,13 @@ int check_problem(const lvae_vocab_problem* q, Plan* pl) {
     // the tiles read W where it lies if its rows are whole 128-byte slices on 16-byte boundaries; else a padded copy
     pl->direct_w = q->dtype != LVAE_F32 && q->H % VG_BK == 0 && q->weight_stride % 8 == 0 &&
                    q->weight_stride < (1 << 22) && ((uintptr_t)q->weight & 15) == 0;
-    // 64-token tiles where 256-token ones would be mostly empty
+    // Tiles of 64 tokens, two workgroups a CU, where tiles of 256 would be mostly empty; for the logits also where there
+    // are too few of those for the 256 CUs.  Step of 2,000 tokens, 4,000 words, width 512 (128 tiles): 112 us narrow, 123
+    // wide; 200 tokens, 50,265 words, width 768 (197 tiles): 179 narrow, 164 wide.
     pl->narrow = T <= 128;
     pl->tile_n = pl->narrow ? 64 : 256;
+    pl->narrow_l = pl->narrow || pl->Vpad / 256 * lvae_ceil_div(T, 256) < 160;
+    pl->tile_l = pl->narrow_l ? 64 : 256;
     return LVAE_OK;
 }
 
@@ -717,9 +718,10 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     pl->lse = take(at, pl->Tpad * 4);
     pl->gy = take(at, pl->Tpad * 4);
     // pieces of the vocabulary: G of one piece takes at most 512 MiB, and every piece is as large as the others.  Fewer
-    // pieces mean fewer rounds of tiles that do not fill the GPU, and fewer additions to the slabs of dHidden
+    // pieces mean fewer rounds of tiles that do not fill the GPU, and fewer additions to the slabs of dHidden (16,384
+    // tokens, width 1,024, 50,265 words, bf16: 6.69 / 6.40 / 6.38 / 6.60 ms at 256 / 512 / 1,024 / 2,048 MiB)
     const int64_t per_word = pl->Tpad * pl->planes * 2;
-    int64_t piece = (VOCAB_G_MIB << 20) / per_word / 256 * 256;
+    int64_t piece = (512ll << 20) / per_word / 256 * 256;
     if (piece < 1024) piece = 1024;
     if (piece > 1 << 20) piece = 1 << 20;
     const int64_t pieces = lvae_ceil_div(pl->Vpad, piece);
@@ -732,7 +734,7 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     const int64_t ks_h = lvae_ceil_div(pl->piece, VG_BK), ks_w = lvae_ceil_div(pl->T, VG_BK);
     const int64_t share = (tiles_h * ks_h + tiles_w * ks_w) / 256 + 1;      // slices a CU, both products
     int64_t most = share * 6 / 10;
-    if (most < 16) most = 16;
+    if (most < 8) most = 8;
     pl->splits_h = (int)lvae_ceil_div(ks_h, most);
     if (pl->splits_h > 32) pl->splits_h = 32;
     // the weight gradient's sum is split only where both products together leave CUs without a tile: its slabs are as
@@ -745,7 +747,7 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     pl->slab = want_h ? take(at, pl->splits_h * pl->Tpad * pl->Kp * 4) : 0;
     pl->slab_w = want_w && pl->splits_w > 1 ? take(at, pl->splits_w * pl->piece * pl->Kp * 4) : 0;
     // column sums of all pieces for one reduction at the end, or of one piece where that would take over 256 MiB
-    const int64_t parts = pl->Tpad / pl->tile_n * (pl->narrow ? 2 : 4);
+    const int64_t parts = pl->Tpad / pl->tile_l * (pl->narrow_l ? 2 : 4);
     pl->ld_dbias = parts * pl->Vpad * 4 <= 256ll << 20 ? pl->Vpad : pl->piece;
     pl->dbias = want_b ? take(at, parts * pl->ld_dbias * 4) : 0;
     pl->bytes = at;
@@ -839,7 +841,7 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     a->N = pl.T;
     a->K = pl.Kp;
     a->n_rows = rows.n_rows;
-    a->tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_n);
+    a->tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_l);
     a->splits = 1;
     a->bias = bias;
     a->tgt = rows.tgt_of;
@@ -938,7 +940,7 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     a.part = part;
     a.ldp = pl.Tpad;
     a.picked = picked;
-    RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow, a, st));
+    RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow_l, a, st));
     FinishArgs f = {};
     f.part = part;
     f.tiles = a.tiles_m;
@@ -994,7 +996,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     RUN(launch_operands(q, pl, rows, ws, &a, st));
     const float* unscale = rows.unscale;
     const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2;
-    const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow ? 2 : 4;
+    const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow_l ? 2 : 4;
     uint16_t* gbuf = (uint16_t*)(ws + pl.g);
     VgArgs dl = a;                                       // the gradient of the logits
     dl.lse = rows.lse_of;
@@ -1015,7 +1017,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     h.N = pl.T;
     h.n_rows = rows.n_rows;
     h.tiles_m = th;
-    h.tiles_n = a.tiles_n;
+    h.tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_n);
     h.splits = pl.splits_h;
     h.slab = (float*)(ws + pl.slab);
     h.ld_slab = pl.Kp;
@@ -1044,7 +1046,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     f.ld_part = pl.ld_dbias;
     f.V = d_bias ? pl.V : 0;
     f.per_tile = waves_n;
-    f.tile_rows = pl.tile_n;
+    f.tile_rows = pl.tile_l;
     f.bias_dt = q->bias_dtype;
     f.d_bias = d_bias;
     f.n_rows = rows.n_rows;
@@ -1058,7 +1060,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         dl.bias = a.bias + v0;
         dl.v0 = v0;
         dl.dbias = d_bias ? (float*)(ws + pl.dbias) + (bias_whole ? v0 : 0) : nullptr;
-        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, dl, st));
+        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow_l, dl, st));
         if (d_bias && !bias_whole) {
             FinalArgs b = f;
             b.V = words;

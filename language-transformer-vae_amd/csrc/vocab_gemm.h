@@ -5,10 +5,17 @@
 //   dWeight d[h,v]  = sum_t H[t,h] G[t,v]      both read across their rows
 //
 // One workgroup owns a tile of TM x TN outputs and walks the summed index 64 at a time: the two operand slices
-// (TM x 64 and TN x 64, 16-bit) go from memory straight into LDS (global_load_lds, 16 bytes a lane), double buffered,
-// so the loads of the next slice fly while the matrix cores work on this one.  Nothing is ever transposed in memory:
-// an operand stored [k][m] is staged as it lies and read with ds_read_b64_tr_b16, which hands each lane four k values of
-// its own column.
+// (TM x 64 and TN x 64, 16-bit) go from memory straight into LDS (global_load_lds, 16 bytes a lane), three slices of a and
+// two of b deep, 160 KiB.  Nothing is ever transposed in memory: an operand stored [k][m] is staged as it lies and read
+// with ds_read_b64_tr_b16, which hands each lane four k values of its own column.
+//
+// What bounds it, at 16,384 tokens, width 1,024, 50,265 words, bf16 (1.69 TFLOP a product): the matrix cores are busy for
+// half of the cycles, at 2.06-2.2 GHz where 2.4 is the card's, that is, power: matrix instructions alone, on random data
+// in registers, reach 1,925 TFLOP/s (2,447 on zeros), this loop without its loads 1,620 and with everything 1,080-1,200;
+// the library's product of 8,192^3 1,253.  Logits 1.46 ms, G 1.77 ms (a tenth of it the store of G), dHidden 1.38 ms,
+// dWeight 1.50 ms.  Measured and not kept: 256 x 128 tiles, two workgroups a CU (64-byte rows: L2 delivers 26 of 55 bytes
+// a clock and CU), wave groups taking turns at LDS and matrix cores, a workgroup streaming through several tiles (no gain
+// where power bounds), four waves of 128 x 128 (registers spill), non-temporal stores of G (1.6 times the time).
 //
 // float32 operands are two fp16 limbs, x 2^e = x1 + 2^-11 x2 with x1 and x2 rounded to 11 bits each, and e such that the
 // tensor's largest magnitude is just below 2^15: good to 2^-22 of every element down to 2^-29 of the largest, and to an
@@ -16,7 +23,7 @@
 // x1 y2 + x2 y1 first, then the sums times 2^-11, then x1 y1; x2 y2, below 2^-22 of |x||y|, is left out.  With the upper
 // limb's own scale the lower one keeps its bits where a plain fp16 remainder would be subnormal (softmax values of
 // unlikely words).  Against three bf16 limbs and six products: half the matrix instructions and two thirds of the bytes
-// (4,096 tokens, width 768, 50,265 words: 1,317 us so, AFTER us with two limbs).
+// (log-likelihood of 64 sentences of up to 64 tokens, width 768, 50,265 words: 1,317 us so, 689 us with two limbs).
 //
 // Row order.  A lane of the 16x16x32 instruction ends up with rows 4g..4g+3 (g = lane / 16) of each of its eight row
 // tiles.  The rows of W that feed row tile i are chosen as m = 32 g + 4 i + r, so that a lane's 8 x 4 results are 32

@@ -409,3 +409,55 @@ def test_bias_gradient_piece_by_piece():
     tol = 2 * (H + 16) * 2 * U * 40 + 2.0 ** -20 + 8 * U * 10      # of a logit; S below 40: |h| < 5, |w| < 1.3, 16 terms of mean 0.16
     bound = mass * (2 * tol + 2.0 ** -21) + 64 * U * (mass + torch.bincount(y, minlength=V)) + U * want.abs()
     assert ((b.grad.double() - want).abs() <= bound).all()
+
+
+def test_float32_beside_much_larger_values():
+    """float32 operands are scaled by one power of two a tensor: rows far below the largest element keep their bits.  Word 0
+    holds 2^20 where the hidden states are 0, the others are 2^-10 small, 2^-30 of it: below what one fp16 limb holds
+    without subnormals.  Their logits are sums of 63 products of 2^-10 and 1, good to 2^-22 each and 2^-51 * 2^20 absolute."""
+    from lvae import decoder_ops as D
+    T, V, H = 100, 40, 64
+    g = torch.Generator().manual_seed(9)
+    h = torch.randn(T, H, generator=g)
+    h[:, 0] = 0.0
+    w = torch.randn(V, H, generator=g) * 2.0 ** -10
+    w[0] = 0.0
+    w[0, 0] = 2.0 ** 20
+    y = torch.randint(0, V, (T,), generator=g)
+    o = oracle(h, w, None, y, torch.ones(T))
+    S = (h.double().abs() @ w.double().abs().T).amax(1)
+    tol = 2 * (H * 2.0 ** -31 * 5 + (H + 16) * 2 * U * S) + 2.0 ** -20 + 8 * U * 5
+    hc, wc = h.cuda().requires_grad_(), w.cuda().requires_grad_()
+    ll = D.token_log_likelihood(hc, wc, y.cuda())
+    close(ll, o["ll"], tol, "ll")
+    (-ll.sum()).backward()
+    close(wc.grad, o["dw"], o["tol_dw"] + 2.0 ** -21 * T, "d_weight")
+    # d_hidden: column 0 sums 2^20 (softmax); the others are of the small rows alone
+    close(hc.grad[:, 0], o["dh"][:, 0], 2.0 ** 20 * 2.0 ** -18, "d_hidden, large")
+    close(hc.grad[:, 1:], o["dh"][:, 1:], 2.0 ** -10 * (V + 5) * 5 * 2.0 ** -18, "d_hidden, small")
+
+
+@pytest.mark.parametrize("T", [9, 200])
+def test_wide_rows_and_unlikely_words(T):
+    """Logits over a range of a few hundred: softmax values down to 0, no overflow; the gradient of words whose
+    probability is about 2^-40 keeps its relative accuracy in float32 (the limbs of G have a scale each)."""
+    from lvae import decoder_ops as D
+    h, w, b, y = inputs(T, 300, 128, torch.float32, ignore=0.0, scale=3.0)
+    b = b - 28.0 * (torch.arange(300) % 2)          # every other word e^-28 as likely
+    y = y - y % 2
+    o = oracle(h, w, b, y, torch.ones(T))
+    hc, wc, bc = h.cuda().requires_grad_(), w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    ll = D.token_log_likelihood(hc, wc, y.cuda(), bias=bc)
+    close(ll, o["ll"], o["tol"], "ll")
+    (-ll.sum()).backward()
+    rare = torch.arange(300) % 2 == 1
+    p = torch.exp(h.double() @ w.double().T + b.double() - o["lse"][:, None])[:, rare]
+    # p is good to 2 tol relative (2^-12 asked, the logits are of order 10 and 128 products), its limbs to 2^-22, or to
+    # 2^-51 / 2^-28 of the largest |g| = 1 absolute: 2^-50
+    bound = (p * 2.0 ** -12 + 2.0 ** -50).T @ h.double().abs() + (T + 16) * 2 * U * (p.T @ h.double().abs())
+    close(wc.grad[rare.cuda()], o["dw"][rare], bound, "d_weight of unlikely words")
+    big = b.clone()
+    big[4] = 400.0                                   # one word takes everything
+    o = oracle(h, w, big, y)
+    ll = D.token_log_likelihood(h.cuda(), w.cuda(), y.cuda(), bias=big.cuda())
+    close(ll, o["ll"], o["tol"], "ll")
