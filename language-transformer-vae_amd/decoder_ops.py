@@ -87,12 +87,12 @@ class _Problem:
             hidden, targets = hidden.contiguous(), targets.contiguous()
             axes = _common_axes(shape, (hidden.stride()[:-1], targets.stride()))
         self.tensors = (hidden, weight, targets, bias)
-        self.pointers = _pointers(self.tensors)
+        self.layout = _layout(self.tensors)
         self.device, self.index = hidden.device, index
         self.T = targets.numel()
         self.ignore_index = ignore_index
         size, (hs, ts) = axes
-        h, w, y, b = self.pointers
+        h, w, y, b = _pointers(self.tensors)
         self.c = N.VocabProblem(h, w, b, y, _Three(*size), _Three(*hs), _Three(*ts), V, w0 if V > 1 else H,
                                 int(ignore_index), H, dtype, 0 if bias is None else N.DTYPES[bias.dtype], 0)
 
@@ -102,8 +102,9 @@ class _Problem:
         return tensors, self
 
     def at(self, tensors):
-        """The plan for tensors that autograd has kept: itself, unless a hook of the saved tensors has moved them."""
-        if _pointers(tensors) == self.pointers:
+        """The plan for tensors that autograd has kept: itself, unless a hook of the saved tensors has moved them or laid
+        them out anew (even at the old address: the memory may have been free in between)."""
+        if _layout(tensors) == self.layout:
             return self
         h, w, y, b = tensors
         return _Problem(h, w, y, b, self.ignore_index)
@@ -114,6 +115,10 @@ _Three = N._i64 * 3
 
 def _pointers(tensors):
     return [None if t is None else t.data_ptr() for t in tensors]
+
+
+def _layout(tensors):
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
 
 
 # How the log-likelihoods of the tokens are put together: as they are, summed over the last axis, or one loss

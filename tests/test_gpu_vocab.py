@@ -461,3 +461,25 @@ def test_wide_rows_and_unlikely_words(T):
     o = oracle(h, w, big, y)
     ll = D.token_log_likelihood(h.cuda(), w.cuda(), y.cuda(), bias=big.cuda())
     close(ll, o["ll"], o["tol"], "ll")
+
+
+def test_saved_tensors_laid_out_anew_at_the_old_address():
+    """A hook of the saved tensors may hand back the hidden states with other strides where they were before."""
+    from lvae import decoder_ops as D
+    T, V, H = 140, 300, 64
+    h, w, b, y = inputs(T, V, H, torch.float32)
+    o = oracle(h, w, b, y, -torch.ones(T))
+    wide = torch.zeros(T, 2 * H, device="cuda")
+    wide[:, :H] = h.cuda()
+    hc = wide[:, :H].detach().requires_grad_()
+
+    def unpack(kept):
+        t, dense = kept
+        if t.dim() != 2 or t.stride(0) != 2 * H:
+            return t
+        t.as_strided((T, H), (H, 1)).copy_(dense)
+        return t.as_strided((T, H), (H, 1))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (t, t.contiguous().clone()), unpack):
+        ll = D.token_log_likelihood(hc, w.cuda(), y.cuda(), b.cuda())
+    ll.sum().backward()
+    close(hc.grad, o["dh"], o["tol_dh"], "d_hidden")
