@@ -188,15 +188,16 @@ template <int DT> __device__ __forceinline__ void list_rows(const RowsArgs& p, i
     float factor = 1.f, norm = 1.f;
     if (p.gy_of) {
         if (p.g_scale) factor = p.g_scale[0];
-        float top = 0.f;                        // the largest upstream gradient, the same in every workgroup
+        // the largest finite upstream gradient, the same in every workgroup: an infinite one spoils its own token alone
+        float top = 0.f;
         if ((p.g.stride[0] | p.g.stride[1] | p.g.stride[2]) == 0) {
-            top = fabsf(p.gy[0] * factor);
-            if (!(top >= 0.f)) top = 0.f;
+            const float a = fabsf(p.gy[0] * factor);
+            top = a < INFINITY ? a : 0.f;
         } else {
             for (int64_t u = threadIdx.x; u < p.T; u += 1024)
                 if (p.targets[at_axes(p.tgt, u)] != p.ignore) {
                     const float a = fabsf(p.gy[at_axes(p.g, u)] * factor);
-                    top = a > top ? a : top;
+                    top = a > top && a < INFINITY ? a : top;
                 }
         }
         top = wave_max(top);
@@ -205,7 +206,7 @@ template <int DT> __device__ __forceinline__ void list_rows(const RowsArgs& p, i
         __syncthreads();
         norm = redf[0];
         for (int w = 1; w < 16; ++w) norm = fmaxf(norm, redf[w]);
-        if (!(norm > 0.f) || !(norm < INFINITY)) norm = p.g_scale_to;      // nothing to keep in range: a factor of 1
+        if (!(norm > 0.f)) norm = p.g_scale_to;             // nothing to keep in range: a factor of 1
         if (blockIdx.x == 0 && threadIdx.x == 0) p.unscale[0] = norm / p.g_scale_to;
     }
     for (int64_t c = first; c < end; c += 1024) {

@@ -483,3 +483,21 @@ def test_saved_tensors_laid_out_anew_at_the_old_address():
         ll = D.token_log_likelihood(hc, w.cuda(), y.cuda(), b.cuda())
     ll.sum().backward()
     close(hc.grad, o["dh"], o["tol_dh"], "d_hidden")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_one_bad_upstream_gradient(dt, bad):
+    """It spoils its own token's gradient; the other tokens' stay what they are, small ones too."""
+    from lvae import decoder_ops as D
+    T, V, H = 140, 300, 64
+    h, w, b, y = inputs(T, V, H, DT[dt], ignore=0.0)
+    gy = torch.randn(T, generator=torch.Generator().manual_seed(1)) * 1e-5
+    gy[3] = 0.0
+    o = oracle(h, w, b, y, gy)
+    gy[3] = bad
+    hc = h.cuda().requires_grad_()
+    D.token_log_likelihood(hc, w.cuda(), y.cuda(), b.cuda()).backward(-gy.cuda())
+    others = torch.arange(T) != 3
+    close(hc.grad[others], o["dh"][others], o["tol_dh"][others], "d_hidden")
+    assert not torch.isfinite(hc.grad[3]).any()
