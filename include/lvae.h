@@ -427,7 +427,8 @@ int lvae_dev_reload_env(void);
  * latent samples of a sentence (stride 0), are passed as they lie; the last axis of hidden and of weight is contiguous.
  * A token whose target is ignore_index has ll = 0 and no gradient, whatever its hidden state holds (NaN too).  Any other
  * target outside [0, V) makes ll, and every gradient that the token takes part in, NaN.  A bias of -inf bans a word.
- * All arithmetic accumulates in float32.
+ * All arithmetic accumulates in float32.  Limits of a call: V < 2^26, H <= 65,536, fewer than 2^27 tokens, tokens x H < 2^33,
+ * tokens x V < 2^38.
  * ------------------------------------------------------------------------------------------- */
 #define LVAE_F32 0
 #define LVAE_BF16 1
@@ -458,14 +459,15 @@ int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, int3
 /* Backward: g is the upstream gradient on ll, over the token axes with strides g_stride (0: shared), times the device
  * scalar g_scale if that is given.  exponents: those of the forward, or NULL.  d_hidden [tokens, H], d_weight [V, H]
  * (contiguous, dtype) and d_bias [V] (bias_dtype) may each be NULL.  The gradient of the logits exists a piece of the
- * vocabulary at a time, in the workspace (512 MiB, or 1,024 words).  Deterministic. */
+ * vocabulary at a time, in the workspace (512 MiB, or 1,024 words), and is held relative to the largest finite |g|: with
+ * LVAE_F16 and LVAE_F32 a token whose |g| is below 2^-28 of that loses bits of its own d_hidden.  Deterministic. */
 int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* problem, int want_hidden, int want_weight, int want_bias,
                                       int64_t* out_bytes);
 int lvae_vocab_ll_bwd(const lvae_vocab_problem* problem, const float* lse, const float* g, const int64_t* g_stride,
                       const float* g_scale, const int32_t* exponents, void* d_hidden, void* d_weight, void* d_bias,
                       void* ws, int64_t ws_bytes, void* stream);
 
-/* out[i] = sum_k x[i * len + k], float64 inside; len may be 0. */
+/* out[i] = sum_k x[i * len + k], i < n < 2^26, float64 inside; len may be 0. */
 int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -647,14 +647,17 @@ int check_problem(const lvae_vocab_problem* q, Plan* pl) {
     LVAE_CHECK_ARG(q, "problem must be non-NULL");
     LVAE_CHECK_ARG(q->dtype >= LVAE_F32 && q->dtype <= LVAE_F16, "unknown dtype %d", q->dtype);
     LVAE_CHECK_ARG(q->bias_dtype >= LVAE_F32 && q->bias_dtype <= LVAE_F16, "unknown bias_dtype %d", q->bias_dtype);
-    LVAE_CHECK_ARG(q->V >= 1 && q->V < (1ll << 31) - 512 && q->H >= 1 && q->H <= 65536, "bad shape: V=%lld H=%d (1 <= H <= 65536)",
-                   (long long)q->V, q->H);
+    // the limits keep every launch below 2^32 threads
+    LVAE_CHECK_ARG(q->V >= 1 && q->V < 1ll << 26 && q->H >= 1 && q->H <= 65536,
+                   "bad shape: V=%lld H=%d (1 <= V < 2^26, 1 <= H <= 65536)", (long long)q->V, q->H);
     int64_t T = 1;
     for (int i = 0; i < 3; ++i) {
         LVAE_CHECK_ARG(q->size[i] >= 1 && q->size[i] < (1ll << 31), "bad shape: size[%d]=%lld", i, (long long)q->size[i]);
         T *= q->size[i];
-        LVAE_CHECK_ARG(T < (1ll << 31) - 512, "too many tokens");
+        LVAE_CHECK_ARG(T < 1ll << 27, "too many tokens: 2^27 or more in one call");
     }
+    LVAE_CHECK_ARG(T * q->H < 1ll << 33 && T * q->V < 1ll << 38, "too many tokens: %lld of them x H=%d >= 2^33, or x V=%lld >= 2^38",
+                   (long long)T, q->H, (long long)q->V);
     LVAE_CHECK_ARG(q->weight_stride >= q->H, "weight_stride %lld < H %d", (long long)q->weight_stride, q->H);
     pl->T = T;
     pl->Tpad = lvae_round_up(T, 256);
@@ -1108,7 +1111,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
 }
 
 extern "C" int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream) {
-    LVAE_CHECK_ARG(n >= 1 && n < (1ll << 33) && len >= 0, "bad shape: n=%lld len=%lld", (long long)n, (long long)len);
+    LVAE_CHECK_ARG(n >= 1 && n < (1ll << 26) && len >= 0, "bad shape: n=%lld len=%lld", (long long)n, (long long)len);
     LVAE_CHECK_ARG(out && (x || len == 0), "x and out must be non-NULL");
     segment_sum_kernel<<<dim3((unsigned)lvae_ceil_div(n, 4)), 256, 0, (hipStream_t)stream>>>(x, n, len, out);
     LVAE_LAUNCH_CHECK();

@@ -52,6 +52,20 @@ def test_problem_refusals(kw, text):
     assert lib.lvae_vocab_ll_bwd(problem(**kw), 256, 256, (ctypes.c_int64 * 3)(), None, None, 256, None, None, 256, 1 << 40, None) == -1
 
 
+@pytest.mark.parametrize("T,V,H,ok", [
+    (1, (1 << 26) - 1, 64, True), (1, 1 << 26, 64, False), (1 << 20, 1 << 17, 8191, True), (1 << 20, 1 << 17, 8192, False),
+    (1 << 20, (1 << 18) - 1, 64, True), (1 << 20, 1 << 18, 64, False), (1 << 26, 1024, 64, True), (1 << 27, 1024, 8, False)])
+def test_limits(T, V, H, ok):
+    """Calls whose launches would pass 2^32 threads are refused before the first."""
+    from lvae import _native as N
+    lib, out, three = N.lib(), ctypes.c_int64(0), ctypes.c_int64 * 3
+    q = problem(size=three(1, 1, T), V=V, H=H, weight_stride=H)
+    assert (lib.lvae_vocab_ll_workspace_bytes(q, out) == 0) == ok
+    assert (lib.lvae_vocab_ll_bwd_workspace_bytes(q, 1, 1, 1, out) == 0) == ok
+    assert lib.lvae_vocab_ll_bwd(q, 256, 256, three(), None, None, 256, None, None, 256, 16, None) == (-2 if ok else -1)
+    assert lib.lvae_segment_sum_f32(256, 1 << 26, 3, 256, None) == -1
+
+
 def test_call_refusals():
     from lvae import _native as N
     lib, out, s = N.lib(), ctypes.c_int64(0), (ctypes.c_int64 * 3)()
