@@ -38,6 +38,13 @@ const at::Tensor* tensor_at(PyObject* list, Py_ssize_t i, const char* name, cons
     return &t;
 }
 
+// whether elements of the tensor share memory, as those of a broadcast one do
+bool repeats(const at::Tensor& t) {
+    for (int64_t k = 0; k < t.dim(); ++k)
+        if (t.size(k) > 1 && t.stride(k) == 0) return t.numel() > 0;
+    return false;
+}
+
 // table(src, dst or None, whether they will be written) -> (table as bytes, device index, whether one requires grad, [places that need a dense copy])
 PyObject* table(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
@@ -81,18 +88,26 @@ PyObject* table(PyObject*, PyObject* args) {
                 }
                 plain = plain && (s->strides() == d->strides() || (s->is_contiguous() && d->is_contiguous()));
             }
+            if (writes && !plain && repeats(d ? *d : *s)) {
+                PyErr_Format(PyExc_RuntimeError, "%s[%zd] is broadcast: several of its elements are one place in memory", d ? "out" : "grads", i);
+                ok = false;
+                break;
+            }
             e[i].src = s->const_data_ptr();
             e[i].dst = d ? d->mutable_data_ptr() : nullptr;
             e[i].n = s->numel();
             e[i].dtype = code(s->scalar_type());
             e[i].out_dtype = d ? code(d->scalar_type()) : e[i].dtype;
-            // a graph that has saved the tensor must see that it changes
-            if (writes && !(d ? d : s)->is_inference()) (d ? d : s)->unsafeGetTensorImpl()->bump_version();
             if (!plain && e[i].n) {
                 PyObject* k = PyLong_FromSsize_t(i);
                 ok = k && PyList_Append(odd, k) == 0;
                 Py_XDECREF(k);
             }
+        }
+        // a graph that has saved one of them must see that it changes; only once all are known to be in order
+        for (Py_ssize_t i = 0; ok && writes && i < n; ++i) {
+            const at::Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(out ? dst : src, i));
+            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
         }
     } catch (...) {
         Py_DECREF(bytes);

@@ -61,15 +61,16 @@ def _as_list(tensors):
 
 def global_grad_norm(grads, norm_type=2.0):
     """Norm over all elements of all tensors, as a 0-dim float32 device tensor: the square root of the sum of squares, or
-    with ``norm_type=inf`` the largest magnitude.  NaN where there is one."""
+    with ``norm_type=inf`` the largest magnitude.  NaN where there is one.  Not differentiable."""
     return _call(_as_list(grads), None, norm_type, False, 0.0)
 
 
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """Scales all gradients by ``min(1, max_norm / (norm + 1e-6))`` and returns their norm before that.  In place; or,
     with ``out`` (one tensor of the same shape for each, of any of the types), into ``out``: 16-bit gradients clipped
-    into the float32 buffers of an optimizer are rounded once.  No element that is written may belong to two of the
-    tensors (LvaeError)."""
+    into the float32 buffers of an optimizer are rounded once.  No element that is written may belong to two dense
+    tensors, or twice to a broadcast one (LvaeError).  Strided tensors go through dense copies made before anything is
+    written, so that the column ranges of one buffer may be listed side by side."""
     if not max_norm >= 0:
         raise ValueError(f"max_norm must not be negative or NaN: {max_norm!r}")
     return _call(_as_list(grads), None if out is None else _as_list(out), norm_type, True, max_norm)

@@ -163,3 +163,31 @@ def test_refusals():
     assert G.global_grad_norm([t, t]).item() == pytest.approx(math.sqrt(200))
     G.clip_grads([t, t], 1.0, out=[torch.empty_like(t), torch.empty_like(t)])      # reading twice is no harm
     assert (t == 1).all()
+
+
+def test_broadcast_tensors():
+    """Read as often as they count; refused, before anything has changed, where they would be written."""
+    from lvae import _native as N, grad_ops as G
+    a, row = torch.randn(50, device="cuda"), torch.randn(1, 7, device="cuda")
+    wide = row.expand(5, 7)
+    n = norm64([a, wide])
+    assert abs(G.global_grad_norm([a, wide]).item() - n) <= 2 * U * n
+    outs = [torch.empty(50, device="cuda"), torch.empty(5, 7, device="cuda")]
+    G.clip_grads([a, wide], n / 2, out=outs)
+    check(outs, [a, wide], (n / 2) / (n + 1e-6), "broadcast into dense")
+    before, version = a.clone(), a._version
+    with pytest.raises(N.LvaeError, match=r"grads\[1\] is broadcast"):
+        G.clip_grads([a, wide], n / 2)
+    with pytest.raises(N.LvaeError, match=r"out\[1\] is broadcast"):
+        G.clip_grads([a, wide], n / 2, out=[a, wide])
+    assert torch.equal(a, before) and a._version == version
+
+
+def test_columns_of_one_buffer():
+    from lvae import grad_ops as G
+    buf = torch.randn(30, 90, device="cuda")
+    src, parts = buf.clone(), [buf[:, :40], buf[:, 40:41], buf[:, 41:]]
+    n = norm64([src])
+    norm = G.clip_grads(parts, n / 3)
+    assert abs(norm.item() - n) <= 2 * U * n
+    check([buf], [src], (n / 3) / (n + 1e-6), "columns")
