@@ -168,7 +168,7 @@ __device__ __forceinline__ float vg_row_sum(float v) {
 template <int WM, int WN, int NJ, int NA> constexpr int vg_lds_bytes() { return (NA * 128 * WM + 2 * 16 * NJ * WN) * VG_BK * 2; }
 
 template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
-__device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* lds) {
+__device__ __forceinline__ void vg_tile(const VgArgs& p, int tm, int tn, int64_t n0, int split, int n_kept, char* lds) {
     constexpr int W = WM * WN, MI = 8, TM = 128 * WM, TN = 16 * NJ * WN, BK = VG_BK;
     constexpr int A_BYTES = TM * BK * 2, B_BYTES = TN * BK * 2;
     constexpr int QA = A_BYTES / 1024 / W, QB = B_BYTES / 1024 / W;
@@ -178,25 +178,9 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave % WM, wn = wave / WM;
 
-    // ---- which tile.  Workgroups go round the 8 XCDs; each XCD walks a contiguous range of tiles, four row tiles
-    // wide, so that the operand slices it shares stay in its own L2.
-    const int n_kept = __builtin_amdgcn_readfirstlane(p.n_rows[0]);
-    int tm, tn, split;
-    {
-        const int per = p.tiles_m * p.tiles_n, total = per * p.splits;
-        const int each = total / 8, rest = total % 8, x = block & 7, l = block >> 3;
-        int id = x * each + min(x, rest) + l;
-        if (l >= each + (x < rest ? 1 : 0)) return;
-        split = id / per;
-        id -= split * per;
-        const int group = 4 * p.tiles_n, g = id / group, first = g * 4, wide = min(4, p.tiles_m - first);
-        tm = first + (id - g * group) % wide;
-        tn = (id - g * group) / wide;
-    }
-    const int64_t m0 = (int64_t)tm * TM, n0 = (int64_t)tn * TN;
+    const int64_t m0 = (int64_t)tm * TM;
     constexpr bool N_TOKENS = !TRB;                     // n counts tokens unless G is read across its rows
     const int64_t n_lim = N_TOKENS ? (int64_t)n_kept : p.N;
-    if (N_TOKENS && n0 >= n_lim) return;                // uniform: every wave leaves
     const int64_t k_lim = TRB ? (int64_t)n_kept : p.K;
 
     constexpr int NP = DT == LVAE_F32 ? 3 : 1;
@@ -580,10 +564,47 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, unsigned block, char* l
     }
 }
 
+// The tile of a workgroup.  Workgroups go round the 8 XCDs; each XCD walks a contiguous range of tiles, four row tiles wide,
+// so that the operand slices it shares stay in its own L2.  How many tokens count is known on the device alone: a last
+// column of tiles with at most half its tokens is multiplied at half the width, and after all others, so that its tiles
+// fill the last round (565 float32 tokens, width 768, 50,265 words, forward and backward: 905 us with whole tiles, 804 us
+// so; 1,300 bfloat16 tokens: 514 and 496 us).
+template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
+__device__ __forceinline__ void vg_run(const VgArgs& p, unsigned block, char* lds) {
+    constexpr int TN = 16 * NJ * WN;
+    const int n_kept = __builtin_amdgcn_readfirstlane(p.n_rows[0]);
+    int n_whole = p.tiles_n, n_half = 0;
+    if constexpr (!TRB) {
+        n_whole = (n_kept + TN - 1) / TN;
+        if (TN == 256 && n_kept > 0 && n_kept - (n_whole - 1) * TN <= TN / 2) {
+            --n_whole;
+            n_half = 1;
+        }
+    }
+    // whole tiles and half ones: the remainder of each goes to XCDs of its own, so that no XCD has more than its share
+    const int per = p.tiles_m * n_whole, total = per * p.splits, total_h = n_half * p.tiles_m * p.splits;
+    const int each = total / 8, rest = total % 8, each_h = total_h / 8, rest_h = total_h % 8;
+    const int x = block & 7, x_h = (x - rest) & 7, mine = each + (x < rest ? 1 : 0);
+    int l = block >> 3;
+    if (l < mine) {
+        int id = x * each + min(x, rest) + l;
+        const int split = id / per;
+        id -= split * per;
+        const int group = 4 * n_whole, g = id / group, first = g * 4, wide = min(4, p.tiles_m - first);
+        const int tm = first + (id - g * group) % wide, tn = (id - g * group) / wide;
+        vg_tile<DT, TRA, TRB, EPI, WM, WN, NJ, NA>(p, tm, tn, (int64_t)tn * TN, split, n_kept, lds);
+    } else if constexpr (!TRB && TN == 256) {
+        l -= mine;
+        if (l >= each_h + (x_h < rest_h ? 1 : 0)) return;
+        const int id = x_h * each_h + min(x_h, rest_h) + l, split = id / p.tiles_m;
+        vg_tile<DT, TRA, TRB, EPI, WM, WN, NJ / 2, NA>(p, id - split * p.tiles_m, n_whole, (int64_t)n_whole * TN, split, n_kept, lds);
+    }
+}
+
 template <int DT, bool TRA, bool TRB, int EPI, int WM, int WN, int NJ, int NA>
 __global__ __launch_bounds__(64 * WM * WN, 2) void vg_kernel(VgArgs p) {
     __shared__ __align__(1024) char lds[vg_lds_bytes<WM, WN, NJ, NA>()];
-    vg_tile<DT, TRA, TRB, EPI, WM, WN, NJ, NA>(p, blockIdx.x, lds);
+    vg_run<DT, TRA, TRB, EPI, WM, WN, NJ, NA>(p, blockIdx.x, lds);
 }
 
 // Both products of a piece's G in one launch, so that the tiles of one fill the CUs that the last round of the other
@@ -593,7 +614,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void vg_both_kernel(VgArgs h, VgAr
     __shared__ __align__(1024) char lds[vg_lds_bytes<WM, WN, NJ, NA>()];
     const unsigned b = blockIdx.x;
     if (h_first ? b < blocks_h : b >= blocks_w)
-        vg_tile<DT, true, false, VG_SLAB, WM, WN, NJ, NA>(h, h_first ? b : b - blocks_w, lds);
+        vg_run<DT, true, false, VG_SLAB, WM, WN, NJ, NA>(h, h_first ? b : b - blocks_w, lds);
     else
-        vg_tile<DT, true, true, EPI_W, WM, WN, NJ, NA>(w, h_first ? b - blocks_h : b, lds);
+        vg_run<DT, true, true, EPI_W, WM, WN, NJ, NA>(w, h_first ? b - blocks_h : b, lds);
 }
