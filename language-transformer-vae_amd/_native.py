@@ -23,9 +23,6 @@ _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
 
-# element types of the vocabulary and gradient entry points
-DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
 
 class VocabProblem(ctypes.Structure):
     """lvae_vocab_problem (include/lvae.h)."""

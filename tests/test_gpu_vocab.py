@@ -501,3 +501,74 @@ def test_one_bad_upstream_gradient(dt, bad):
     others = torch.arange(T) != 3
     close(hc.grad[others], o["dh"][others], o["tol_dh"][others], "d_hidden")
     assert not torch.isfinite(hc.grad[3]).any()
+
+
+def test_refusals_on_the_gpu():
+    from lvae import _native as N, decoder_ops as D
+    h, w, y, b = torch.zeros(70, 8).cuda(), torch.zeros(5, 8).cuda(), torch.zeros(70, dtype=torch.int64).cuda(), torch.zeros(5).cuda()
+    for f in (D.token_log_likelihood, D.vocab_cross_entropy):
+        for hh in (h, h.clone().requires_grad_()):
+            for args, error in (
+                    ((hh.half(), w, y), TypeError), ((hh, w.bfloat16(), y), TypeError), ((hh.double(), w.double(), y), TypeError),
+                    ((hh, w, y.int()), TypeError), ((hh, w, y, b.double()), TypeError), ((hh, w.tolist(), y), TypeError),
+                    ((hh, w.to_sparse(), y), TypeError),
+                    ((hh, w[:, :7], y), ValueError), ((hh, w[0], y), ValueError), ((hh[0, 0], w, y), ValueError),
+                    ((hh, w, y[:69]), ValueError), ((hh, w, y[None]), ValueError), ((hh, w, y, b[:4]), ValueError),
+                    ((hh, w, y, b[None]), ValueError), ((hh, w[:0], y), ValueError), ((hh[:, :0], w[:, :0], y), ValueError),
+                    ((hh, w, y, b, 1 << 63), OverflowError), ((hh, w, y, b, 0.5), TypeError),
+                    ((hh.cpu(), w, y), N.LvaeError), ((hh, w.cpu(), y), N.LvaeError), ((hh, w, y.cpu()), N.LvaeError),
+                    ((hh, w, y, b.cpu()), N.LvaeError)):
+                with pytest.raises(error):
+                    f(*args)
+    with pytest.raises(N.LvaeError, match="65536"):
+        D.token_log_likelihood(torch.zeros(70, 65537).cuda(), torch.zeros(5, 65537).cuda(), y)
+
+
+def test_with_autograd():
+    """Twice through a kept graph; no second derivatives; changes in place are noticed; nothing is recorded without need."""
+    from lvae import _native as N, decoder_ops as D
+    for T in (20, 150):
+        h, w, b, y = (t.cuda() for t in inputs(T, 300, 64, torch.float32))
+        hr = h.clone().requires_grad_()
+        loss = D.vocab_cross_entropy(hr, w, y, b)
+        first, = torch.autograd.grad(loss, hr, retain_graph=True)
+        again, = torch.autograd.grad(loss, hr, create_graph=True)
+        assert torch.equal(first, again)
+        with pytest.raises(N.LvaeError, match="second derivatives"):
+            again.sum().backward()
+        h2 = hr * 1.0
+        loss = D.vocab_cross_entropy(h2, w, y, b)
+        h2.mul_(2.0)
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+        with torch.no_grad():
+            assert not D.token_log_likelihood(hr, w, y, b).requires_grad
+        with torch.inference_mode():
+            D.token_log_likelihood(hr, w, y, b)
+        # a broadcast input: its gradient is the sum over the places it went to
+        one = h[:1].clone().requires_grad_()
+        D.vocab_cross_entropy(one.expand(T, 64), w, y, b, reduction="sum").backward()
+        o = oracle(h[:1].expand(T, 64).cpu(), w.cpu(), b.cpu(), y.cpu(), torch.ones(T))
+        close(one.grad, o["dh"].sum(0, keepdim=True), o["tol_dh"].sum(0, keepdim=True) + T * U * o["dh"].abs().sum(0, keepdim=True), "d_hidden")
+
+
+def test_two_at_once():
+    """Two streams with operators of their own under way at the same time, forward and backward."""
+    from lvae import decoder_ops as D
+    work = [tuple(t.cuda() for t in inputs(T, 5000, 128, torch.bfloat16, seed=T)) for T in (300, 700)]
+
+    def step(h, w, b, y):
+        ts = [t.detach().requires_grad_() for t in (h, w, b)]
+        loss = D.vocab_cross_entropy(ts[0], ts[1], y, ts[2])
+        return [loss.detach()] + list(torch.autograd.grad(loss, ts))
+    want = [step(*x) for x in work]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(5):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(step(*work[k]))
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for r in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
