@@ -257,8 +257,9 @@ template <int DT> __device__ __forceinline__ void list_rows(const RowsArgs& p, i
 
 // All operands of the products in one launch: the list of tokens and their hidden states, the bias in float32 with -inf
 // behind the vocabulary (no word beyond the last can count), and a padded copy of W where its rows do not serve as they
-// lie.
-template <int DT> __global__ __launch_bounds__(1024) void prepare_kernel(RowsArgs p) {
+// lie.  With float32, two workgroups a CU, so that those that list tokens do not keep W waiting: 64 sentences of 64 tokens,
+// width 768, 50,265 words: 83 us with one, 71 us with two; the list alone, 16 bits, gains nothing.
+template <int DT> __global__ __launch_bounds__(1024, DT == LVAE_F32 ? 8 : 4) void prepare_kernel(RowsArgs p) {
     int b = blockIdx.x, e_h = 0, e_w = 0;
     if (DT == LVAE_F32) {
         if (p.w_blocks) {
