@@ -446,25 +446,27 @@ typedef struct {
 
 /* ll, lse [size0*size1*size2] float32, contiguous; lse (0 for ignored tokens) is what the backward needs and may be
  * NULL.  Up to LVAE_VOCAB_FEW tokens the weights are streamed once past all tokens in registers; beyond, matrix-core
- * tiles (float32 as two fp16 limbs).  exponents [2] int32 on the device, or NULL: written by float32 calls of more than
- * LVAE_VOCAB_FEW tokens, the powers of two that hidden and weight are scaled by; handed to the backward of the same
- * inputs they save it a read of weight.  loss, each [1] float32 on the device, or both NULL: loss = -sum(ll), with
+ * tiles (float32 as two fp16 limbs).  kept: lvae_vocab_ll_kept_bytes of device memory, 256-byte aligned, or NULL; float32
+ * calls of more than LVAE_VOCAB_FEW tokens (else the size is 0, and kept has to be NULL) leave weight in it as limbs, with
+ * the powers of two that hidden and weight are scaled by; handed to the backward of the same inputs, unchanged, that saves
+ * it two reads and a write of weight.  With kept, either call needs kept_bytes - 256 bytes less workspace.  loss, each [1] float32 on the device, or both NULL: loss = -sum(ll), with
  * mean != 0 over max(1, tokens whose target is not ignore_index); each, the factor of each ll in it (the g_scale of the
  * backward). */
 #define LVAE_VOCAB_FEW 64
 int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* problem, int64_t* out_bytes);
-int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, int32_t* exponents, float* loss, float* each,
+int lvae_vocab_ll_kept_bytes(const lvae_vocab_problem* problem, int64_t* out_bytes);
+int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, void* kept, float* loss, float* each,
                   int mean, void* ws, int64_t ws_bytes, void* stream);
 
 /* Backward: g is the upstream gradient on ll, over the token axes with strides g_stride (0: shared), times the device
- * scalar g_scale if that is given.  exponents: those of the forward, or NULL.  d_hidden [tokens, H], d_weight [V, H]
+ * scalar g_scale if that is given.  kept: that of the forward, or NULL.  d_hidden [tokens, H], d_weight [V, H]
  * (contiguous, dtype) and d_bias [V] (bias_dtype) may each be NULL.  The gradient of the logits exists a piece of the
  * vocabulary at a time, in the workspace (512 MiB, or 1,024 words), and is held relative to the largest finite |g|: with
  * LVAE_F16 and LVAE_F32 a token whose |g| is below 2^-28 of that loses bits of its own d_hidden.  Deterministic. */
 int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* problem, int want_hidden, int want_weight, int want_bias,
                                       int64_t* out_bytes);
 int lvae_vocab_ll_bwd(const lvae_vocab_problem* problem, const float* lse, const float* g, const int64_t* g_stride,
-                      const float* g_scale, const int32_t* exponents, void* d_hidden, void* d_weight, void* d_bias,
+                      const float* g_scale, const void* kept, void* d_hidden, void* d_weight, void* d_bias,
                       void* ws, int64_t ws_bytes, void* stream);
 
 /* out[i] = sum_k x[i * len + k], i < n < 2^26, float64 inside; len may be 0. */

@@ -119,6 +119,7 @@ _SIGNATURES = {
     "lvae_kernel_matrix_f32": (_int, [_c_f32p, _c_f32p, _i64, _i64, _int, ctypes.POINTER(_f32), _int, _f32,
                                       _c_f32p, ctypes.c_void_p, _i64, ctypes.c_void_p]),
     "lvae_vocab_ll_workspace_bytes": (_int, [ctypes.POINTER(VocabProblem), ctypes.POINTER(_i64)]),
+    "lvae_vocab_ll_kept_bytes": (_int, [ctypes.POINTER(VocabProblem), ctypes.POINTER(_i64)]),
     "lvae_vocab_ll": (_int, [ctypes.POINTER(VocabProblem), _c_f32p, _c_f32p, ctypes.c_void_p, _c_f32p, _c_f32p, _int,
                              ctypes.c_void_p, _i64, ctypes.c_void_p]),
     "lvae_vocab_ll_bwd_workspace_bytes": (_int, [ctypes.POINTER(VocabProblem), _int, _int, _int, ctypes.POINTER(_i64)]),
@@ -135,7 +136,6 @@ _SIGNATURES = {
 }
 
 NOALLOC_SCRATCH_BYTES = 64 << 20
-VOCAB_FEW = 64                # lvae_vocab_ll streams the weights once up to so many tokens
 REDUCE_WS_BYTES = 8192
 KMAT_WS_BYTES = 4096
 

@@ -18,6 +18,7 @@ namespace {
 
 struct Library {
     decltype(&lvae_vocab_ll_workspace_bytes) ll_bytes;
+    decltype(&lvae_vocab_ll_kept_bytes) kept_bytes;
     decltype(&lvae_vocab_ll) ll;
     decltype(&lvae_vocab_ll_bwd_workspace_bytes) bwd_bytes;
     decltype(&lvae_vocab_ll_bwd) bwd;
@@ -167,22 +168,25 @@ PyObject* wrap(const at::Tensor& t) {
 }
 at::Tensor unwrap(PyObject* o) { return o == Py_None ? at::Tensor() : THPVariable_Unpack(o); }
 
-// forward(hidden, weight, targets, bias, ignore_index, how, for_backward, few) -> result, or with for_backward
-// (result, hidden, weight, targets, bias as they are read, LSE of every token, factor of every token in a loss, exponents)
+// forward(hidden, weight, targets, bias, ignore_index, how, for_backward) -> result, or with for_backward
+// (result, hidden, weight, targets, bias as they are read, LSE of every token, factor of every token in a loss, what is kept of
+// the weights)
 PyObject* forward(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
     PyObject *hidden, *weight, *targets, *bias;
     long long ignore_index;
-    int how, for_backward, few;
-    if (!PyArg_ParseTuple(args, "OOOOLipi", &hidden, &weight, &targets, &bias, &ignore_index, &how, &for_backward, &few)) return nullptr;
+    int how, for_backward;
+    if (!PyArg_ParseTuple(args, "OOOOLip", &hidden, &weight, &targets, &bias, &ignore_index, &how, &for_backward)) return nullptr;
     Problem q;
     prepare(q, hidden, weight, targets, bias, ignore_index);
     const c10::DeviceGuard guard(q.device);
     const at::Tensor ll = q.empty(q.shape, at::kFloat);
-    at::Tensor lse, exponents, loss, each, out = ll;
+    at::Tensor lse, kept, loss, each, out = ll;
+    int64_t kept_bytes = 0;
     if (for_backward) {
         lse = q.empty(q.shape, at::kFloat);
-        if (q.tokens > few && q.c.dtype == LVAE_F32) exponents = q.empty({2}, at::kInt);
+        if (q.tokens) check(lib.kept_bytes(&q.c, &kept_bytes));
+        if (kept_bytes) kept = q.empty({kept_bytes}, at::kByte);
     }
     if (how >= MEAN) {
         const at::TensorOptions o = at::TensorOptions(q.device).dtype(at::kFloat);
@@ -194,9 +198,10 @@ PyObject* forward(PyObject*, PyObject* args) {
     if (q.tokens) {
         int64_t bytes = 0;
         check(lib.ll_bytes(&q.c, &bytes));
+        if (kept_bytes) bytes -= kept_bytes - 256;
         const at::Tensor ws = q.empty({bytes}, at::kByte);
         check(without_gil([&] {
-            return lib.ll(&q.c, (float*)data(ll), (float*)data(lse), (int32_t*)data(exponents), (float*)data(loss), (float*)data(each),
+            return lib.ll(&q.c, (float*)data(ll), (float*)data(lse), data(kept), (float*)data(loss), (float*)data(each),
                           how == MEAN, data(ws), bytes, q.stream);
         }));
     }
@@ -204,25 +209,25 @@ PyObject* forward(PyObject*, PyObject* args) {
         check(without_gil([&] { return lib.segment_sum((const float*)data(ll), out.numel(), q.shape.back(), (float*)data(out), q.stream); }));
     if (!for_backward) return wrap(out);
     return Py_BuildValue("NNNNNNNN", wrap(out), wrap(q.hidden), wrap(q.weight), wrap(q.targets), wrap(q.bias), wrap(lse), wrap(each),
-                         wrap(exponents));
+                         wrap(kept));
     END_HANDLE_TH_ERRORS
 }
 
-// backward(hidden, weight, targets, bias, ignore_index, how, lse, each, exponents, g, three truth values) -> gradients of
+// backward(hidden, weight, targets, bias, ignore_index, how, lse, each, kept, g, three truth values) -> gradients of
 // hidden, weight and bias, None where not wanted
 PyObject* backward(PyObject*, PyObject* args) {
     HANDLE_TH_ERRORS
-    PyObject *hidden, *weight, *targets, *bias, *lse_, *each_, *exponents_, *g_;
+    PyObject *hidden, *weight, *targets, *bias, *lse_, *each_, *kept_, *g_;
     long long ignore_index;
     int how, want_h, want_w, want_b;
-    if (!PyArg_ParseTuple(args, "OOOOLiOOOOppp", &hidden, &weight, &targets, &bias, &ignore_index, &how, &lse_, &each_, &exponents_, &g_,
+    if (!PyArg_ParseTuple(args, "OOOOLiOOOOppp", &hidden, &weight, &targets, &bias, &ignore_index, &how, &lse_, &each_, &kept_, &g_,
                           &want_h, &want_w, &want_b))
         return nullptr;
     // planned anew: a hook of the saved tensors may have moved them or laid them out in another way
     Problem q;
     prepare(q, hidden, weight, targets, bias, ignore_index);
     const c10::DeviceGuard guard(q.device);
-    at::Tensor lse = unwrap(lse_).contiguous(), each = unwrap(each_), exponents = unwrap(exponents_), g = unwrap(g_);
+    at::Tensor lse = unwrap(lse_).contiguous(), each = unwrap(each_), kept = unwrap(kept_), g = unwrap(g_);
     if (g.scalar_type() != at::kFloat) g = g.to(at::kFloat);
     int64_t g_stride[3] = {0, 0, 0};
     if (how < MEAN) {
@@ -239,10 +244,11 @@ PyObject* backward(PyObject*, PyObject* args) {
     if (q.tokens) {
         int64_t bytes = 0;
         check(lib.bwd_bytes(&q.c, want_h, want_w, want_b, &bytes));
+        if (kept.defined()) bytes -= kept.numel() - 256;
         const at::Tensor ws = q.empty({bytes}, at::kByte);
         check(without_gil([&] {
             return lib.bwd(&q.c, (const float*)data(lse), (const float*)data(g), g_stride, (const float*)data(each),
-                           (const int32_t*)data(exponents), data(d_h), data(d_w), data(d_b), data(ws), bytes, q.stream);
+                           data(kept), data(d_h), data(d_w), data(d_b), data(ws), bytes, q.stream);
         }));
     } else {
         if (want_w) d_w.zero_();
@@ -279,17 +285,18 @@ PyObject* py_common_axes(PyObject*, PyObject* args) {
 
 // bind([addresses of the entry points, in the order of Library], exception class, device index -> stream handle)
 PyObject* bind(PyObject*, PyObject* args) {
-    unsigned long long a[6];
+    unsigned long long a[7];
     PyObject *error, *raw_stream;
-    if (!PyArg_ParseTuple(args, "(KKKKKK)OO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &error, &raw_stream)) return nullptr;
+    if (!PyArg_ParseTuple(args, "(KKKKKKK)OO", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &error, &raw_stream)) return nullptr;
     Py_INCREF(error);
     Py_INCREF(raw_stream);
     lib.ll_bytes = (decltype(lib.ll_bytes))a[0];
-    lib.ll = (decltype(lib.ll))a[1];
-    lib.bwd_bytes = (decltype(lib.bwd_bytes))a[2];
-    lib.bwd = (decltype(lib.bwd))a[3];
-    lib.segment_sum = (decltype(lib.segment_sum))a[4];
-    lib.last_error = (decltype(lib.last_error))a[5];
+    lib.kept_bytes = (decltype(lib.kept_bytes))a[1];
+    lib.ll = (decltype(lib.ll))a[2];
+    lib.bwd_bytes = (decltype(lib.bwd_bytes))a[3];
+    lib.bwd = (decltype(lib.bwd))a[4];
+    lib.segment_sum = (decltype(lib.segment_sum))a[5];
+    lib.last_error = (decltype(lib.last_error))a[6];
     Py_XDECREF(lib.error);
     Py_XDECREF(lib.raw_stream);
     lib.error = error;
@@ -298,8 +305,8 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "bind(entry points, exception class, stream of a device)"},
-                         {"forward", forward, METH_VARARGS, "forward(hidden, weight, targets, bias, ignore_index, how, for_backward, few)"},
-                         {"backward", backward, METH_VARARGS, "backward(hidden, weight, targets, bias, ignore_index, how, lse, each, exponents, g, wanted...)"},
+                         {"forward", forward, METH_VARARGS, "forward(hidden, weight, targets, bias, ignore_index, how, for_backward)"},
+                         {"backward", backward, METH_VARARGS, "backward(hidden, weight, targets, bias, ignore_index, how, lse, each, kept, g, wanted...)"},
                          {"common_axes", py_common_axes, METH_VARARGS, "common_axes(shape, [strides of each tensor])"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -22,6 +22,7 @@ namespace {
 // G in 16 bits is kept relative to the largest upstream gradient: the -1 of a target is then exact (with the 1 / n of a
 // mean inside, all targets would share one rounding error), and fp16, with the largest at 2^14, holds what is 2^-28 of it
 constexpr float F16_G_SCALE = 16384.f;       // also of the limbs of float32
+constexpr int64_t KEPT_HEAD = 256;
 constexpr int MAX_PARTS = 512;              // workgroups that look for the largest magnitude of W, and of H
 
 struct Axes {
@@ -641,6 +642,7 @@ struct Plan {
     int splits_h, splits_w;
     // offsets into the workspace, bytes
     int64_t tok, tgt, inv, lse, gy, head, largest, bias, hpack, wpack, part, picked, sums, g, slab, slab_w, dbias, bytes;
+    int64_t kept, planes_bytes; // what a forward of float32 leaves for its backward: exponents, and W as limbs from KEPT_HEAD on
     int64_t few_blocks, ld_dbias;
 };
 
@@ -670,6 +672,8 @@ int check_problem(const lvae_vocab_problem* q, Plan* pl) {
     // the tiles read W where it lies if its rows are whole 128-byte slices on 16-byte boundaries; else a padded copy
     pl->direct_w = q->dtype != LVAE_F32 && q->H % VG_BK == 0 && q->weight_stride % 8 == 0 &&
                    q->weight_stride < (1 << 22) && ((uintptr_t)q->weight & 15) == 0;
+    pl->planes_bytes = lvae_round_up(pl->planes * pl->V * pl->Kp * 2, 256);
+    pl->kept = q->dtype == LVAE_F32 && T > LVAE_VOCAB_FEW ? KEPT_HEAD + pl->planes_bytes : 0;
     // Tiles of 64 tokens, two workgroups a CU, where tiles of 256 would be mostly empty; for the logits also where there
     // are too few of those for the 256 CUs.  Step of 2,000 tokens, 4,000 words, width 512 (128 tiles): 112 us narrow, 123
     // wide; 200 tokens, 50,265 words, width 768 (197 tiles): 179 narrow, 164 wide.
@@ -694,7 +698,12 @@ void plan_common(Plan* pl) {
     pl->tgt = take(at, pl->Tpad * 4);
     pl->bias = take(at, pl->Vpad * 4);
     pl->hpack = take(at, pl->planes * pl->Tpad * pl->Kp * 2);
-    pl->wpack = pl->direct_w ? 0 : take(at, pl->planes * pl->V * pl->Kp * 2);
+    pl->bytes = at;
+}
+// the last of the workspace, and not in it with `kept`
+void plan_weight(Plan* pl) {
+    int64_t at = pl->bytes;
+    pl->wpack = pl->direct_w ? 0 : take(at, pl->planes_bytes);
     pl->bytes = at;
 }
 
@@ -714,6 +723,7 @@ void plan_forward(Plan* pl) {
     pl->picked = take(at, pl->Tpad * 4);
     pl->sums = take(at, pl->Tpad / 16 * 8);
     pl->bytes = at;
+    plan_weight(pl);
 }
 
 void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
@@ -756,6 +766,7 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     pl->ld_dbias = parts * pl->Vpad * 4 <= 256ll << 20 ? pl->Vpad : pl->piece;
     pl->dbias = want_b ? take(at, parts * pl->ld_dbias * 4) : 0;
     pl->bytes = at;
+    plan_weight(pl);
 }
 
 Axes axes_of(const lvae_vocab_problem* q, const int64_t* stride) {
@@ -767,7 +778,10 @@ Axes axes_of(const lvae_vocab_problem* q, const int64_t* stride) {
     return a;
 }
 
-int check_ws(const Plan& pl, void* ws, int64_t ws_bytes) {
+int check_ws(Plan& pl, const void* kept, void* ws, int64_t ws_bytes) {
+    LVAE_CHECK_ARG(!kept || pl.kept, "nothing is kept of this problem: kept must be NULL");
+    LVAE_CHECK_ARG(((uintptr_t)kept & 255) == 0, "kept must be 256-byte aligned");
+    if (kept) pl.bytes -= pl.planes_bytes;
     if (!ws) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace is NULL (%lld bytes needed)", (long long)pl.bytes);
     if ((uintptr_t)ws & 255) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace must be 256-byte aligned");
     if (ws_bytes < pl.bytes)
@@ -797,9 +811,9 @@ int launch_both(int dtype, int mode_w, const VgArgs& h, const VgArgs& w, int h_f
 }
 
 // rows, bias, W and hidden as the products read them; fills the operands of the logits' product
-int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows, char* ws, VgArgs* a, hipStream_t st) {
+int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows, char* kept, char* ws, VgArgs* a, hipStream_t st) {
     uint16_t* hp = (uint16_t*)(ws + pl.hpack);
-    uint16_t* wp = pl.direct_w ? nullptr : (uint16_t*)(ws + pl.wpack);
+    uint16_t* wp = pl.direct_w ? nullptr : (uint16_t*)(kept ? kept + KEPT_HEAD : ws + pl.wpack);
     float* bias = (float*)(ws + pl.bias);
     rows.tokens = lvae_round_up(lvae_ceil_div(pl.T, 512), 16);
     rows.hpack = hp;
@@ -817,8 +831,8 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     rows.Kp = (int)pl.Kp;
     rows.hidden = q->hidden;
     rows.largest = (float*)(ws + pl.largest);
-    const bool known = rows.exponents && rows.lse_of;        // a backward that got those of its forward
-    if (!rows.exponents) rows.exponents = (int*)(ws + pl.head + 128);
+    const bool known = kept && rows.lse_of;                  // a backward that got what its forward has left
+    rows.exponents = (int*)(kept ? kept : ws + pl.head + 128);
     if (q->dtype == LVAE_F32 && !known) {
         rows.h_blocks = (int)lvae_ceil_div(pl.T, 16);
         rows.w_blocks = (int)lvae_ceil_div(pl.V, 16);
@@ -827,7 +841,7 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
         largest_kernel<<<dim3((unsigned)(rows.h_blocks + rows.w_blocks)), 1024, 0, st>>>(rows);
         LVAE_LAUNCH_CHECK();
     }
-    const dim3 grid((unsigned)(rows.row_blocks + rows.bias_blocks + (wp ? lvae_ceil_div(pl.V, 16) : 0)));
+    const dim3 grid((unsigned)(rows.row_blocks + rows.bias_blocks + (wp && !known ? lvae_ceil_div(pl.V, 16) : 0)));
     if (q->dtype == LVAE_F32) prepare_kernel<LVAE_F32><<<grid, 1024, 0, st>>>(rows);
     else prepare_kernel<LVAE_BF16><<<grid, 1024, 0, st>>>(rows);       // 16 bits are 16 bits
     LVAE_LAUNCH_CHECK();
@@ -890,7 +904,15 @@ extern "C" int lvae_vocab_ll_workspace_bytes(const lvae_vocab_problem* q, int64_
     return LVAE_OK;
 }
 
-extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, int32_t* exponents, float* loss, float* each,
+extern "C" int lvae_vocab_ll_kept_bytes(const lvae_vocab_problem* q, int64_t* out_bytes) {
+    Plan pl = {};
+    LVAE_CHECK_ARG(out_bytes, "out_bytes must be non-NULL");
+    RUN(check_problem(q, &pl));
+    *out_bytes = pl.kept;
+    return LVAE_OK;
+}
+
+extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse, void* kept, float* loss, float* each,
                              int mean, void* wsv, int64_t ws_bytes, void* stream) {
     Plan pl = {};
     RUN(check_problem(q, &pl));
@@ -898,7 +920,7 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     LVAE_CHECK_ARG(ll, "ll must be non-NULL");
     LVAE_CHECK_ARG(!loss == !each, "loss and each go together");
     plan_forward(&pl);
-    RUN(check_ws(pl, wsv, ws_bytes));
+    RUN(check_ws(pl, kept, wsv, ws_bytes));
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)wsv;
     float2* part = (float2*)(ws + pl.part);
@@ -937,9 +959,8 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     RowsArgs rows = rows_args(q, pl, ws);
     rows.ll = ll;
     rows.lse_out = lse;
-    rows.exponents = exponents;
     VgArgs a;
-    RUN(launch_operands(q, pl, rows, ws, &a, st));
+    RUN(launch_operands(q, pl, rows, (char*)kept, ws, &a, st));
     a.M = pl.V;
     a.tiles_m = (int)(pl.Vpad / 256);
     a.part = part;
@@ -976,7 +997,7 @@ extern "C" int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* q, in
 }
 
 extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, const float* g, const int64_t* g_stride,
-                                 const float* g_scale, const int32_t* exponents, void* d_hidden, void* d_weight,
+                                 const float* g_scale, const void* kept, void* d_hidden, void* d_weight,
                                  void* d_bias, void* wsv, int64_t ws_bytes, void* stream) {
     Plan pl = {};
     RUN(check_problem(q, &pl));
@@ -984,7 +1005,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     LVAE_CHECK_ARG(lse && g && g_stride, "lse, g and g_stride must be non-NULL");
     LVAE_CHECK_ARG(d_hidden || d_weight || d_bias, "no gradient asked for");
     plan_backward(&pl, d_hidden != nullptr, d_weight != nullptr, d_bias != nullptr);
-    RUN(check_ws(pl, wsv, ws_bytes));
+    RUN(check_ws(pl, kept, wsv, ws_bytes));
     hipStream_t st = (hipStream_t)stream;
     char* ws = (char*)wsv;
     RowsArgs rows = rows_args(q, pl, ws);
@@ -996,9 +1017,8 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     rows.inv = (int*)(ws + pl.inv);
     rows.lse_of = (float*)(ws + pl.lse);
     rows.gy_of = (float*)(ws + pl.gy);
-    rows.exponents = const_cast<int32_t*>(exponents);     // read only: w_blocks stays 0
     VgArgs a;
-    RUN(launch_operands(q, pl, rows, ws, &a, st));
+    RUN(launch_operands(q, pl, rows, (char*)const_cast<void*>(kept), ws, &a, st)       /* read only there */);
     const float* unscale = rows.unscale;
     const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2;
     const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow_l ? 2 : 4;

@@ -37,8 +37,9 @@ def _calls():
     if _bound is not lib:
         if _decoder_calls is None:
             raise N.LvaeError("_decoder_calls.so is missing: build it with `make -C csrc` (there is no Python fallback)")
-        entry_points = (lib.lvae_vocab_ll_workspace_bytes, lib.lvae_vocab_ll, lib.lvae_vocab_ll_bwd_workspace_bytes,
-                        lib.lvae_vocab_ll_bwd, lib.lvae_segment_sum_f32, lib.lvae_last_error)
+        entry_points = (lib.lvae_vocab_ll_workspace_bytes, lib.lvae_vocab_ll_kept_bytes, lib.lvae_vocab_ll,
+                        lib.lvae_vocab_ll_bwd_workspace_bytes, lib.lvae_vocab_ll_bwd, lib.lvae_segment_sum_f32,
+                        lib.lvae_last_error)
         _decoder_calls.bind(tuple(ctypes.cast(f, ctypes.c_void_p).value for f in entry_points), N.LvaeError, N.raw_stream)
         _bound = lib
     return _decoder_calls
@@ -59,18 +60,18 @@ class _VocabLL(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, bias, targets, ignore_index, how):
-        out, *saved = _calls().forward(hidden, weight, targets, bias, ignore_index, how, True, N.VOCAB_FEW)
+        out, *saved = _calls().forward(hidden, weight, targets, bias, ignore_index, how, True)
         ctx.save_for_backward(*saved)
         ctx.how, ctx.ignore_index = how, ignore_index
         return out
 
     @staticmethod
     def backward(ctx, g):
-        hidden, weight, targets, bias, lse, each, exponents = ctx.saved_tensors
+        hidden, weight, targets, bias, lse, each, kept = ctx.saved_tensors
         needs = ctx.needs_input_grad[:3]
         if not any(needs):
             return None, None, None, None, None, None
-        grads = _calls().backward(hidden, weight, targets, bias, ctx.ignore_index, ctx.how, lse, each, exponents, g, *needs)
+        grads = _calls().backward(hidden, weight, targets, bias, ctx.ignore_index, ctx.how, lse, each, kept, g, *needs)
         if torch.is_grad_enabled():                       # create_graph
             grads = (None if t is None else _Once.apply(t, hidden, weight, bias, g) for t in grads)
         return (*grads, None, None, None)
@@ -91,7 +92,7 @@ class _Once(torch.autograd.Function):
 def _run(hidden, weight, targets, bias, ignore_index, how):
     if _needs_grad(hidden, weight, bias):
         return _VocabLL.apply(hidden, weight, bias, targets, ignore_index, how)
-    return _calls().forward(hidden, weight, targets, bias, ignore_index, how, False, N.VOCAB_FEW)
+    return _calls().forward(hidden, weight, targets, bias, ignore_index, how, False)
 
 
 def token_log_likelihood(hidden, weight, targets, bias=None, ignore_index=-100):

@@ -572,3 +572,30 @@ def test_two_at_once():
     for k in (0, 1):
         for r in got[k]:
             assert all(torch.equal(a, b) for a, b in zip(r, want[k]))
+
+
+@pytest.mark.parametrize("T", [40, 150])
+def test_backward_without_what_the_forward_kept(T):
+    """Through the C entry points: the backward makes the limbs itself, to the same bits."""
+    import ctypes
+    from lvae import _native as N, decoder_ops as D
+    V, H = 1000, 72
+    h, w, b, y = (t.cuda() for t in inputs(T, V, H, torch.float32))
+    ts = [t.clone().requires_grad_() for t in (h, w, b)]
+    want = torch.autograd.grad(D.vocab_cross_entropy(ts[0], ts[1], y, ts[2], reduction="sum"), ts)
+    three, lib, n = ctypes.c_int64 * 3, N.lib(), ctypes.c_int64(0)
+    q = N.VocabProblem(h.data_ptr(), w.data_ptr(), b.data_ptr(), y.data_ptr(), three(1, 1, T), three(0, 0, H), three(0, 0, 1), V, H,
+                       -100, H, 0, 0, 0)
+    stream = N.raw_stream(0)
+    N.check(lib.lvae_vocab_ll_workspace_bytes(q, n))
+    ws = N.workspace(n.value, h.device)
+    ll, lse = torch.empty(T, device="cuda"), torch.empty(T, device="cuda")
+    N.check(lib.lvae_vocab_ll(q, ll.data_ptr(), lse.data_ptr(), None, None, None, 0, ws.data_ptr(), n.value, stream))
+    N.check(lib.lvae_vocab_ll_bwd_workspace_bytes(q, 1, 1, 1, n))
+    ws = N.workspace(n.value, h.device)
+    got, g = [torch.empty_like(t) for t in (h, w, b)], torch.full((1,), -1.0, device="cuda")
+    N.check(lib.lvae_vocab_ll_bwd(q, lse.data_ptr(), g.data_ptr(), three(0, 0, 0), None, None, *[t.data_ptr() for t in got],
+                                  ws.data_ptr(), n.value, stream))
+    assert torch.equal(ll, D.token_log_likelihood(h, w, y, b))
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)

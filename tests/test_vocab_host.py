@@ -86,6 +86,26 @@ def test_call_refusals():
     assert lib.lvae_segment_sum_f32(None, 3, 3, 256, None) == -1 and lib.lvae_segment_sum_f32(256, 3, -1, 256, None) == -1
 
 
+def test_what_a_forward_keeps():
+    """float32 tiles keep their exponents and W as two planes of 16 bits, which then need no workspace; nothing else does."""
+    from lvae import _native as N
+    lib, out, three = N.lib(), ctypes.c_int64(0), ctypes.c_int64 * 3
+    for kw, kept in ((dict(dtype=0), 256 + 1000 * 64 * 4), (dict(dtype=0, H=65, weight_stride=70), 256 + 1000 * 128 * 4),
+                     (dict(dtype=0, size=three(1, 8, 8)), 0), (dict(dtype=1), 0), (dict(dtype=2, H=63), 0)):
+        assert lib.lvae_vocab_ll_kept_bytes(problem(**kw), out) == 0 and out.value == kept, kw
+        assert lib.lvae_vocab_ll_workspace_bytes(problem(**kw), out) == 0
+        need = out.value - (kept - 256 if kept else 0)
+        rc = lib.lvae_vocab_ll(problem(**kw), 256, None, 256, None, None, 0, 256, need - 1, None)
+        assert rc == (-2 if kept else -1) and (b"too small" if kept else b"nothing is kept") in lib.lvae_last_error()
+        assert lib.lvae_vocab_ll_bwd_workspace_bytes(problem(**kw), 1, 1, 1, out) == 0
+        need = out.value - (kept - 256 if kept else 0)
+        rc = lib.lvae_vocab_ll_bwd(problem(**kw), 256, 256, three(), None, 256, 256, 256, 256, 256, need - 1, None)
+        assert rc == (-2 if kept else -1) and (b"too small" if kept else b"nothing is kept") in lib.lvae_last_error()
+    assert lib.lvae_vocab_ll(problem(dtype=0), 256, None, 260, None, None, 0, 256, 1 << 40, None) == -1
+    assert b"kept must be 256-byte aligned" in lib.lvae_last_error()
+    assert lib.lvae_vocab_ll_kept_bytes(problem(), None) == -1 and lib.lvae_vocab_ll_kept_bytes(problem(V=0), out) == -1
+
+
 def entries(*rows):
     flat = (ctypes.c_int64 * (4 * len(rows)))()
     for i, (src, dst, n, dt, ot) in enumerate(rows):
