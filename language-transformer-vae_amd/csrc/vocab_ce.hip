@@ -363,10 +363,15 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishArgs p) {
 
 // ---- few tokens: W streamed once -------------------------------------------------------------------------------
 // A wave owns 16 words, whose rows come from memory into registers as they lie in the instruction's operand (a lane reads
-// 32 consecutive bytes of its word's row: 128 bytes a row and step), four steps ahead of their use.  The tokens' rows go
-// through LDS, four steps at a time, shared by the four waves: read from memory by every wave they cost more accesses of
-// the first-level cache than W (24 float32 tokens: 66 us so, 48 us through LDS).  The order of the summed index inside
-// a step is the lanes' own, the same on both sides.  Bound by the read of W.
+// 32 consecutive bytes of its word's row: 128 bytes a row and step), a round of steps ahead of their use.  The tokens' rows
+// go through LDS a round at a time, shared by eight waves.  The order of the summed index inside a step is the lanes' own,
+// the same on both sides.  Bound by the read of W (width 768, 50,265 words, one token: 4.1 TB/s, with the launch that joins
+// the parts 22 us in bfloat16, 42 in float32); beyond 32 float32 tokens by the float32 matrix instructions.  Measured, a
+// call: 24 float32 tokens with the tokens read from memory by every wave 66 us, through LDS shared by four waves 51, by
+// eight 47, by sixteen 47; 64 bfloat16 tokens by four 34, by eight 30.  Rounds of two steps serve more than 16 float32
+// tokens and more than 32 others (24 float32: 47 us, 49 with four steps; 64: 69 and 72; 64 bfloat16: 30 both, without
+// spilling), of four everything else (one bfloat16 token: 22.4 us, 22.7 with two); loads two rounds ahead gain nothing.
+constexpr int FEW_WAVES = 8;
 template <int DT> struct FewStep {
     static constexpr int K = DT == LVAE_F32 ? 32 : 64, LANE = K / 4;       // elements a step, and a lane's share
 };
@@ -378,8 +383,9 @@ template <int DT, bool ALIGNED> __device__ __forceinline__ void few_load(const v
         const int at = k + h * E;
         out[h] = f32x4{0.f, 0.f, 0.f, 0.f};
         if constexpr (ALIGNED) {
-            // behind H the row's first piece is read and dropped: no branch, so that the loads of a step go out together
-            const f32x4 v = *(const f32x4*)((const char*)row + (at < H ? at : 0) * SZ);
+            // behind H the row's last piece is read again and dropped: no branch, so that loads go out together and the
+            // compiler knows how many are in flight
+            const f32x4 v = *(const f32x4*)((const char*)row + min(at, H - E) * SZ);
             out[h] = at < H ? v : out[h];
         } else if constexpr (DT == LVAE_F32) {
             if (at + 4 <= H) out[h] = *(const f32x4_u*)((const float*)row + at);
@@ -419,60 +425,67 @@ struct FewArgs {
     float* picked;              // [T]
 };
 
-template <int DT, int NT, bool ALIGNED> __global__ __launch_bounds__(256) void few_kernel(FewArgs p) {
+template <int DT, int NT, bool ALIGNED> __global__ __launch_bounds__(64 * FEW_WAVES, 4) void few_kernel(FewArgs p) {
     constexpr int SZ = DT == LVAE_F32 ? 4 : 2, KS = FewStep<DT>::K, KL = FewStep<DT>::LANE;
-    constexpr int U = 4, PITCH = U * 128 + 16;          // steps a round; a token's bytes of one in LDS
-    __shared__ float2 red[4][NT * 16];
+    constexpr int U = NT * SZ > 4 ? 2 : 4, R = U * KS;       // steps and elements a round
+    constexpr int PITCH = U * 128 + 16;                 // a token's bytes of a round in LDS
+    constexpr int PER = U * 4, ROWS = 64 * FEW_WAVES / PER, PASSES = (NT * 16 + ROWS - 1) / ROWS;      // threads a token
+    __shared__ float2 red[FEW_WAVES][NT * 16];
     __shared__ __align__(16) char tok[2][NT * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mp = lane & 15, g4 = lane >> 4;
-    const int64_t vw = ((int64_t)blockIdx.x * 4 + wave) * 16;
+    const int64_t vw = ((int64_t)blockIdx.x * FEW_WAVES + wave) * 16;
     const char* wrow = (const char*)p.weight + min(vw + mp, p.V - 1) * p.wstride * SZ;
-    const char* trow[NT];                   // rows that this thread brings into LDS: 32 bytes of each a round
+    const int t_row = threadIdx.x / PER, t_at = threadIdx.x % PER;
+    const char* trow[PASSES];               // rows that this thread brings into LDS: 32 bytes of each a round
 #pragma unroll
-    for (int i = 0; i < NT; ++i)
-        trow[i] = (const char*)p.hidden + at_axes(p.hid, min(i * 16 + (int)(threadIdx.x >> 4), p.T - 1)) * SZ;
+    for (int i = 0; i < PASSES; ++i)
+        trow[i] = (const char*)p.hidden + at_axes(p.hid, min(i * ROWS + t_row, p.T - 1)) * SZ;
     f32x4 acc[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    f32x4 a[U][2], an[U][2], bt[NT][2];
-    auto load_w = [&](int k0) {
+    f32x4 w[2][U][2], bt[PASSES][2];          // this round's and the next one's
+    auto load_w = [&](f32x4 (&to)[U][2], int k0) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) few_load<DT, ALIGNED>(wrow, k0 + u * KS + g4 * KL, p.H, an[u]);
+        for (int u = 0; u < U; ++u) few_load<DT, ALIGNED>(wrow, k0 + u * KS + g4 * KL, p.H, to[u]);
     };
     auto load_t = [&](int k0) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) few_load<DT, ALIGNED>(trow[i], k0 + (threadIdx.x & 15) * KL, p.H, bt[i]);
+        for (int i = 0; i < PASSES; ++i) few_load<DT, ALIGNED>(trow[i], k0 + t_at * KL, p.H, bt[i]);
     };
     auto store_t = [&](int to) {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            char* q = tok[to] + (i * 16 + (threadIdx.x >> 4)) * PITCH + (threadIdx.x & 15) * 32;
+        for (int i = 0; i < PASSES; ++i) {
+            if (NT * 16 < ROWS && t_row >= NT * 16) continue;
+            char* q = tok[to] + (i * ROWS + t_row) * PITCH + t_at * 32;
             *(f32x4*)q = bt[i][0];
             *(f32x4*)(q + 16) = bt[i][1];
         }
     };
     load_t(0);
-    load_w(0);
+    load_w(w[0], 0);
     store_t(0);
-    int buf = 0;
-    for (int k0 = 0; k0 < p.H; k0 += U * KS) {
+    for (int k0 = 0;; k0 += 2 * R) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) { a[u][0] = an[u][0]; a[u][1] = an[u][1]; }
-        __syncthreads();
-        const bool more = k0 + U * KS < p.H;
-        if (more) { load_t(k0 + U * KS); load_w(k0 + U * KS); }
+        for (int d = 0; d < 2; ++d) {
+            const int k = k0 + d * R;
+            if (k >= p.H) goto done;
+            __syncthreads();
+            load_t(k + R);
+            load_w(w[d ^ 1], k + R);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const char* q = tok[buf] + (n * 16 + mp) * PITCH + u * 128 + g4 * 32;
-                const f32x4 b[2] = {*(const f32x4*)q, *(const f32x4*)(q + 16)};
-                acc[n] = few_mma<DT>(a[u], b, acc[n]);
-            }
-        buf ^= 1;
-        if (more) store_t(buf);             // the other buffer: its readers have passed the barrier above
+                for (int n = 0; n < NT; ++n) {
+                    const char* q = tok[d] + (n * 16 + mp) * PITCH + u * 128 + g4 * 32;
+                    const f32x4 b[2] = {*(const f32x4*)q, *(const f32x4*)(q + 16)};
+                    acc[n] = few_mma<DT>(w[d][u], b, acc[n]);
+                }
+            store_t(d ^ 1);                 // the other buffer: its readers have passed the barrier above
+        }
     }
+done:
     const int64_t v0 = vw + g4 * 4;
     float bias[4];
 #pragma unroll
@@ -499,10 +512,10 @@ template <int DT, int NT, bool ALIGNED> __global__ __launch_bounds__(256) void f
         if (g4 == 0) red[wave][t] = make_float2(top, sum);
     }
     __syncthreads();
-    for (int t = threadIdx.x; t < p.T; t += 256) {
+    for (int t = threadIdx.x; t < p.T; t += 64 * FEW_WAVES) {
         float2 x = red[0][t];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) x = merge_lse(x, red[w][t]);
+        for (int w = 1; w < FEW_WAVES; ++w) x = merge_lse(x, red[w][t]);
         p.part[(int64_t)t * p.blocks + blockIdx.x] = x;
     }
 }
@@ -711,7 +724,7 @@ void plan_forward(Plan* pl) {
     pl->few = pl->T <= LVAE_VOCAB_FEW;
     if (pl->few) {
         int64_t at = 0;
-        pl->few_blocks = lvae_ceil_div(pl->V, 64);
+        pl->few_blocks = lvae_ceil_div(pl->V, 16 * FEW_WAVES);
         pl->part = take(at, pl->T * pl->few_blocks * 8);
         pl->picked = take(at, pl->T * 4);
         pl->bytes = at;
@@ -884,8 +897,8 @@ RowsArgs rows_args(const lvae_vocab_problem* q, const Plan& pl, char* ws) {
 }
 
 template <int DT, int NT> void start_few(const FewArgs& f, bool aligned, hipStream_t st) {
-    if (aligned) few_kernel<DT, NT, true><<<dim3((unsigned)f.blocks), 256, 0, st>>>(f);
-    else few_kernel<DT, NT, false><<<dim3((unsigned)f.blocks), 256, 0, st>>>(f);
+    if (aligned) few_kernel<DT, NT, true><<<dim3((unsigned)f.blocks), 64 * FEW_WAVES, 0, st>>>(f);
+    else few_kernel<DT, NT, false><<<dim3((unsigned)f.blocks), 64 * FEW_WAVES, 0, st>>>(f);
 }
 template <int DT> void start_few_n(const FewArgs& f, bool aligned, hipStream_t st) {
     if (f.T <= 16) start_few<DT, 1>(f, aligned, st);
