@@ -599,3 +599,54 @@ def test_backward_without_what_the_forward_kept(T):
     assert torch.equal(ll, D.token_log_likelihood(h, w, y, b))
     for a, e in zip(got, want):
         assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_saved_tensors_kept_on_the_host(dt):
+    from lvae import decoder_ops as D
+    h, w, b, y = (t.cuda() for t in inputs(150, 700, 72, DT[dt]))
+
+    def step():
+        ts = [t.clone().requires_grad_() for t in (h, w, b)]
+        ll = D.sequence_log_likelihood(ts[0].view(3, 50, 72), ts[1], y.view(3, 50), ts[2])
+        return [ll.detach()] + list(torch.autograd.grad(ll.sum(), ts))
+    want = step()
+    with torch.autograd.graph.save_on_cpu():
+        got = step()
+    for a, e in zip(got, want):
+        assert torch.equal(a, e)
+
+
+def test_two_captured_steps_that_share_their_memory():
+    """Loss, gradients and clipping of a float32 and of a bfloat16 step in two graphs of one pool, replayed in turn."""
+    from lvae import decoder_ops as D, grad_ops as G
+    data = [tuple(t.cuda() for t in inputs(T, 900, 64, dt, seed=T)) for T, dt in ((200, torch.float32), (40, torch.bfloat16))]
+
+    def step(h, w, b, y):
+        ts = [t.detach().requires_grad_() for t in (h, w, b)]
+        loss = D.vocab_cross_entropy(ts[0], ts[1], y, ts[2])
+        grads = list(torch.autograd.grad(loss, ts))
+        norm = G.clip_grads(grads, 0.05)
+        return [loss.detach(), norm] + grads
+    static = [[t.clone() for t in d] for d in data]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in static:
+            step(*s)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for s in static:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], pool=graphs[0].pool() if len(graphs) > 1 else None):
+            outs.append(step(*s))
+    for k in range(4):
+        for i, s in enumerate(static):
+            h, _, _, y = (t.cuda() for t in inputs(data[i][0].shape[0], 900, 64, data[i][0].dtype, seed=50 + k, ignore=0.25 * k))
+            s[0].copy_(h)
+            s[3].copy_(y)
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            want = step(h, data[i][1], data[i][2], y)
+            for a, e in zip(outs[i], want):
+                assert torch.equal(a, e)
