@@ -650,3 +650,26 @@ def test_two_captured_steps_that_share_their_memory():
             want = step(h, data[i][1], data[i][2], y)
             for a, e in zip(outs[i], want):
                 assert torch.equal(a, e)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_two_pieces_of_the_vocabulary(dt):
+    """More tokens x words than the workspace holds the gradient of at once, the second piece smaller than the first
+    (the oracle in float64 on the GPU)."""
+    import ctypes
+    from lvae import _native as N, decoder_ops as D
+    T, V, H = 4096, 70001, 64
+    h, w, b, y = (t.cuda() for t in inputs(T, V, H, DT[dt], seed=3))
+    gy = torch.randn(T, generator=torch.Generator().manual_seed(1)).cuda()
+    three, out = ctypes.c_int64 * 3, ctypes.c_int64(0)
+    q = N.VocabProblem(256, 256, 256, 256, three(1, 1, T), three(0, 0, H), three(0, 0, 1), V, H, -100, H, 1 if dt == "bf16" else 0, 0, 0)
+    N.check(N.lib().lvae_vocab_ll_bwd_workspace_bytes(q, 0, 1, 0, out))
+    assert out.value < T * V * (2 if dt == "bf16" else 4)          # not all of it at once
+    ts = [t.clone().requires_grad_() for t in (h, w, b)]
+    ll = D.token_log_likelihood(ts[0], ts[1], y, ts[2])
+    ll.backward(-gy)
+    o = {k: v.cpu() for k, v in oracle(h, w, b, y, gy).items()}
+    close(ll, o["ll"], o["tol"], "ll")
+    close(ts[0].grad, o["dh"], o["tol_dh"], "d_hidden")
+    close(ts[1].grad, o["dw"], o["tol_dw"], "d_weight")
+    close(ts[2].grad, o["db"], o["tol_db"], "d_bias")
