@@ -574,7 +574,15 @@ __global__ __launch_bounds__(256) void final_kernel(FinalArgs p) {
         const int h = (int)(i - t * per) * 4, j = p.inv[t];
         f32x4 x = {0.f, 0.f, 0.f, 0.f};
         if (j >= 0) {
-            for (int s = 0; s < p.splits; ++s) x += *(const f32x4*)(p.slab + s * p.slab_stride + j * p.ld + h);
+            const float* q = p.slab + j * p.ld + h;
+            for (int s = 0; s < p.splits; s += 4) {         // four loads in flight
+                f32x4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = *(const f32x4*)(q + min(s + k, p.splits - 1) * p.slab_stride);
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (s + k < p.splits) x += v[k];
+            }
             x *= p.unscale[0];
             if (p.dt == LVAE_F32) {
 #pragma unroll
@@ -649,8 +657,7 @@ struct Plan {
     int64_t T, Tpad, V, Vpad, H, Kp;
     int planes;
     bool few, direct_w;
-    int narrow, tile_n;         // of dHidden
-    int narrow_l, tile_l;       // of the logits
+    int narrow, tile_n;         // of the logits
     int64_t piece;              // words of the vocabulary a time (backward)
     int splits_h, splits_w;
     // offsets into the workspace, bytes
@@ -687,13 +694,12 @@ int check_problem(const lvae_vocab_problem* q, Plan* pl) {
                    q->weight_stride < (1 << 22) && ((uintptr_t)q->weight & 15) == 0;
     pl->planes_bytes = lvae_round_up(pl->planes * pl->V * pl->Kp * 2, 256);
     pl->kept = q->dtype == LVAE_F32 && T > LVAE_VOCAB_FEW ? KEPT_HEAD + pl->planes_bytes : 0;
-    // Tiles of 64 tokens, two workgroups a CU, where tiles of 256 would be mostly empty; for the logits also where there
-    // are too few of those for the 256 CUs.  Step of 2,000 tokens, 4,000 words, width 512 (128 tiles): 112 us narrow, 123
-    // wide; 200 tokens, 50,265 words, width 768 (197 tiles): 179 narrow, 164 wide.
-    pl->narrow = T <= 128;
+    // Tiles of 64 tokens, two workgroups a CU, where tiles of 256 would be mostly empty; for the logits also where these are
+    // at most 128, so that the small ones take one round of the 256 CUs.  Step of 1,024 bfloat16 tokens, 4,900 words, width
+    // 768 (80 tiles): 101 us narrow, 113 wide; 2,000 tokens, 3,800 words, width 640 (120): 133 and 144; 2,528 tokens, 3,697
+    // words, width 640 (150): 157 and 150.
+    pl->narrow = T <= 128 || pl->Vpad / 256 * lvae_ceil_div(T, 256) <= 128;
     pl->tile_n = pl->narrow ? 64 : 256;
-    pl->narrow_l = pl->narrow || pl->Vpad / 256 * lvae_ceil_div(T, 256) < 160;
-    pl->tile_l = pl->narrow_l ? 64 : 256;
     return LVAE_OK;
 }
 
@@ -758,24 +764,27 @@ void plan_backward(Plan* pl, bool want_h, bool want_w, bool want_b) {
     const int64_t th = lvae_ceil_div(pl->H, 256);
     // the sum of d_hidden runs over the whole piece: it is split so that no tile takes more than 0.6 of a CU's share of the
     // launch that holds both products
-    const int64_t tiles_h = th * lvae_ceil_div(pl->T, pl->tile_n), tiles_w = th * lvae_ceil_div(pl->piece, 256);
+    const int64_t tiles_h = th * lvae_ceil_div(pl->T, 256), tiles_w = th * lvae_ceil_div(pl->piece, 256);
     const int64_t ks_h = lvae_ceil_div(pl->piece, VG_BK), ks_w = lvae_ceil_div(pl->T, VG_BK);
     const int64_t share = (tiles_h * ks_h + tiles_w * ks_w) / 256 + 1;      // slices a CU, both products
     int64_t most = share * 6 / 10;
     if (most < 8) most = 8;
     pl->splits_h = (int)lvae_ceil_div(ks_h, most);
     if (pl->splits_h > 32) pl->splits_h = 32;
-    // the weight gradient's sum is split only where both products together leave CUs without a tile: its slabs are as
-    // large as the gradient itself
+    // The weight gradient's sum is split where its tiles, unsplit, would outlast the rest of the launch by more than its
+    // slabs take to write and to add up: at about 1.5 us a slice and product of limbs against 4 TB/s and a launch.  2,528
+    // float32 tokens, width 640, 3,697 words: both products 188 us unsplit, 114 us and 11 for the sum in three parts.
     pl->splits_w = 1;
-    if (tiles_w + tiles_h * pl->splits_h < 192 && ks_w > most) {
-        pl->splits_w = (int)lvae_ceil_div(ks_w, most);
-        if (pl->splits_w > 32) pl->splits_w = 32;
+    const int64_t most_w = share < 8 ? 8 : share;
+    if (ks_w > most_w) {
+        const int64_t n = lvae_ceil_div(ks_w, most_w) < 32 ? lvae_ceil_div(ks_w, most_w) : 32;
+        const double saved = 1.5 * (pl->planes == 2 ? 3 : 1) * (double)(ks_w - lvae_ceil_div(ks_w, n));
+        if (saved > 6.0 + (double)(n * pl->piece * pl->Kp) * 8 / 4e6) pl->splits_w = (int)n;
     }
     pl->slab = want_h ? take(at, pl->splits_h * pl->Tpad * pl->Kp * 4) : 0;
     pl->slab_w = want_w && pl->splits_w > 1 ? take(at, pl->splits_w * pl->piece * pl->Kp * 4) : 0;
     // column sums of all pieces for one reduction at the end, or of one piece where that would take over 256 MiB
-    const int64_t parts = pl->Tpad / pl->tile_l * (pl->narrow_l ? 2 : 4);
+    const int64_t parts = pl->Tpad / pl->tile_n * (pl->narrow ? 2 : 4);
     pl->ld_dbias = parts * pl->Vpad * 4 <= 256ll << 20 ? pl->Vpad : pl->piece;
     pl->dbias = want_b ? take(at, parts * pl->ld_dbias * 4) : 0;
     pl->bytes = at;
@@ -873,7 +882,7 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
     a->N = pl.T;
     a->K = pl.Kp;
     a->n_rows = rows.n_rows;
-    a->tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_l);
+    a->tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_n);
     a->splits = 1;
     a->bias = bias;
     a->tgt = rows.tgt_of;
@@ -979,7 +988,7 @@ extern "C" int lvae_vocab_ll(const lvae_vocab_problem* q, float* ll, float* lse,
     a.part = part;
     a.ldp = pl.Tpad;
     a.picked = picked;
-    RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow_l, a, st));
+    RUN(launch_tiles(q->dtype, VG_LOGITS_LSE, pl.narrow, a, st));
     FinishArgs f = {};
     f.part = part;
     f.tiles = a.tiles_m;
@@ -1034,7 +1043,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     RUN(launch_operands(q, pl, rows, (char*)const_cast<void*>(kept), ws, &a, st)       /* read only there */);
     const float* unscale = rows.unscale;
     const int64_t esz = q->dtype == LVAE_F32 ? 4 : 2;
-    const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow_l ? 2 : 4;
+    const int th = (int)lvae_ceil_div(pl.H, 256), waves_n = pl.narrow ? 2 : 4;
     uint16_t* gbuf = (uint16_t*)(ws + pl.g);
     VgArgs dl = a;                                       // the gradient of the logits
     dl.lse = rows.lse_of;
@@ -1055,7 +1064,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     h.N = pl.T;
     h.n_rows = rows.n_rows;
     h.tiles_m = th;
-    h.tiles_n = (int)lvae_ceil_div(pl.T, pl.tile_n);
+    h.tiles_n = (int)lvae_ceil_div(pl.T, 256);
     h.splits = pl.splits_h;
     h.slab = (float*)(ws + pl.slab);
     h.ld_slab = pl.Kp;
@@ -1084,7 +1093,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
     f.ld_part = pl.ld_dbias;
     f.V = d_bias ? pl.V : 0;
     f.per_tile = waves_n;
-    f.tile_rows = pl.tile_l;
+    f.tile_rows = pl.tile_n;
     f.bias_dt = q->bias_dtype;
     f.d_bias = d_bias;
     f.n_rows = rows.n_rows;
@@ -1098,7 +1107,7 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         dl.bias = a.bias + v0;
         dl.v0 = v0;
         dl.dbias = d_bias ? (float*)(ws + pl.dbias) + (bias_whole ? v0 : 0) : nullptr;
-        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow_l, dl, st));
+        RUN(launch_tiles(q->dtype, VG_LOGITS_GRAD, pl.narrow, dl, st));
         if (d_bias && !bias_whole) {
             FinalArgs b = f;
             b.V = words;
@@ -1112,11 +1121,11 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
         w.N = words;
         w.tiles_n = dl.tiles_m;
         w.out = (char*)d_weight + v0 * pl.H * esz;
-        if (d_hidden && d_weight && !pl.narrow) {
+        if (d_hidden && d_weight) {
             const int64_t ks_h = lvae_ceil_div(words, VG_BK) / pl.splits_h, ks_w = lvae_ceil_div(pl.T, VG_BK) / pl.splits_w;
             RUN(launch_both(q->dtype, mode_w, h, w, ks_h >= ks_w, st));
         } else {
-            if (d_hidden) RUN(launch_tiles(q->dtype, VG_DHIDDEN, pl.narrow, h, st));
+            if (d_hidden) RUN(launch_tiles(q->dtype, VG_DHIDDEN, 0, h, st));
             if (d_weight) RUN(launch_tiles(q->dtype, mode_w, 0, w, st));
         }
         if (d_weight && pl.splits_w > 1) {

@@ -11,21 +11,19 @@ static int vg_start(const VgArgs& p, hipStream_t st) {
     return LVAE_OK;
 }
 
-template <int DT, int WM, int WN, int NJ, int NA> static int vg_mode(int mode, const VgArgs& p, hipStream_t st) {
-    switch (mode) {
-        case VG_LOGITS_LSE: return vg_start<DT, false, false, VG_LSE, WM, WN, NJ, NA>(p, st);
-        case VG_LOGITS_GRAD: return vg_start<DT, false, false, VG_GRAD, WM, WN, NJ, NA>(p, st);
-        case VG_DHIDDEN: return vg_start<DT, true, false, VG_SLAB, WM, WN, NJ, NA>(p, st);
-        case VG_DWEIGHT_SLAB: return vg_start<DT, true, true, VG_SLAB, WM, WN, NJ, NA>(p, st);
-        default: return vg_start<DT, true, true, VG_OUT, WM, WN, NJ, NA>(p, st);
-    }
-}
-
 #define VG_WIDE 2, 4, 4, 3
 #define VG_NARROW 2, 2, 2, 2
 
 int VG_NAME(int mode, int narrow, const VgArgs& p, hipStream_t st) {
-    return narrow ? vg_mode<VG_DT, VG_NARROW>(mode, p, st) : vg_mode<VG_DT, VG_WIDE>(mode, p, st);
+    switch (mode) {
+        case VG_LOGITS_LSE:
+            return narrow ? vg_start<VG_DT, false, false, VG_LSE, VG_NARROW>(p, st) : vg_start<VG_DT, false, false, VG_LSE, VG_WIDE>(p, st);
+        case VG_LOGITS_GRAD:
+            return narrow ? vg_start<VG_DT, false, false, VG_GRAD, VG_NARROW>(p, st) : vg_start<VG_DT, false, false, VG_GRAD, VG_WIDE>(p, st);
+        case VG_DHIDDEN: return vg_start<VG_DT, true, false, VG_SLAB, VG_WIDE>(p, st);
+        case VG_DWEIGHT_SLAB: return vg_start<VG_DT, true, true, VG_SLAB, VG_WIDE>(p, st);
+        default: return vg_start<VG_DT, true, true, VG_OUT, VG_WIDE>(p, st);
+    }
 }
 
 int VG_NAME_BOTH(int mode_w, const VgArgs& h, const VgArgs& w, int h_first, hipStream_t st) {
