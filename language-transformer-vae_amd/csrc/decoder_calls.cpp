@@ -1,15 +1,17 @@
-// Host helper of decoder_ops: checks the tensors of a call, lays them out as lvae_vocab_problem, allocates what it
-// writes and calls liblvae.
+// Host side of decoder_ops: checks the tensors of a call, lays them out as lvae_vocab_problem, allocates what it writes,
+// calls liblvae, and stands in autograd's graph.
 //
-// A training step of a few hundred tokens is 80 us of GPU work; the same in Python, through ctypes, took 45 us of host time
-// in a warm loop and twice that between the threads of autograd, more than the rest of the step.  The entry points are
-// those of the library that Python has loaded (bind), so there is one library and one place that finds it.
+// A training step of a few hundred tokens is 50-80 us of GPU work; with all this in Python, through ctypes, it took 45 us of
+// host time in a warm loop and twice that between the threads of autograd, more than the rest of the step (340 float16
+// tokens, 9,999 words: 160 us so, 102 us with calls and layout here, 82 us with the node of the graph here too).  The
+// entry points are those of the library that Python has loaded (bind), so there is one library and one place that finds it.
 #define PY_SSIZE_T_CLEAN
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/object_ptr.h>
+#include <pybind11/pybind11.h>
 #include <ATen/ops/empty.h>
-#include <ATen/ops/zeros.h>
 #include <c10/core/DeviceGuard.h>
 
 #include "../../include/lvae.h"
@@ -34,9 +36,16 @@ int code(at::ScalarType t) {
     return t == at::kFloat ? LVAE_F32 : t == at::kBFloat16 ? LVAE_BF16 : t == at::kHalf ? LVAE_F16 : -1;
 }
 
+// what Python has set, as an exception that may cross threads: a backward runs on one of autograd's own
+[[noreturn]] void throw_python() {
+    python_error e;
+    e.persist();
+    throw e;
+}
 [[noreturn]] void fail(PyObject* type, const std::string& what) {
+    pybind11::gil_scoped_acquire gil;
     PyErr_SetString(type, what.c_str());
-    throw python_error();
+    throw_python();
 }
 void check(int rc) {
     if (rc != LVAE_OK) fail(lib.error, "liblvae status " + std::to_string(rc) + ": " + lib.last_error());
@@ -80,18 +89,27 @@ struct Problem {
     at::Tensor empty(at::IntArrayRef sizes, at::ScalarType t) const { return at::empty(sizes, at::TensorOptions(device).dtype(t)); }
 };
 
-at::Tensor tensor(PyObject* o, const char* name) {
-    if (!THPVariable_Check(o)) fail(PyExc_TypeError, std::string(name) + " must be a torch.Tensor");
-    at::Tensor t = THPVariable_Unpack(o);
-    if (!t.is_cuda()) fail(lib.error, std::string(name) + " is on " + t.device().str() + ": the HIP path needs a GPU tensor (no CPU fallback)");
-    return t;
+void* current_stream(at::Device device) {
+    pybind11::gil_scoped_acquire gil;
+    THPObjectPtr h(PyObject_CallFunction(lib.raw_stream, "i", (int)device.index()));
+    void* stream = h ? PyLong_AsVoidPtr(h) : nullptr;
+    if (!stream && PyErr_Occurred()) throw_python();
+    return stream;
 }
 
-void prepare(Problem& q, PyObject* hidden, PyObject* weight, PyObject* targets, PyObject* bias, int64_t ignore_index) {
-    q.hidden = tensor(hidden, "hidden");
-    q.weight = tensor(weight, "weight");
-    q.targets = tensor(targets, "targets");
-    if (bias != Py_None) q.bias = tensor(bias, "bias");
+void on_gpu(const at::Tensor& t, const char* name) {
+    if (!t.is_cuda()) fail(lib.error, std::string(name) + " is on " + t.device().str() + ": the HIP path needs a GPU tensor (no CPU fallback)");
+}
+
+void prepare(Problem& q, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const at::Tensor& bias, int64_t ignore_index) {
+    on_gpu(hidden, "hidden");
+    on_gpu(weight, "weight");
+    on_gpu(targets, "targets");
+    if (bias.defined()) on_gpu(bias, "bias");
+    q.hidden = hidden;
+    q.weight = weight;
+    q.targets = targets;
+    q.bias = bias;
     q.device = q.hidden.device();
     if (q.weight.device() != q.device || q.targets.device() != q.device || (q.bias.defined() && q.bias.device() != q.device))
         fail(PyExc_ValueError, "hidden, weight, targets and bias must be on one device");
@@ -147,51 +165,40 @@ void prepare(Problem& q, PyObject* hidden, PyObject* weight, PyObject* targets, 
     q.c.dtype = dtype;
     q.c.bias_dtype = bias_dtype;
     q.c.reserved = 0;
-    THPObjectPtr stream(PyObject_CallFunction(lib.raw_stream, "i", (int)q.device.index()));
-    if (!stream) throw python_error();
-    q.stream = PyLong_AsVoidPtr(stream);
-    if (!q.stream && PyErr_Occurred()) throw python_error();
+    q.stream = current_stream(q.device);
 }
 
+// f() while other Python threads may run
 template <class F> int without_gil(F f) {
-    int rc;
-    Py_BEGIN_ALLOW_THREADS
-    rc = f();
-    Py_END_ALLOW_THREADS
-    return rc;
+    if (!PyGILState_Check()) return f();
+    pybind11::gil_scoped_release released;
+    return f();
 }
 
 void* data(const at::Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
-PyObject* wrap(const at::Tensor& t) {
-    if (!t.defined()) Py_RETURN_NONE;
-    return THPVariable_Wrap(t);
-}
-at::Tensor unwrap(PyObject* o) { return o == Py_None ? at::Tensor() : THPVariable_Unpack(o); }
 
-// forward(hidden, weight, targets, bias, ignore_index, how, for_backward) -> result, or with for_backward
-// (result, hidden, weight, targets, bias as they are read, LSE of every token, factor of every token in a loss, what is kept of
-// the weights)
-PyObject* forward(PyObject*, PyObject* args) {
-    HANDLE_TH_ERRORS
-    PyObject *hidden, *weight, *targets, *bias;
-    long long ignore_index;
-    int how, for_backward;
-    if (!PyArg_ParseTuple(args, "OOOOLip", &hidden, &weight, &targets, &bias, &ignore_index, &how, &for_backward)) return nullptr;
-    Problem q;
-    prepare(q, hidden, weight, targets, bias, ignore_index);
+// What a forward leaves for its backward: the LSE of every token, the factor of every token in a loss, limbs of the weights
+struct Saved {
+    at::Tensor lse, each, kept;
+};
+
+at::Tensor run_forward(const Problem& q, int how, Saved* saved) {
     const c10::DeviceGuard guard(q.device);
     const at::Tensor ll = q.empty(q.shape, at::kFloat);
     at::Tensor lse, kept, loss, each, out = ll;
     int64_t kept_bytes = 0;
-    if (for_backward) {
+    if (saved) {
         lse = q.empty(q.shape, at::kFloat);
         if (q.tokens) check(lib.kept_bytes(&q.c, &kept_bytes));
         if (kept_bytes) kept = q.empty({kept_bytes}, at::kByte);
     }
     if (how >= MEAN) {
-        const at::TensorOptions o = at::TensorOptions(q.device).dtype(at::kFloat);
-        loss = q.tokens ? at::empty({}, o) : at::zeros({}, o);
-        each = q.tokens ? at::empty({}, o) : at::zeros({}, o);
+        loss = q.empty({}, at::kFloat);
+        each = q.empty({}, at::kFloat);
+        if (!q.tokens) {
+            loss.zero_();
+            each.zero_();
+        }
         out = loss;
     }
     if (how == SEQUENCES) out = q.empty(at::IntArrayRef(q.shape).slice(0, q.shape.size() - 1), at::kFloat);
@@ -201,33 +208,23 @@ PyObject* forward(PyObject*, PyObject* args) {
         if (kept_bytes) bytes -= kept_bytes - 256;
         const at::Tensor ws = q.empty({bytes}, at::kByte);
         check(without_gil([&] {
-            return lib.ll(&q.c, (float*)data(ll), (float*)data(lse), data(kept), (float*)data(loss), (float*)data(each),
-                          how == MEAN, data(ws), bytes, q.stream);
+            return lib.ll(&q.c, (float*)data(ll), (float*)data(lse), data(kept), (float*)data(loss), (float*)data(each), how == MEAN,
+                          data(ws), bytes, q.stream);
         }));
     }
     if (how == SEQUENCES && out.numel())
         check(without_gil([&] { return lib.segment_sum((const float*)data(ll), out.numel(), q.shape.back(), (float*)data(out), q.stream); }));
-    if (!for_backward) return wrap(out);
-    return Py_BuildValue("NNNNNNNN", wrap(out), wrap(q.hidden), wrap(q.weight), wrap(q.targets), wrap(q.bias), wrap(lse), wrap(each),
-                         wrap(kept));
-    END_HANDLE_TH_ERRORS
+    if (saved) *saved = Saved{lse, each, kept};
+    return out;
 }
 
-// backward(hidden, weight, targets, bias, ignore_index, how, lse, each, kept, g, three truth values) -> gradients of
-// hidden, weight and bias, None where not wanted
-PyObject* backward(PyObject*, PyObject* args) {
-    HANDLE_TH_ERRORS
-    PyObject *hidden, *weight, *targets, *bias, *lse_, *each_, *kept_, *g_;
-    long long ignore_index;
-    int how, want_h, want_w, want_b;
-    if (!PyArg_ParseTuple(args, "OOOOLiOOOOppp", &hidden, &weight, &targets, &bias, &ignore_index, &how, &lse_, &each_, &kept_, &g_,
-                          &want_h, &want_w, &want_b))
-        return nullptr;
-    // planned anew: a hook of the saved tensors may have moved them or laid them out in another way
-    Problem q;
-    prepare(q, hidden, weight, targets, bias, ignore_index);
+struct Gradients {
+    at::Tensor hidden, weight, bias;
+};
+
+Gradients run_backward(const Problem& q, int how, const Saved& saved, at::Tensor g, bool want_h, bool want_w, bool want_b) {
     const c10::DeviceGuard guard(q.device);
-    at::Tensor lse = unwrap(lse_).contiguous(), each = unwrap(each_), kept = unwrap(kept_), g = unwrap(g_);
+    const at::Tensor lse = saved.lse.contiguous();
     if (g.scalar_type() != at::kFloat) g = g.to(at::kFloat);
     int64_t g_stride[3] = {0, 0, 0};
     if (how < MEAN) {
@@ -237,24 +234,99 @@ PyObject* backward(PyObject*, PyObject* args) {
         g_stride[1] = q.c.size[2];
         g_stride[2] = 1;
     }
-    at::Tensor d_h, d_w, d_b;
-    if (want_h) d_h = q.empty(q.hidden.sizes(), q.hidden.scalar_type());
-    if (want_w) d_w = q.empty(q.weight.sizes(), q.weight.scalar_type());
-    if (want_b) d_b = q.empty(q.bias.sizes(), q.bias.scalar_type());
+    Gradients d;
+    if (want_h) d.hidden = q.empty(q.hidden.sizes(), q.hidden.scalar_type());
+    if (want_w) d.weight = q.empty(q.weight.sizes(), q.weight.scalar_type());
+    if (want_b) d.bias = q.empty(q.bias.sizes(), q.bias.scalar_type());
     if (q.tokens) {
         int64_t bytes = 0;
         check(lib.bwd_bytes(&q.c, want_h, want_w, want_b, &bytes));
-        if (kept.defined()) bytes -= kept.numel() - 256;
+        if (saved.kept.defined()) bytes -= saved.kept.numel() - 256;
         const at::Tensor ws = q.empty({bytes}, at::kByte);
         check(without_gil([&] {
-            return lib.bwd(&q.c, (const float*)data(lse), (const float*)data(g), g_stride, (const float*)data(each),
-                           data(kept), data(d_h), data(d_w), data(d_b), data(ws), bytes, q.stream);
+            return lib.bwd(&q.c, (const float*)data(lse), (const float*)data(g), g_stride, (const float*)data(saved.each), data(saved.kept),
+                           data(d.hidden), data(d.weight), data(d.bias), data(ws), bytes, q.stream);
         }));
     } else {
-        if (want_w) d_w.zero_();
-        if (want_b) d_b.zero_();
+        if (want_w) d.weight.zero_();
+        if (want_b) d.bias.zero_();
     }
-    return Py_BuildValue("NNN", wrap(d_h), wrap(d_w), wrap(d_b));
+    return d;
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// A gradient that refuses to be differentiated again, rather than to count as a constant
+struct Once : torch::autograd::Function<Once> {
+    static at::Tensor forward(AutogradContext*, const at::Tensor& t, const at::Tensor&, const at::Tensor&, const std::optional<at::Tensor>&,
+                              const at::Tensor&) {
+        return t.view_as(t);
+    }
+    static variable_list backward(AutogradContext*, const variable_list&) {
+        fail(lib.error, "the log-likelihoods have no second derivatives");
+    }
+};
+
+// Token log-likelihoods, put together, with a HIP backward: the softmax is computed again from the saved LSE, a piece of
+// the vocabulary at a time
+struct LogLikelihood : torch::autograd::Function<LogLikelihood> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets,
+                              const std::optional<at::Tensor>& bias, int64_t ignore_index, int64_t how) {
+        Problem q;
+        prepare(q, hidden, weight, targets, bias.value_or(at::Tensor()), ignore_index);
+        Saved saved;
+        const at::Tensor out = run_forward(q, (int)how, &saved);
+        ctx->save_for_backward({q.hidden, q.weight, q.targets, q.bias, saved.lse, saved.each, saved.kept});
+        ctx->saved_data["ignore_index"] = ignore_index;
+        ctx->saved_data["how"] = how;
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, const variable_list& g) {
+        const variable_list s = ctx->get_saved_variables();
+        const at::Tensor &hidden = s[0], &weight = s[1], &bias = s[3];
+        const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = bias.defined() && ctx->needs_input_grad(3);
+        variable_list d(6);
+        if (!want_h && !want_w && !want_b) return d;
+        Gradients got;
+        {
+            const at::NoGradGuard no_grad;
+            // planned anew: a hook of the saved tensors may have moved them or laid them out in another way
+            Problem q;
+            prepare(q, hidden, weight, s[2], bias, ctx->saved_data["ignore_index"].toInt());
+            got = run_backward(q, (int)ctx->saved_data["how"].toInt(), Saved{s[4], s[5], s[6]}, g[0], want_h, want_w, want_b);
+        }
+        const std::optional<at::Tensor> b = bias.defined() ? std::optional<at::Tensor>(bias) : std::nullopt;
+        auto once = [&](const at::Tensor& t) {
+            return t.defined() && at::GradMode::is_enabled() ? Once::apply(t, hidden, weight, b, g[0]) : t;      // create_graph
+        };
+        d[0] = once(got.hidden);
+        d[1] = once(got.weight);
+        d[3] = once(got.bias);
+        return d;
+    }
+};
+
+at::Tensor tensor(PyObject* o, const char* name) {
+    if (!THPVariable_Check(o)) fail(PyExc_TypeError, std::string(name) + " must be a torch.Tensor");
+    return THPVariable_Unpack(o);
+}
+
+// log_likelihood(hidden, weight, targets, bias, ignore_index, how)
+PyObject* log_likelihood(PyObject*, PyObject* args) {
+    HANDLE_TH_ERRORS
+    PyObject *hidden_, *weight_, *targets_, *bias_;
+    long long ignore_index;
+    int how;
+    if (!PyArg_ParseTuple(args, "OOOOLi", &hidden_, &weight_, &targets_, &bias_, &ignore_index, &how)) return nullptr;
+    const at::Tensor hidden = tensor(hidden_, "hidden"), weight = tensor(weight_, "weight"), targets = tensor(targets_, "targets");
+    const at::Tensor bias = bias_ == Py_None ? at::Tensor() : tensor(bias_, "bias");
+    if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad())))
+        return THPVariable_Wrap(LogLikelihood::apply(hidden, weight, targets, bias.defined() ? std::optional<at::Tensor>(bias) : std::nullopt,
+                                                     (int64_t)ignore_index, (int64_t)how));
+    Problem q;
+    prepare(q, hidden, weight, targets, bias, ignore_index);
+    return THPVariable_Wrap(run_forward(q, how, nullptr));
     END_HANDLE_TH_ERRORS
 }
 
@@ -305,8 +377,7 @@ PyObject* bind(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "bind(entry points, exception class, stream of a device)"},
-                         {"forward", forward, METH_VARARGS, "forward(hidden, weight, targets, bias, ignore_index, how, for_backward)"},
-                         {"backward", backward, METH_VARARGS, "backward(hidden, weight, targets, bias, ignore_index, how, lse, each, kept, g, wanted...)"},
+                         {"log_likelihood", log_likelihood, METH_VARARGS, "log_likelihood(hidden, weight, targets, bias, ignore_index, how)"},
                          {"common_axes", py_common_axes, METH_VARARGS, "common_axes(shape, [strides of each tensor])"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

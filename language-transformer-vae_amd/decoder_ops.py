@@ -20,7 +20,6 @@ import ctypes
 import torch
 
 from . import _native as N
-from .estimators import _needs_grad
 
 try:
     from . import _decoder_calls
@@ -31,7 +30,7 @@ _bound = None
 
 
 def _calls():
-    """The C++ side of a call (checks, layout, allocation, launches), bound to the library that is loaded."""
+    """The C++ side of a call (checks, layout, allocation, launches, autograd), bound to the library that is loaded."""
     global _bound
     lib = N.lib()
     if _bound is not lib:
@@ -54,45 +53,8 @@ def _common_axes(shape, strides):
 _TOKENS, _SEQUENCES, _MEAN, _SUM = range(4)
 
 
-class _VocabLL(torch.autograd.Function):
-    """Token log-likelihoods, put together, with a HIP backward (lvae_vocab_ll_bwd): the softmax is computed again from
-    the saved LSE, a piece of the vocabulary at a time."""
-
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, targets, ignore_index, how):
-        out, *saved = _calls().forward(hidden, weight, targets, bias, ignore_index, how, True)
-        ctx.save_for_backward(*saved)
-        ctx.how, ctx.ignore_index = how, ignore_index
-        return out
-
-    @staticmethod
-    def backward(ctx, g):
-        hidden, weight, targets, bias, lse, each, kept = ctx.saved_tensors
-        needs = ctx.needs_input_grad[:3]
-        if not any(needs):
-            return None, None, None, None, None, None
-        grads = _calls().backward(hidden, weight, targets, bias, ctx.ignore_index, ctx.how, lse, each, kept, g, *needs)
-        if torch.is_grad_enabled():                       # create_graph
-            grads = (None if t is None else _Once.apply(t, hidden, weight, bias, g) for t in grads)
-        return (*grads, None, None, None)
-
-
-class _Once(torch.autograd.Function):
-    """A gradient that refuses to be differentiated again, rather than to count as a constant."""
-
-    @staticmethod
-    def forward(ctx, t, *depends_on):
-        return t.view_as(t)
-
-    @staticmethod
-    def backward(ctx, _):
-        raise N.LvaeError("the log-likelihoods have no second derivatives")
-
-
 def _run(hidden, weight, targets, bias, ignore_index, how):
-    if _needs_grad(hidden, weight, bias):
-        return _VocabLL.apply(hidden, weight, bias, targets, ignore_index, how)
-    return _calls().forward(hidden, weight, targets, bias, ignore_index, how, False)
+    return _calls().log_likelihood(hidden, weight, targets, bias, ignore_index, how)
 
 
 def token_log_likelihood(hidden, weight, targets, bias=None, ignore_index=-100):
