@@ -191,3 +191,18 @@ def test_columns_of_one_buffer():
     norm = G.clip_grads(parts, n / 3)
     assert abs(norm.item() - n) <= 2 * U * n
     check([buf], [src], (n / 3) / (n + 1e-6), "columns")
+
+
+@pytest.mark.parametrize("a,b", [("bf16", "f32"), ("f16", None), ("f32", "bf16")])
+def test_lists_larger_than_the_caches(a, b):
+    """The scaling that goes past the caches, in 16 bits, off the natural alignment and with a ragged end."""
+    from lvae import grad_ops as G
+    src = [torch.randn(40_000_003, device="cuda").to(DT[a])[3:], torch.randn(1001, device="cuda").to(DT[a])]
+    keep = [t.clone() for t in src]
+    out = None if b is None else [torch.empty(t.shape, dtype=DT[b], device="cuda") for t in src]
+    n = norm64(src)
+    norm = G.clip_grads(src, n / 5, out=out)
+    assert abs(norm.item() - n) <= 2 * U * n
+    check(out or src, keep, (n / 5) / (n + 1e-6), "large")
+    if out:
+        assert all(torch.equal(x, y) for x, y in zip(src, keep))
