@@ -99,7 +99,8 @@ template <int DT> __device__ __forceinline__ void pack_row(const void* src, int6
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = 0.f;
             if (there && k + 8 <= H) {
-                const f32x4 a = *(const f32x4_u*)q, b = *(const f32x4_u*)(q + 4);
+                // past the caches: what is read next are the limbs (step of 565 tokens 770 us without, 761 with)
+                const f32x4 a = __builtin_nontemporal_load((const f32x4_u*)q), b = __builtin_nontemporal_load((const f32x4_u*)(q + 4));
 #pragma unroll
                 for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[4 + i] = b[i]; }
             } else if (there) {
