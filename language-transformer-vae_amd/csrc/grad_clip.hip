@@ -11,8 +11,8 @@
 // tensors in the arguments of the two kernels themselves; longer lists are first written to the workspace by launches
 // that only do that (2 us each), because one full launch over all tensors beats several of a part of the GPU each
 // (260 tensors, 60 M bfloat16 elements into float32: 156 us with a launch for each 112, 130 us so; 389 float32 tensors,
-// 253 M elements, 715 and 606 us).
-// The norm reads 5.2 TB/s (253 M float32), scaling moves 5.3 TB/s (a large copy: 4.8).
+// 253 M elements, 715 and 606 us; with scaling past the caches, below, 96 and 560 us).
+// The norm reads 5.2-5.8 TB/s (253 M float32), scaling moves 5.4 TB/s (a large copy: 4.8).
 #include <stdlib.h>
 
 #include "vocab_gemm.h"
