@@ -673,3 +673,55 @@ def test_two_pieces_of_the_vocabulary(dt):
     close(ts[0].grad, o["dh"], o["tol_dh"], "d_hidden")
     close(ts[1].grad, o["dw"], o["tol_dw"], "d_weight")
     close(ts[2].grad, o["db"], o["tol_db"], "d_bias")
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_recomputed_in_the_backward(dt, reentrant):
+    from torch.utils.checkpoint import checkpoint
+    from lvae import decoder_ops as D
+    h, w, b, y = (t.cuda() for t in inputs(150, 700, 72, DT[dt]))
+
+    def loss(h, w, b):
+        return D.vocab_cross_entropy(h * 2.0, w, y, b)
+
+    def step(f):
+        ts = [t.clone().requires_grad_() for t in (h, w, b)]
+        out = f(*ts)
+        out.backward()
+        return [out.detach()] + [t.grad for t in ts]
+    for a, e in zip(step(lambda *ts: checkpoint(loss, *ts, use_reentrant=reentrant)), step(loss)):
+        assert torch.equal(a, e)
+
+
+def test_two_host_threads():
+    """Calls from two Python threads on streams of their own, errors of one not reported by the other."""
+    import threading
+    from lvae import decoder_ops as D
+    work = [tuple(t.cuda() for t in inputs(T, 2000, 128, dt, seed=T)) for T, dt in ((50, torch.bfloat16), (300, torch.float32))]
+
+    def step(h, w, b, y):
+        ts = [t.detach().requires_grad_() for t in (h, w, b)]
+        loss = D.vocab_cross_entropy(ts[0], ts[1], y, ts[2])
+        return [loss.detach()] + list(torch.autograd.grad(loss, ts))
+    want = [step(*x) for x in work]
+    torch.cuda.synchronize()
+    failures = []
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got = step(*work[k])
+                    with pytest.raises(ValueError, match="do not expand"):
+                        D.token_log_likelihood(work[k][0], work[k][1], work[k][3][:-1])
+                    torch.cuda.current_stream().synchronize()
+                    assert all(torch.equal(a, e) for a, e in zip(got, want[k]))
+        except BaseException as e:                        # reported by the main thread
+            failures.append(e)
+    threads = [threading.Thread(target=run, args=(k,)) for k in (0, 1)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
