@@ -445,7 +445,7 @@ typedef struct {
 } lvae_vocab_problem;
 
 /* ll, lse [size0*size1*size2] float32, contiguous; lse (0 for ignored tokens) is what the backward needs and may be
- * NULL.  Up to LVAE_VOCAB_FEW tokens the weights are streamed once past all tokens in registers; beyond, matrix-core
+ * NULL.  Up to LVAE_VOCAB_FEW tokens the weights are streamed once past all tokens; beyond, matrix-core
  * tiles (float32 as two fp16 limbs).  kept: lvae_vocab_ll_kept_bytes of device memory, 256-byte aligned, or NULL; float32
  * calls of more than LVAE_VOCAB_FEW tokens (else the size is 0, and kept has to be NULL) leave weight in it as limbs, with
  * the powers of two that hidden and weight are scaled by; handed to the backward of the same inputs, unchanged, that saves

@@ -4,7 +4,7 @@
 //   forward   rows -> pack -> tiles (running maximum and sum of each token over 256 words) -> finish
 //   backward  rows -> pack -> per piece of the vocabulary: logits again -> G (16 bits, workspace) -> dHidden += G W,
 //             dWeight = G^T H -> finish
-//   few       up to 64 tokens: every wave streams 16 rows of W past all tokens in registers -> finish
+//   few       up to 64 tokens: every wave streams 16 rows of W past all tokens -> finish
 //
 // `rows` lists the tokens that count, in order, with the place of their hidden state: padding costs nothing in the
 // products, and what a hidden state of padding holds (NaN) meets nothing.

@@ -457,6 +457,10 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, int tm, int tn, int64_t
             p.part[(int64_t)tm * p.ldp + n0 + c] = x;
         }
     } else if constexpr (EPI == VG_GRAD) {
+        // 16 columns of G at a time go through this wave's own part of LDS, so that a store writes 256 bytes of a row at once
+        // instead of 16 bytes of 64 places; two parts in turn.  A wave's LDS accesses complete in order.
+        constexpr int PLANES = DT == LVAE_F32 ? 2 : 1, ROW = 256 + 16;
+        static_assert(2 * W * PLANES * 16 * ROW <= vg_lds_bytes<WM, WN, WN == 4 ? 4 : NJ, NA>(), "LDS of the kernel");
         f32x4 colsum[MI];
 #pragma unroll
         for (int i = 0; i < MI; ++i) colsum[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -468,7 +472,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, int tm, int tn, int64_t
             const float lse = there ? p.lse[n] : 0.f, gy = there ? p.gy[n] : 0.f;
             const bool all = n0 + (wn + 1) * 16 * NJ <= n_lim;
             const bool hit = __any(rel >= 0 && rel < 32);
-            uint16_t* row = p.g + n * p.ldg + mb;
+            char* stage = lds + (wave * 2 + (j & 1)) * PLANES * 16 * ROW;
 #pragma unroll
             for (int i = 0; i < MI; ++i) {
 #pragma unroll
@@ -500,8 +504,20 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, int tm, int tn, int64_t
                     }
                 }
 #pragma unroll
-                for (int l = 0; l < (DT == LVAE_F32 ? 2 : 1); ++l) *(s16x8*)(row + l * p.plane_g + 4 * i) = o[l];
+                for (int l = 0; l < PLANES; ++l) *(s16x8*)(stage + l * 16 * ROW + mp * ROW + g4 * 64 + i * 8) = o[l];
             }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int l = 0; l < PLANES; ++l)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int r = q * 4 + g4;
+                    *(s16x8*)(p.g + l * p.plane_g + (n0 + wn * 16 * NJ + j * 16 + r) * p.ldg + m0 + wm * 128 + mp * 8) =
+                        *(const s16x8*)(stage + l * 16 * ROW + r * ROW + mp * 16);
+                }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("" ::: "memory");
         }
         if (p.dbias) {
             float* d = p.dbias + ((int64_t)tn * WN + wn) * p.ld_dbias + mb;
