@@ -529,53 +529,68 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, int tm, int tn, int64_t
                 if (mp == 0) *(f32x4*)(d + 4 * i) = v;
             }
         }
-    } else if constexpr (EPI == VG_SLAB) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int64_t n = n0 + nb + j * 16;
-            if (n >= n_lim) continue;
-            float* row = p.slab + split * p.slab_stride + n * p.ld_slab + mb;
-#pragma unroll
-            for (int i = 0; i < MI; ++i) {
-                if (mb + 4 * i >= p.ld_slab) continue;  // the pitch is a multiple of 64
-                f32x4 v = acc[i][j];
-                if (p.slab_add) v += *(const f32x4*)(row + 4 * i);
-                *(f32x4*)(row + 4 * i) = v;
-            }
-        }
     } else {
-        const float f = p.unscale ? p.unscale[0] : 1.f;
-        const int e = DT == LVAE_F32 ? -p.exponents[p.exponent_of] : 0;
-        const bool whole = mb + 32 <= p.M;              // rows of any alignment: the stores need that of an element alone
+        // float32 slabs, or the output: 16 columns at a time through LDS as above, 256 or 512 bytes of a row at once
+        constexpr bool F32 = EPI == VG_SLAB || DT == LVAE_F32;
+        constexpr int ROW = (F32 ? 512 : 256) + 16, LANES = F32 ? 32 : 16, E = 128 / LANES;     // lanes a row, elements a lane
+        static_assert(2 * W * 16 * ROW <= vg_lds_bytes<WM, WN, WN == 4 ? 4 : NJ, NA>(), "LDS of the kernel");
+        const float f = EPI == VG_OUT && p.unscale ? p.unscale[0] : 1.f;
+        const int e = EPI == VG_OUT && DT == LVAE_F32 ? -p.exponents[p.exponent_of] : 0;
+        const int64_t m = m0 + wm * 128 + (lane % LANES) * E;
+        const bool whole = m + E <= p.M;                // rows of any alignment: the stores need that of an element alone
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            const int64_t n = n0 + nb + j * 16;
-            if (n >= n_lim) continue;
-            if constexpr (DT == LVAE_F32) {
-                float* row = (float*)p.out + n * p.ld_out + mb;
+            char* stage = lds + (wave * 2 + (j & 1)) * 16 * ROW;
 #pragma unroll
-                for (int i = 0; i < MI; ++i) {
-                    f32x4 o;
+            for (int i = 0; i < MI; i += 2) {
+                if constexpr (F32) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[r] = ldexpf(acc[i][j][r] * f, e);
-                    if (whole) *(f32x4_u*)(row + 4 * i) = o;
-                    else
-                        for (int r = 0; r < 4; ++r)
-                            if (mb + 4 * i + r < p.M) row[4 * i + r] = o[r];
-                }
-            } else {
-                uint16_t* row = (uint16_t*)p.out + n * p.ld_out + mb;
+                    for (int h = 0; h < 2; ++h) {
+                        f32x4 o = acc[i + h][j];
+                        if constexpr (EPI == VG_OUT)
 #pragma unroll
-                for (int i = 0; i < MI; i += 2) {
+                            for (int r = 0; r < 4; ++r) o[r] = ldexpf(o[r] * f, e);
+                        *(f32x4*)(stage + mp * ROW + g4 * 128 + (i + h) * 16) = o;
+                    }
+                } else {
                     s16x8 o;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] = vg_round<DT>(acc[i + (e >> 2)][j][e & 3] * f);
-                    if (whole) *(s16x8_u*)(row + 4 * i) = o;
-                    else
-                        for (int e = 0; e < 8; ++e)
-                            if (mb + 4 * i + e < p.M) row[4 * i + e] = o[e];
+                    for (int k = 0; k < 8; ++k) o[k] = vg_round<DT>(acc[i + (k >> 2)][j][k & 3] * f);
+                    *(s16x8*)(stage + mp * ROW + g4 * 64 + i * 8) = o;
                 }
             }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int q = 0; q < LANES / 4; ++q) {
+                const int r = q * (64 / LANES) + lane / LANES;
+                const int64_t n = n0 + wn * 16 * NJ + j * 16 + r;
+                const char* from = stage + r * ROW + (lane % LANES) * 16;
+                if (n >= n_lim) continue;
+                if constexpr (EPI == VG_SLAB) {
+                    float* to = p.slab + split * p.slab_stride + n * p.ld_slab + m;
+                    if (m >= p.ld_slab) continue;       // the pitch is a multiple of 64
+                    f32x4 v = *(const f32x4*)from;
+                    if (p.slab_add) v += *(const f32x4*)to;
+                    *(f32x4*)to = v;
+                } else if constexpr (F32) {
+                    float* to = (float*)p.out + n * p.ld_out + m;
+                    const f32x4 v = *(const f32x4*)from;
+                    if (whole) *(f32x4_u*)to = v;
+                    else
+                        for (int k = 0; k < 4; ++k)
+                            if (m + k < p.M) to[k] = v[k];
+                } else {
+                    uint16_t* to = (uint16_t*)p.out + n * p.ld_out + m;
+                    const s16x8 v = *(const s16x8*)from;
+                    if (whole) *(s16x8_u*)to = v;
+                    else
+                        for (int k = 0; k < 8; ++k)
+                            if (m + k < p.M) to[k] = v[k];
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            asm volatile("" ::: "memory");
         }
     }
 }
