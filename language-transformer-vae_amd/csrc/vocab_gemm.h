@@ -12,7 +12,7 @@
 // What bounds it, at 16,384 tokens, width 1,024, 50,265 words, bf16 (1.69 TFLOP a product): the matrix cores are busy for
 // half of the cycles, at 2.06-2.2 GHz where 2.4 is the card's, that is, power: matrix instructions alone, on random data
 // in registers, reach 1,925 TFLOP/s (2,447 on zeros), this loop without its loads 1,620 and with everything 1,080-1,200;
-// the library's product of 8,192^3 1,253.  Logits 1.46 ms, G 1.77 ms (1.60 stored through LDS), dHidden 1.38 ms,
+// the library's product of 8,192^3 1,253.  Logits 1.46 ms, G 1.77 ms (5 % less since it is stored through LDS), dHidden 1.38 ms,
 // dWeight 1.50 ms.  Measured and not kept: 256 x 128 tiles, two workgroups a CU (64-byte rows: L2 delivers 26 of 55 bytes
 // a clock and CU), wave groups taking turns at LDS and matrix cores, a workgroup streaming through several tiles (no gain
 // where power bounds), four waves of 128 x 128 (registers spill), non-temporal stores of G (1.6 times the time).
