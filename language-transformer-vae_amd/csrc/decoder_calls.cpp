@@ -15,6 +15,7 @@
 #include <c10/core/DeviceGuard.h>
 
 #include "../../include/lvae.h"
+#include "tensor_checks.h"
 
 namespace {
 
@@ -99,6 +100,15 @@ void* current_stream(at::Device device) {
 
 void on_gpu(const at::Tensor& t, const char* name) {
     if (!t.is_cuda()) fail(lib.error, std::string(name) + " is on " + t.device().str() + ": the HIP path needs a GPU tensor (no CPU fallback)");
+}
+
+// refused wherever it lives: its result would be wrong without a word
+void check_plain(const at::Tensor& t, const char* name) {
+    if (!t.defined()) return;
+    if (const char* why = more_than_memory(t)) fail(lib.error, std::string(name) + " " + why);
+}
+void check_not_traced() {
+    if (being_traced()) fail(lib.error, "the log-likelihoods cannot be traced: a trace would not hold their kernels");
 }
 
 void prepare(Problem& q, const at::Tensor& hidden, const at::Tensor& weight, const at::Tensor& targets, const at::Tensor& bias, int64_t ignore_index) {
@@ -288,6 +298,8 @@ struct LogLikelihood : torch::autograd::Function<LogLikelihood> {
         const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = bias.defined() && ctx->needs_input_grad(3);
         variable_list d(6);
         if (!want_h && !want_w && !want_b) return d;
+        check_not_traced();
+        check_plain(g[0], "the upstream gradient");
         Gradients got;
         {
             const at::NoGradGuard no_grad;
@@ -321,6 +333,11 @@ PyObject* log_likelihood(PyObject*, PyObject* args) {
     if (!PyArg_ParseTuple(args, "OOOOLi", &hidden_, &weight_, &targets_, &bias_, &ignore_index, &how)) return nullptr;
     const at::Tensor hidden = tensor(hidden_, "hidden"), weight = tensor(weight_, "weight"), targets = tensor(targets_, "targets");
     const at::Tensor bias = bias_ == Py_None ? at::Tensor() : tensor(bias_, "bias");
+    check_not_traced();
+    check_plain(hidden, "hidden");
+    check_plain(weight, "weight");
+    check_plain(bias, "bias");
+    check_plain(targets, "targets");
     if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (bias.defined() && bias.requires_grad())))
         return THPVariable_Wrap(LogLikelihood::apply(hidden, weight, targets, bias.defined() ? std::optional<at::Tensor>(bias) : std::nullopt,
                                                      (int64_t)ignore_index, (int64_t)how));

@@ -8,6 +8,7 @@
 #include <torch/csrc/Exceptions.h>
 
 #include "../../include/lvae.h"
+#include "tensor_checks.h"
 
 namespace {
 
@@ -23,6 +24,10 @@ const at::Tensor* tensor_at(PyObject* list, Py_ssize_t i, const char* name, cons
         return nullptr;
     }
     const at::Tensor& t = THPVariable_Unpack(o);
+    if (const char* why = t.defined() ? more_than_memory(t) : nullptr) {
+        PyErr_Format(PyExc_RuntimeError, "%s[%zd] %s", name, i, why);
+        return nullptr;
+    }
     if (!t.defined() || !t.is_cuda()) {
         PyErr_Format(PyExc_RuntimeError, "%s[%zd] is not on a GPU: the HIP path needs GPU tensors (no CPU fallback)", name, i);
         return nullptr;
@@ -51,6 +56,10 @@ PyObject* table(PyObject*, PyObject* args) {
     PyObject *src, *dst;
     int writes = 0;
     if (!PyArg_ParseTuple(args, "O!Op", &PyList_Type, &src, &dst, &writes)) return nullptr;
+    if (being_traced()) {
+        PyErr_SetString(PyExc_RuntimeError, "the norm of gradients and their clipping cannot be traced: a trace would not hold their kernels");
+        return nullptr;
+    }
     const bool out = dst != Py_None;
     const Py_ssize_t n = PyList_GET_SIZE(src);
     if (out && (!PyList_Check(dst) || PyList_GET_SIZE(dst) != n)) {

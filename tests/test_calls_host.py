@@ -1,0 +1,68 @@
+"""CPU-side checks of what the vocabulary and gradient operators refuse before they ask where a tensor lives."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwd
+
+
+def arguments():
+    return torch.randn(3, 8), torch.randn(5, 8), torch.randn(5), torch.zeros(3, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_derivatives_are_refused(which, grad):
+    """The kernels read memory and carry no tangent: a result without one would count as a derivative of zero."""
+    from lvae import _native as N, decoder_ops as D, grad_ops as G
+    h, w, b, y = arguments()
+    ts = [h, w, b]
+    if grad:
+        ts[which].requires_grad_()
+    with fwd.dual_level():
+        dual = list(ts)
+        dual[which] = fwd.make_dual(ts[which], torch.ones_like(ts[which]))
+        for f in (D.token_log_likelihood, D.sequence_log_likelihood, D.vocab_cross_entropy):
+            with pytest.raises(N.LvaeError, match="forward-mode"):
+                f(dual[0], dual[1], y, dual[2])
+            with torch.no_grad(), pytest.raises(N.LvaeError, match="forward-mode"):
+                f(dual[0], dual[1], y, dual[2])
+        for f in (G.global_grad_norm, lambda t: G.clip_grads(t, 1.0)):
+            with pytest.raises(N.LvaeError, match="forward-mode"):
+                f([dual[which]])
+    with pytest.raises(N.LvaeError, match="no CPU fallback"):     # the tangent has gone with its level
+        D.token_log_likelihood(dual[0], dual[1], y, dual[2])
+
+
+def test_transforms_are_refused():
+    """torch.func wraps its tensors: they have no memory of their own."""
+    from lvae import _native as N, decoder_ops as D, grad_ops as G
+    h, w, b, y = arguments()
+    loss = lambda h: D.vocab_cross_entropy(h, w, y, b)
+    with pytest.raises(N.LvaeError, match="torch.func"):
+        torch.func.grad(loss)(h)
+    with pytest.raises(N.LvaeError, match="torch.func"):
+        torch.func.jvp(loss, (h,), (h,))
+    with pytest.raises(N.LvaeError, match="torch.func"):
+        torch.func.vmap(loss)(h[None])
+    with pytest.raises(N.LvaeError, match="torch.func"):
+        torch.func.vmap(lambda y: D.token_log_likelihood(h, w, y, b))(y[None])
+    with pytest.raises(N.LvaeError, match="torch.func"):
+        torch.func.vmap(lambda t: G.global_grad_norm([t]))(h)
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tracing_is_refused(grad):
+    """A trace would hold the allocations and not the kernels."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from lvae import _native as N, decoder_ops as D, grad_ops as G
+    h, w, b, y = arguments()
+    h.requires_grad_(grad)
+    calls = [(lambda h: D.token_log_likelihood(h, w, y, b), h), (lambda h: D.vocab_cross_entropy(h, w, y, b), h),
+             (lambda t: G.global_grad_norm([t]), w), (lambda t: G.clip_grads([t], 1.0), w)]
+    for f, x in calls:
+        with pytest.raises(N.LvaeError, match="traced"):
+            torch.jit.trace(f, (x,))
+        with pytest.raises(N.LvaeError, match="traced"):
+            make_fx(f)(x)
+        with FakeTensorMode() as fake, pytest.raises(N.LvaeError, match="traced"):
+            f(fake.from_tensor(x))
