@@ -116,10 +116,11 @@ void prepare(Problem& q, const at::Tensor& hidden, const at::Tensor& weight, con
     on_gpu(weight, "weight");
     on_gpu(targets, "targets");
     if (bias.defined()) on_gpu(bias, "bias");
-    q.hidden = hidden;
-    q.weight = weight;
-    q.targets = targets;
-    q.bias = bias;
+    // a negated view (the imaginary part of a conjugate) holds the other sign in memory
+    q.hidden = hidden.resolve_neg();
+    q.weight = weight.resolve_neg();
+    q.targets = targets.resolve_neg();
+    q.bias = bias.defined() ? bias.resolve_neg() : bias;
     q.device = q.hidden.device();
     if (q.weight.device() != q.device || q.targets.device() != q.device || (q.bias.defined() && q.bias.device() != q.device))
         fail(PyExc_ValueError, "hidden, weight, targets and bias must be on one device");
@@ -235,6 +236,7 @@ struct Gradients {
 Gradients run_backward(const Problem& q, int how, const Saved& saved, at::Tensor g, bool want_h, bool want_w, bool want_b) {
     const c10::DeviceGuard guard(q.device);
     const at::Tensor lse = saved.lse.contiguous();
+    g = g.resolve_neg();
     if (g.scalar_type() != at::kFloat) g = g.to(at::kFloat);
     int64_t g_stride[3] = {0, 0, 0};
     if (how < MEAN) {

@@ -83,7 +83,8 @@ PyObject* table(PyObject*, PyObject* args) {
             if (!ok) break;
             if (i == 0) device = s->device();
             wants_grad = wants_grad || s->requires_grad();
-            bool plain = s->is_contiguous() || s->is_non_overlapping_and_dense();
+            // a negated view (the imaginary part of a conjugate) holds the other sign in memory
+            bool plain = (s->is_contiguous() || s->is_non_overlapping_and_dense()) && !s->is_neg();
             const at::Tensor* d = nullptr;
             if (out) {
                 d = tensor_at(dst, i, "out", &device);
@@ -95,7 +96,7 @@ PyObject* table(PyObject*, PyObject* args) {
                     ok = false;
                     break;
                 }
-                plain = plain && (s->strides() == d->strides() || (s->is_contiguous() && d->is_contiguous()));
+                plain = plain && !d->is_neg() && (s->strides() == d->strides() || (s->is_contiguous() && d->is_contiguous()));
             }
             if (writes && !plain && repeats(d ? *d : *s)) {
                 PyErr_Format(PyExc_RuntimeError, "%s[%zd] is broadcast: several of its elements are one place in memory", d ? "out" : "grads", i);

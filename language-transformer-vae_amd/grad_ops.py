@@ -36,7 +36,7 @@ def _call(src, dst, norm_type, scale, max_norm):
     if odd:
         src2, copies = list(src), list(copies)
         for i in odd:
-            src2[i] = src[i].detach().contiguous()
+            src2[i] = src[i].detach().resolve_neg().contiguous()
             copies[i] = src2[i] if dst is None else torch.empty(dst[i].shape, dtype=dst[i].dtype, device=dst[i].device)
         table = _table(src2, None if dst is None else copies)[0]
     count = len(src)

@@ -27,3 +27,35 @@ def test_forward_mode_derivatives_are_refused():
         plain, = torch.autograd.grad(ll, hr, one)          # tensors without a tangent are served as ever
         assert torch.isfinite(plain).all()
     assert (t == 1).all() and (out == 0).all()
+
+
+def test_negated_views():
+    """The imaginary part of a conjugate is a view whose memory holds the other sign; nothing else shows it."""
+    from lvae import decoder_ops as D, grad_ops as G
+    for T in (9, 100):
+        g = torch.Generator(device="cuda").manual_seed(T)
+        r = lambda *s: torch.randn(*s, device="cuda", generator=g)
+        h, w, b = r(T, 8), r(300, 8), r(300)
+        y = torch.randint(0, 300, (T,), device="cuda", generator=g)
+
+        def step(h, w, b):
+            ll = D.token_log_likelihood(h, w, y, b)
+            return [ll.detach()] + list(torch.autograd.grad(ll.sum(), (h, w, b)))
+        negated = [torch._neg_view(-t) for t in (h, w, b)]
+        assert all(t.is_neg() and torch.equal(t, u) for t, u in zip(negated, (h, w, b)))
+        want = step(*[t.requires_grad_() for t in (h, w, b)])
+        for a, e in zip(step(*[t.requires_grad_() for t in negated]), want):
+            assert torch.equal(a, e)
+        one = torch.complex(h.detach()[:, 0], h.detach()[:, 1]).conj().imag[:, None]       # a single column, two apart
+        w1 = w.detach()[:, :1].contiguous()
+        assert one.is_neg() and torch.equal(D.token_log_likelihood(one, w1, y), D.token_log_likelihood((-h.detach()[:, 1:2]).contiguous(), w1, y))
+    t = torch.randn(50, device="cuda")
+    for src, dst in ((torch._neg_view(t.clone()), torch.empty(50, device="cuda")), ((-t), torch._neg_view(torch.empty(50, device="cuda"))),
+                     (torch._neg_view(t.clone()), torch._neg_view(torch.empty(50, device="cuda")))):
+        G.clip_grads([src], 0.5, out=[dst])
+        want = torch.empty(50, device="cuda")
+        G.clip_grads([-t], 0.5, out=[want])
+        assert torch.equal(dst, want)
+    n = torch._neg_view(t.clone())
+    G.clip_grads([n], 0.5)
+    assert torch.equal(n, want)
