@@ -114,11 +114,6 @@ PyObject* table(PyObject*, PyObject* args) {
                 Py_XDECREF(k);
             }
         }
-        // a graph that has saved one of them must see that it changes; only once all are known to be in order
-        for (Py_ssize_t i = 0; ok && writes && i < n; ++i) {
-            const at::Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(out ? dst : src, i));
-            if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-        }
     } catch (...) {
         Py_DECREF(bytes);
         Py_DECREF(odd);
@@ -133,7 +128,19 @@ PyObject* table(PyObject*, PyObject* args) {
     END_HANDLE_TH_ERRORS
 }
 
+// written(tensors): a graph that has saved one of them sees that it has changed
+PyObject* written(PyObject*, PyObject* list) {
+    HANDLE_TH_ERRORS
+    for (Py_ssize_t i = 0; i < PyList_GET_SIZE(list); ++i) {
+        const at::Tensor& t = THPVariable_Unpack(PyList_GET_ITEM(list, i));
+        if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+    }
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {{"table", table, METH_VARARGS, "table(src, dst or None, writes) -> (bytes, device, requires_grad, odd)"},
+                         {"written", written, METH_O, "written(tensors of a list that table() has taken)"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -50,6 +50,7 @@ def _call(src, dst, norm_type, scale, max_norm):
         N.check(lib.lvae_clip_grads(table, count, int(norm_type == float("inf")), int(scale), float(max_norm), norm.data_ptr(),
                                     ws.data_ptr(), nbytes.value, N.raw_stream(index)))
     if scale:
+        _tensor_list.written(src if dst is None else dst)
         for i in odd:
             (src if dst is None else dst)[i].detach().copy_(copies[i])
     return norm

@@ -59,3 +59,33 @@ def test_negated_views():
     n = torch._neg_view(t.clone())
     G.clip_grads([n], 0.5)
     assert torch.equal(n, want)
+
+
+def test_a_refused_clip_changes_nothing():
+    """Neither values nor version counters: a graph that has saved one of the tensors still runs backward."""
+    from lvae import _native as N, grad_ops as G
+    t, u = torch.full((100,), 2.0, device="cuda"), torch.full((100,), 3.0, device="cuda")
+    wants = torch.full((100,), 2.0, device="cuda", requires_grad=True)
+    x = torch.ones(100, device="cuda", requires_grad=True)
+    out = x * t
+    for call, error in ((lambda: G.clip_grads([t, t], 1.0), "share memory"), (lambda: G.clip_grads([t[:60], t[50:]], 1.0), "share memory"),
+                        (lambda: G.clip_grads([u, u.clone()], 1.0, out=[t, t]), "share memory"),
+                        (lambda: G.clip_grads([t, wants], 1.0), "requires grad"), (lambda: G.clip_grads([u, u], 1.0, out=[t, wants]), "requires grad")):
+        before = t._version, u._version, wants._version
+        with pytest.raises(N.LvaeError, match=error):
+            call()
+        assert (t._version, u._version, wants._version) == before
+        assert (t == 2).all() and (u == 3).all() and (wants == 2).all()
+    out.sum().backward()
+    assert torch.equal(x.grad, t)
+    out = x * t
+    before = u._version
+    G.clip_grads([u], 1.0, out=[t])
+    assert u._version == before
+    with pytest.raises(RuntimeError, match="inplace"):            # what was written is noticed as before
+        out.sum().backward()
+    column = torch.ones(30, 4, device="cuda")
+    out = x[:30, None] * column
+    G.clip_grads([column[:, 1]], 0.5)                            # through a dense copy
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
