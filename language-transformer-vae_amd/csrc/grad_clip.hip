@@ -79,22 +79,24 @@ template <bool STREAM> __device__ __forceinline__ void load8(const void* p, int6
         }
     }
 }
-template <bool STREAM, class V> __device__ __forceinline__ void store_as(V* p, V v) {
-    if (STREAM) __builtin_nontemporal_store(v, p);
-    else *p = v;
-}
 template <bool STREAM> __device__ __forceinline__ void store8(void* p, int64_t i0, int dt, const float x[8]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int64_t i = i0 + h * (CHUNK / 2) + threadIdx.x * 4;
         if (dt == LVAE_F32) {
-            store_as<STREAM>((f32x4_u*)((float*)p + i), f32x4_u{x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]});
+            // the pointer's own type has to reach the store: through a deduced parameter it would lose its alignment
+            f32x4_u* q = (f32x4_u*)((float*)p + i);
+            const f32x4 v = {x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]};
+            if (STREAM) __builtin_nontemporal_store(v, q);
+            else *q = v;
         } else {
-            s16x4_u v;
+            s16x4_u* q = (s16x4_u*)((uint16_t*)p + i);
+            s16x4 v;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 v[e] = (short)(dt == LVAE_BF16 ? vg_round<LVAE_BF16>(x[4 * h + e]) : vg_round<LVAE_F16>(x[4 * h + e]));
-            store_as<STREAM>((s16x4_u*)((uint16_t*)p + i), v);
+            if (STREAM) __builtin_nontemporal_store(v, q);
+            else *q = v;
         }
     }
 }

@@ -66,3 +66,18 @@ def test_tracing_is_refused(grad):
             make_fx(f)(x)
         with FakeTensorMode() as fake, pytest.raises(N.LvaeError, match="traced"):
             f(fake.from_tensor(x))
+
+
+@pytest.mark.parametrize("source", ["grad_clip", "vocab_ce", "vocab_tiles_f32", "vocab_tiles_bf16", "vocab_tiles_f16"])
+def test_no_kernel_promises_an_alignment_that_its_callers_need_not_have(source):
+    """Tensors are views that start anywhere: an access through a pointer that has lost its reduced alignment on the way
+    promises the compiler 8 or 16 bytes.  The compiler's own diagnosis, as an error."""
+    import os
+    import subprocess
+    hipcc = "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("no HIP compiler")
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "language-transformer-vae_amd", "csrc")
+    r = subprocess.run([hipcc, "-std=c++17", "--offload-arch=gfx950", "-fsyntax-only", "-Werror=align-mismatch", source + ".hip"],
+                       cwd=csrc, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-3000:]
