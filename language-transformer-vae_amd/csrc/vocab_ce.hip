@@ -24,6 +24,9 @@ namespace {
 constexpr float F16_G_SCALE = 16384.f;       // also of the limbs of float32
 constexpr int64_t KEPT_HEAD = 256;
 constexpr int MAX_PARTS = 512;              // workgroups that look for the largest magnitude of W, and of H
+// workgroups that copy W, 1,024 threads each: with those that list tokens (512) and those of the bias (V / 1,024 < 2^16) a
+// launch stays below 2^32 threads for every V; up to 2^25 words each copies its 16 rows and is done
+constexpr int64_t MAX_COPIERS = 1 << 21;
 
 struct Axes {
     int64_t size[3], stride[3];
@@ -286,8 +289,10 @@ template <int DT> __global__ __launch_bounds__(1024, DT == LVAE_F32 ? 8 : 4) voi
         if (v < p.Vpad) p.bias_out[v] = v >= p.V ? -INFINITY : p.bias ? load_any(p.bias, v, p.bias_dtype) : 0.f;
         return;
     }
-    const int64_t r = (int64_t)(b - p.bias_blocks) * 16 + (threadIdx.x >> 6);
-    if (r < p.V) pack_row<DT>(p.weight, r * p.wstride, true, p.H, p.Kp, e_w, p.wpack + r * p.Kp, p.V * p.Kp);
+    b -= p.bias_blocks;
+    const int64_t step = (int64_t)(gridDim.x - p.row_blocks - p.bias_blocks) * 16;
+    for (int64_t r = (int64_t)b * 16 + (threadIdx.x >> 6); r < p.V; r += step)
+        pack_row<DT>(p.weight, r * p.wstride, true, p.H, p.Kp, e_w, p.wpack + r * p.Kp, p.V * p.Kp);
 }
 
 __device__ __forceinline__ float2 merge_lse(float2 a, float2 b) {
@@ -867,7 +872,8 @@ int launch_operands(const lvae_vocab_problem* q, const Plan& pl, RowsArgs& rows,
         largest_kernel<<<dim3((unsigned)(rows.h_blocks + rows.w_blocks)), 1024, 0, st>>>(rows);
         LVAE_LAUNCH_CHECK();
     }
-    const dim3 grid((unsigned)(rows.row_blocks + rows.bias_blocks + (wp && !known ? lvae_ceil_div(pl.V, 16) : 0)));
+    const int64_t copiers = wp && !known ? lvae_ceil_div(pl.V, 16) : 0;
+    const dim3 grid((unsigned)(rows.row_blocks + rows.bias_blocks + (copiers < MAX_COPIERS ? copiers : MAX_COPIERS)));
     if (q->dtype == LVAE_F32) prepare_kernel<LVAE_F32><<<grid, 1024, 0, st>>>(rows);
     else prepare_kernel<LVAE_BF16><<<grid, 1024, 0, st>>>(rows);       // 16 bits are 16 bits
     LVAE_LAUNCH_CHECK();
