@@ -639,12 +639,12 @@ __global__ __launch_bounds__(256) void dweight_kernel(const float* slab, int spl
 }
 
 __global__ __launch_bounds__(256) void segment_sum_kernel(const float* x, int64_t n, int64_t len, float* out) {
-    const int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (s >= n) return;
-    double a = 0.0;
-    for (int64_t i = threadIdx.x & 63; i < len; i += 64) a += x[s * len + i];
-    a = wave_sum_d(a);
-    if ((threadIdx.x & 63) == 0) out[s] = (float)a;
+    for (int64_t s = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); s < n; s += (int64_t)gridDim.x * 4) {
+        double a = 0.0;
+        for (int64_t i = threadIdx.x & 63; i < len; i += 64) a += x[s * len + i];
+        a = wave_sum_d(a);
+        if ((threadIdx.x & 63) == 0) out[s] = (float)a;
+    }
 }
 
 // the loss of few tokens
@@ -1168,7 +1168,8 @@ extern "C" int lvae_vocab_ll_bwd(const lvae_vocab_problem* q, const float* lse, 
 extern "C" int lvae_segment_sum_f32(const float* x, int64_t n, int64_t len, float* out, void* stream) {
     LVAE_CHECK_ARG(n >= 1 && n < (1ll << 26) && len >= 0, "bad shape: n=%lld len=%lld", (long long)n, (long long)len);
     LVAE_CHECK_ARG(out && (x || len == 0), "x and out must be non-NULL");
-    segment_sum_kernel<<<dim3((unsigned)lvae_ceil_div(n, 4)), 256, 0, (hipStream_t)stream>>>(x, n, len, out);
+    const int64_t blocks = lvae_ceil_div(n, 4), most = 1 << 23;              // 2^24 workgroups would be 2^32 threads
+    segment_sum_kernel<<<dim3((unsigned)(blocks < most ? blocks : most)), 256, 0, (hipStream_t)stream>>>(x, n, len, out);
     LVAE_LAUNCH_CHECK();
     return LVAE_OK;
 }

@@ -36,3 +36,15 @@ def test_most_words(dt):
         assert abs((l[y[t]] - lse).item() - ll[t].item()) <= 2.0 ** -8, t
         want = wd[y[t]] - (torch.exp(l - lse) * wd).sum()
         assert abs(want.item() - hr.grad[t, 0].item()) <= 2.0 ** -8 + (0 if dt == "f32" else 3 * 2.0 ** -8), t
+
+
+@pytest.mark.parametrize("n,length", [((1 << 26) - 1, 1), ((1 << 25) + 5, 3), (1000, 70), (3, 0)])
+def test_most_segments(n, length):
+    """2^26 - 1 sums: one workgroup for four of them would be 2^32 threads.  float64 inside, rounded once."""
+    from lvae import _native as N
+    x = torch.randn(n, length, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n))
+    out = torch.full((n + 4,), 7.0, device="cuda")
+    N.check(N.lib().lvae_segment_sum_f32(x.data_ptr(), n, length, out.data_ptr(), N.raw_stream(0)))
+    want = x.double().sum(1)
+    assert ((out[:n].double() - want).abs() <= U * want.abs() + length * 2.0 ** -48).all()
+    assert (out[n:] == 7).all()
