@@ -57,6 +57,10 @@ typedef enum {
                                 * form at D > 256; not for the permutation sums). */
 
 const char* lvae_last_error(void);
+
+/* Advanced with every change of an entry point's arguments or of a structure.  lvae_version() is that of the library as it was
+ * built: a caller compiled against another one must not call it. */
+#define LVAE_VERSION 102
 int lvae_version(void);
 
 /* ---------------------------------------------------------------------------------------------

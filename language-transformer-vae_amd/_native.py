@@ -10,6 +10,7 @@ import os
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
+VERSION = 102                  # LVAE_VERSION of the header that the signatures below are those of
 LIB_PATH = os.environ.get("LVAE_LIB", os.path.join(_HERE, "liblvae.so"))
 
 SPREAD_LOGVAR, SPREAD_VAR = 0, 1
@@ -144,6 +145,12 @@ class LvaeError(RuntimeError):
     pass
 
 
+def check_version(what, version):
+    """A library built from another header would take its arguments for others, pointers among them."""
+    if version != VERSION:
+        raise LvaeError(f"{what} is of version {version}, this package of {VERSION}: build it again with `make -C {_HERE}/csrc`")
+
+
 def lib():
     """Load liblvae.so once.  Raises if it has not been built (python __graft_entry__.py build)."""
     global _lib
@@ -152,6 +159,7 @@ def lib():
             raise LvaeError(f"{LIB_PATH} is missing: build it with `make -C {_HERE}/csrc` "
                             "(there is no CPU or PyTorch fallback)")
         handle = ctypes.CDLL(LIB_PATH)
+        check_version(LIB_PATH, handle.lvae_version())
         for name, (res, args) in _SIGNATURES.items():
             fn = getattr(handle, name)
             fn.restype = res

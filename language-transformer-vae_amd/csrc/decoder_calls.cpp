@@ -403,4 +403,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_decoder_calls", nullptr, -1, meth
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__decoder_calls() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__decoder_calls() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddIntConstant(m, "VERSION", LVAE_VERSION) != 0) Py_CLEAR(m);
+    return m;
+}

@@ -235,7 +235,7 @@ extern "C" int lvae_dev_reload_env(void) {
     load_switches();
     return LVAE_OK;
 }
-extern "C" int lvae_version(void) { return 100; }
+extern "C" int lvae_version(void) { return LVAE_VERSION; }
 
 // ---- optional per-launch timing of the dominant (pair) kernels ------------------------------------
 // HIP events recorded on the caller's stream right around the pair kernels, so a benchmark can price

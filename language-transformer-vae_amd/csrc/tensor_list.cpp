@@ -146,4 +146,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_list", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__tensor_list() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__tensor_list() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddIntConstant(m, "VERSION", LVAE_VERSION) != 0) Py_CLEAR(m);
+    return m;
+}

@@ -36,6 +36,7 @@ def _calls():
     if _bound is not lib:
         if _decoder_calls is None:
             raise N.LvaeError("_decoder_calls.so is missing: build it with `make -C csrc` (there is no Python fallback)")
+        N.check_version("_decoder_calls.so", getattr(_decoder_calls, "VERSION", None))
         entry_points = (lib.lvae_vocab_ll_workspace_bytes, lib.lvae_vocab_ll_kept_bytes, lib.lvae_vocab_ll,
                         lib.lvae_vocab_ll_bwd_workspace_bytes, lib.lvae_vocab_ll_bwd, lib.lvae_segment_sum_f32,
                         lib.lvae_last_error)

@@ -17,6 +17,7 @@ except ImportError:                                       # told on the first ca
 def _table(src, dst, writes=False):
     if _tensor_list is None:
         raise N.LvaeError("_tensor_list.so is missing: build it with `make -C csrc` (there is no Python fallback)")
+    N.check_version("_tensor_list.so", getattr(_tensor_list, "VERSION", None))
     try:
         return _tensor_list.table(src, dst, writes)
     except RuntimeError as e:

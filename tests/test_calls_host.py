@@ -81,3 +81,36 @@ def test_no_kernel_promises_an_alignment_that_its_callers_need_not_have(source):
     r = subprocess.run([hipcc, "-std=c++17", "--offload-arch=gfx950", "-fsyntax-only", "-Werror=align-mismatch", source + ".hip"],
                        cwd=csrc, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-3000:]
+
+
+def test_the_libraries_say_what_they_were_built_from():
+    from lvae import _decoder_calls, _native as N, _tensor_list
+    import os
+    import re
+    header = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "lvae.h")).read()
+    assert int(re.search(r"#define LVAE_VERSION (\d+)", header).group(1)) == N.VERSION == N.lib().lvae_version()
+    assert _decoder_calls.VERSION == _tensor_list.VERSION == N.VERSION
+
+
+def test_a_library_of_another_version_is_refused(tmp_path, monkeypatch):
+    """Before anything is called with arguments that it would take for others."""
+    import os
+    import subprocess
+    import sys
+    import types
+    from lvae import _native as N, decoder_ops as D, grad_ops as G
+    (tmp_path / "old.c").write_text("int lvae_version(void) { return 100; }\n")
+    subprocess.run(["gcc", "-shared", "-fPIC", "old.c", "-o", "old.so"], cwd=tmp_path, check=True)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", "from lvae import _native as N\ntry: N.lib()\nexcept N.LvaeError as e: print('refused:', e)"],
+                       cwd=root, env=dict(os.environ, LVAE_LIB=str(tmp_path / "old.so")), capture_output=True, text=True, timeout=300)
+    assert r.stdout.startswith("refused:") and "is of version 100" in r.stdout, r.stdout + r.stderr
+    old = types.SimpleNamespace(bind=None, log_likelihood=None, table=None)       # an extension from before it said so
+    monkeypatch.setattr(D, "_decoder_calls", old)
+    monkeypatch.setattr(D, "_bound", None)
+    monkeypatch.setattr(G, "_tensor_list", old)
+    h, w, b, y = arguments()
+    with pytest.raises(N.LvaeError, match="_decoder_calls.so is of version None"):
+        D.token_log_likelihood(h, w, y, b)
+    with pytest.raises(N.LvaeError, match="_tensor_list.so is of version None"):
+        G.global_grad_norm([h])
