@@ -114,3 +114,21 @@ def test_a_library_of_another_version_is_refused(tmp_path, monkeypatch):
         D.token_log_likelihood(h, w, y, b)
     with pytest.raises(N.LvaeError, match="_tensor_list.so is of version None"):
         G.global_grad_norm([h])
+
+
+def test_the_c_library_builds_without_python_and_torch():
+    """`make` (dry run) of a user of the C ABI alone."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "language-transformer-vae_amd", "csrc")
+
+    def commands(*args):
+        r = subprocess.run(["make", "-n", "-B", "-C", csrc, *args], capture_output=True, text=True, timeout=60)
+        assert r.returncode == 0, r.stderr
+        assert "-o ../liblvae.so" in r.stdout
+        return r
+    for args in (["PYTHON=/nonexistent/python3"], ["lib"], ["lib", "PYTHON=/nonexistent/python3"]):
+        r = commands(*args)
+        assert "_decoder_calls.cpp" not in r.stdout and "python3.1" not in r.stdout
+        assert "decoder_calls.cpp -o" not in r.stdout and "No such file" not in r.stderr
+    assert "decoder_calls.cpp -o" in commands().stdout and "tensor_list.cpp -o" in commands().stdout
