@@ -172,29 +172,30 @@ template <bool INF, class T> __global__ __launch_bounds__(256) void norm_kernel(
     if (threadIdx.x == 0) part[blockIdx.x] = v;
 }
 
-template <bool INF> __device__ __forceinline__ float total(const double* part, int parts, double* red) {
+template <bool INF> __device__ __forceinline__ double total(const double* part, int parts, double* red) {
     double v = 0.0;
     for (int i = threadIdx.x; i < parts; i += 256) v = join<INF>(v, part[i]);
     v = block_join<INF>(v, red);
-    return (float)(INF ? v : sqrt(v));
+    return INF ? v : sqrt(v);
 }
 
 template <bool INF> __global__ __launch_bounds__(256) void total_kernel(const double* part, int parts, float* norm) {
     __shared__ double red[4];
-    const float n = total<INF>(part, parts, red);
-    if (threadIdx.x == 0) norm[0] = n;
+    const double n = total<INF>(part, parts, red);
+    if (threadIdx.x == 0) norm[0] = (float)n;
 }
 
 // STREAM: past the caches, for lists that pass through them anyway and would only push out what others need.  In 16 bits into
 // float32, 60 M elements: a call 136 us without, 102 us with (loads alone 127, stores alone 119); 253 M float32: 614 and 571 us.
 // The norm gains nothing: where the list fits the memory-side cache it is read from there (60 M: 41 us, streamed 51).
 template <bool INF, bool STREAM, class T>
-__global__ __launch_bounds__(256) void scale_kernel(T t, const double* part, int parts, float max_norm, float* norm) {
+__global__ __launch_bounds__(256) void scale_kernel(T t, const double* part, int parts, double max_norm, float* norm) {
     __shared__ double red[4];
-    const float n_all = total<INF>(part, parts, red);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = n_all;
-    float f = max_norm / (n_all + 1e-6f);
-    f = f > 1.f ? 1.f : f;                   // NaN stays
+    const double n_all = total<INF>(part, parts, red);
+    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (float)n_all;
+    // all elements share the factor's error: it is rounded once
+    const double factor = max_norm / (n_all + 1e-6);
+    const float f = factor > 1.0 ? 1.f : (float)factor;         // NaN stays
     uint32_t c, c1;
     my_chunks(t, c, c1);
     if (c >= c1 || (f == 1.f && !t.out)) return;
@@ -300,7 +301,7 @@ int64_t long_bytes(int64_t count) { return lvae_round_up(count * (8 + 8 + 8 + 4 
 constexpr int64_t STREAM_BYTES = 128ll << 20;
 
 template <bool INF, class T>
-int launch(const T& t, int scale, int64_t bytes, float max_norm, double* part, float* norm, hipStream_t st) {
+int launch(const T& t, int scale, int64_t bytes, double max_norm, double* part, float* norm, hipStream_t st) {
     const int g = (int)(t.chunks < BLOCKS ? t.chunks : BLOCKS);
     norm_kernel<INF, T><<<dim3((unsigned)g), 256, 0, st>>>(t, part);
     LVAE_LAUNCH_CHECK();
@@ -348,7 +349,6 @@ extern "C" int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int i
     if (ws_bytes < need) return lvae_set_error(LVAE_ERR_WORKSPACE, "workspace too small: %lld < %lld bytes", (long long)ws_bytes, (long long)need);
     hipStream_t st = (hipStream_t)stream;
     double* part = (double*)ws;
-    const float bound = (float)max_norm;
     Table t;
     uint32_t at = 0;
     int64_t i = fill(list, count, 0, &at, &t);
@@ -358,7 +358,7 @@ extern "C" int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int i
         return LVAE_OK;
     }
     if (i == count)
-        return inf_norm ? launch<true>(t, scale, bytes, bound, part, norm, st) : launch<false>(t, scale, bytes, bound, part, norm, st);
+        return inf_norm ? launch<true>(t, scale, bytes, max_norm, part, norm, st) : launch<false>(t, scale, bytes, max_norm, part, norm, st);
     char* p = (char*)ws + PART_BYTES;
     LongTable l;
     l.src = (const void**)p;
@@ -378,5 +378,5 @@ extern "C" int lvae_clip_grads(const lvae_grad_entry* list, int64_t count, int i
         i = fill(list, count, i, &at, &t);
     }
     l.chunks = at;
-    return inf_norm ? launch<true>(l, scale, bytes, bound, part, norm, st) : launch<false>(l, scale, bytes, bound, part, norm, st);
+    return inf_norm ? launch<true>(l, scale, bytes, max_norm, part, norm, st) : launch<false>(l, scale, bytes, max_norm, part, norm, st);
 }

@@ -89,3 +89,22 @@ def test_a_refused_clip_changes_nothing():
     G.clip_grads([column[:, 1]], 0.5)                            # through a dense copy
     with pytest.raises(RuntimeError, match="inplace"):
         out.sum().backward()
+
+
+def test_the_factor_of_clipping_is_rounded_once():
+    """n ones have the norm sqrt(n): each becomes the factor itself, max_norm / (sqrt(n) + 1e-6) in float64, rounded to float32 (half
+    a step, 2^-24 of the value; 2^-40 of it for the float64 arithmetic)."""
+    from lvae import grad_ops as G
+    for n in range(2, 400, 7):
+        for bound in (0.1, 1.0 / 3.0, 0.7):
+            want = bound / (n ** 0.5 + 1e-6)
+            t = [torch.ones(n, device="cuda")]
+            G.clip_grads(t, bound)
+            assert (t[0].double() - want).abs().max().item() <= (2.0 ** -24 + 2.0 ** -40) * want, (n, bound)
+        t = [torch.ones(n, device="cuda")]
+        G.clip_grads(t, 0.1, norm_type=float("inf"))
+        assert (t[0].double() - 0.1 / (1 + 1e-6)).abs().max().item() <= (2.0 ** -24 + 2.0 ** -40) * 0.1
+    # a norm beyond float32, which reads as inf, of elements that are not: they are scaled by what it is
+    t = [torch.full((100,), 3e38, device="cuda")]
+    assert G.clip_grads(t, 1e10).item() == float("inf")
+    assert (t[0].double() - 1e9).abs().max().item() <= (2.0 ** -23 + 2.0 ** -40) * 1e9        # the factor and the product
