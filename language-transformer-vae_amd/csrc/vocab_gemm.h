@@ -9,13 +9,15 @@
 // two of b deep, 160 KiB.  Nothing is ever transposed in memory: an operand stored [k][m] is staged as it lies and read
 // with ds_read_b64_tr_b16, which hands each lane four k values of its own column.
 //
-// What bounds it, at 16,384 tokens, width 1,024, 50,265 words, bf16 (1.69 TFLOP a product): the matrix cores are busy for
-// half of the cycles, at 2.06-2.2 GHz where 2.4 is the card's, that is, power: matrix instructions alone, on random data
-// in registers, reach 1,925 TFLOP/s (2,447 on zeros), this loop without its loads 1,620 and with everything 1,080-1,200;
-// the library's product of 8,192^3 1,253.  Logits 1.46 ms, G 1.77 ms (5 % less since it is stored through LDS), dHidden 1.38 ms,
-// dWeight 1.50 ms.  Measured and not kept: 256 x 128 tiles, two workgroups a CU (64-byte rows: L2 delivers 26 of 55 bytes
-// a clock and CU), wave groups taking turns at LDS and matrix cores, a workgroup streaming through several tiles (no gain
-// where power bounds), four waves of 128 x 128 (registers spill), non-temporal stores of G (1.6 times the time).
+// What bounds it, at 16,384 tokens, width 1,024, 50,265 words, bf16 (1.69 TFLOP a product): power.  By the counters
+// (SQ_VALU_MFMA_BUSY_CYCLES over 1,024 SIMDs, GRBM_GUI_ACTIVE) the matrix cores are busy for 53 % of the cycles in the logits,
+// 45 % in G and 55 % in dHidden and dWeight together, at 1.93-1.97 GHz where 2.4 is the card's; matrix instructions alone, on
+// random data in registers, reach 1,925 TFLOP/s (2,447 on zeros), this loop without its loads 1,620 and with everything
+// 1,080-1,210; the library's product of 8,192^3 1,253.  Logits 1.45 ms, G 1.68 ms, dHidden and dWeight together 2.79 ms.
+// Measured there and not kept: 256 x 128 tiles, two workgroups a CU (64-byte rows: L2 delivers 26 of 55 bytes a clock and
+// CU), wave groups taking turns at LDS and matrix cores, a workgroup streaming through several tiles (no gain; not measured
+// with tiles of few slices, where power does not bind), four waves of 128 x 128 (registers spill), non-temporal stores of G
+// (1.6 times the time).
 //
 // float32 operands are two fp16 limbs, x 2^e = x1 + 2^-11 x2 with x1 and x2 rounded to 11 bits each, and e such that the
 // tensor's largest magnitude is just below 2^15: good to 2^-22 of every element down to 2^-29 of the largest, and to an
@@ -78,8 +80,7 @@ struct VgArgs {
     void* out;                  // direct output [N][ld_out] of the operand type (float32 for limbs)
     int64_t ld_out;
     const float* unscale;       // device factor of the outputs, or NULL
-    const int* exponents;       // limbs: e of the hidden states and of the weights
-    int exponent_of;            // which of the two the outputs carry
+    const int* exponents;       // limbs: e of the hidden states and of the weights; an output (dWeight) carries the first
 };
 
 enum { VG_LSE = 0, VG_GRAD = 1, VG_SLAB = 2, VG_OUT = 3 };
@@ -535,7 +536,7 @@ __device__ __forceinline__ void vg_tile(const VgArgs& p, int tm, int tn, int64_t
         constexpr int ROW = (F32 ? 512 : 256) + 16, LANES = F32 ? 32 : 16, E = 128 / LANES;     // lanes a row, elements a lane
         static_assert(2 * W * 16 * ROW <= vg_lds_bytes<WM, WN, WN == 4 ? 4 : NJ, NA>(), "LDS of the kernel");
         const float f = EPI == VG_OUT && p.unscale ? p.unscale[0] : 1.f;
-        const int e = EPI == VG_OUT && DT == LVAE_F32 ? -p.exponents[p.exponent_of] : 0;
+        const int e = EPI == VG_OUT && DT == LVAE_F32 ? -p.exponents[0] : 0;
         const int64_t m = m0 + wm * 128 + (lane % LANES) * E;
         const bool whole = m + E <= p.M;                // rows of any alignment: the stores need that of an element alone
 #pragma unroll
