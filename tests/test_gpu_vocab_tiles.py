@@ -106,3 +106,23 @@ def test_sequences_in_float16():
     out.backward(-gs.cuda())
     close(hc.grad, o["dh"].view(B, K, L, H), o["tol_dh"].view(B, K, L, H), "d_hidden")
     close(wc.grad, o["dw"], o["tol_dw"], "d_weight")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("T,V,H", [(20, 300, 64), (150, 500, 72), (2100, 300, 64), (700, 12000, 128)])
+def test_each_gradient_alone(dt, T, V, H):
+    """A frozen decoder, or frozen hidden states: what is asked for has the bits that it has beside the others."""
+    from lvae import decoder_ops as D
+    g = torch.Generator(device="cuda").manual_seed(T)
+    data = [torch.randn(T, H, device="cuda", generator=g).to(DT[dt]), (torch.randn(V, H, device="cuda", generator=g) / 8).to(DT[dt]),
+            torch.randn(V, device="cuda", generator=g)]
+    y = torch.randint(0, V, (T,), device="cuda", generator=g)
+    y[::7] = -100
+
+    def gradients(wanted):
+        ts = [t.clone().requires_grad_(k in wanted) for k, t in enumerate(data)]
+        return torch.autograd.grad(D.vocab_cross_entropy(ts[0], ts[1], y, ts[2]), [ts[k] for k in wanted])
+    whole = gradients((0, 1, 2))
+    for wanted in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        for k, got in zip(wanted, gradients(wanted)):
+            assert torch.equal(got, whole[k]), wanted
