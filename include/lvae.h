@@ -431,7 +431,9 @@ int lvae_dev_reload_env(void);
  * latent samples of a sentence (stride 0), are passed as they lie; the last axis of hidden and of weight is contiguous.
  * A token whose target is ignore_index has ll = 0 and no gradient, whatever its hidden state holds (NaN too).  Any other
  * target outside [0, V) makes ll, and every gradient that the token takes part in, NaN.  A bias of -inf bans a word.
- * All arithmetic accumulates in float32.  Limits of a call: V < 2^26, H <= 65,536, fewer than 2^27 tokens, tokens x H < 2^33,
+ * All arithmetic accumulates in float32.  LVAE_F32 calls of more than LVAE_VOCAB_FEW tokens, and their backward at any number,
+ * multiply operands of 22 bits (two fp16 limbs after scaling by a power of two of the tensor): elements below 2^-29 of the
+ * tensor's largest lose bits, those below 2^-51 of it count as 0.  Limits of a call: V < 2^26, H <= 65,536, fewer than 2^27 tokens, tokens x H < 2^33,
  * tokens x V < 2^38.
  * ------------------------------------------------------------------------------------------- */
 #define LVAE_F32 0
@@ -465,7 +467,7 @@ int lvae_vocab_ll(const lvae_vocab_problem* problem, float* ll, float* lse, void
 /* Backward: g is the upstream gradient on ll, over the token axes with strides g_stride (0: shared), times the device
  * scalar g_scale if that is given.  kept: that of the forward, or NULL.  d_hidden [tokens, H], d_weight [V, H]
  * (contiguous, dtype) and d_bias [V] (bias_dtype) may each be NULL.  The gradient of the logits exists a piece of the
- * vocabulary at a time, in the workspace (512 MiB, or 1,024 words), and is held relative to the largest finite |g|: with
+ * vocabulary at a time, in the workspace (512 MiB, or 1,024 words), and is held in the operands' type, relative to the largest finite |g|: with
  * LVAE_F16 and LVAE_F32 a token whose |g| is below 2^-28 of that loses bits of its own d_hidden.  Deterministic. */
 int lvae_vocab_ll_bwd_workspace_bytes(const lvae_vocab_problem* problem, int want_hidden, int want_weight, int want_bias,
                                       int64_t* out_bytes);

@@ -12,8 +12,13 @@ axis, so that the ``[B, L]`` words of a batch serve the ``[B, K, L, H]`` states 
 whatever their hidden state holds.  A target outside the vocabulary makes its result, and the gradients it takes part
 in, NaN.  A bias of -inf bans a word; hidden states and weights that count have to be finite.  Results are float32, held
 and summed in float32 or more; gradients come in the type of what they belong to, and can be taken once (no second
-derivatives; forward-mode tangents, torch.func transforms and tracing are refused).  The backward of float32 and float16 is held relative to the largest finite upstream gradient: a position
-whose own is below 2^-28 of that loses bits of its hidden state's gradient.
+derivatives; forward-mode tangents, torch.func transforms and tracing are refused).
+
+What is held in fewer bits: with bfloat16 and float16, the gradient of the logits is rounded to that type once, before the
+two products that make the gradients from it.  With float32, more than 64 tokens and any backward multiply operands of 22
+bits: an element of hidden, weight or the gradient of the logits below 2^-29 of the largest of its tensor loses bits, and
+below 2^-51 of it counts as 0.  The backward of float32 and float16 is held relative to the largest finite upstream
+gradient: a position whose own is below 2^-28 of that loses bits of its hidden state's gradient.
 """
 import ctypes
 

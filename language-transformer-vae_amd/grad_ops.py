@@ -1,6 +1,6 @@
 """The norm of all gradients together, and clipping by it: what a training step does between backward and update.
 
-Two launches a list of tensors (lvae_clip_grads) instead of several for each; the sum of squares is held in float64, and
+Two launches a list of tensors (lvae_clip_grads), and one more for every 112 of a longer one, instead of several for each; the sum of squares is held in float64, and
 gradients whose norm is within the bound are not touched.  float32, bfloat16 and float16 gradients may be mixed.
 Nothing is copied to or from the host.  Tensors with a forward-mode tangent, torch.func transforms and tracing are refused.
 """
